@@ -6,6 +6,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
+#include <vector>
+
 #include "ops.h"
 
 namespace {
@@ -25,11 +28,21 @@ int* status_ptr(const c10::optional<at::Tensor>& s) {
   return s->data_ptr<int>();
 }
 
+// a device row count (int32, one element) or null
+const int* count_ptr(const c10::optional<at::Tensor>& c, const at::Tensor& like) {
+  if (!c.has_value()) return nullptr;
+  TORCH_CHECK(c->scalar_type() == at::kInt && c->numel() == 1 && c->device() == like.device(),
+              "a device row count is one int32 on the operands' device");
+  return c->data_ptr<int>();
+}
+
 // C = alpha * op(A) op(B)^T (+ beta * D).
 // a: [M,K] (a_mn_major=false) or [K,M] (true); b: [N,K] or [K,N]; c: [M,N]
+// m_limit / k_limit: device counts of the rows of C / of the summed rows in use (splits 1)
 void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_major, at::Tensor& c,
           const c10::optional<at::Tensor>& d, double alpha, double beta, int64_t splits, int64_t bn,
-          const c10::optional<at::Tensor>& status) {
+          const c10::optional<at::Tensor>& status, const c10::optional<at::Tensor>& m_limit,
+          const c10::optional<at::Tensor>& k_limit) {
   check_cuda(a, "a");
   check_cuda(b, "b");
   check_cuda(c, "c");
@@ -69,6 +82,8 @@ void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_m
   p.allow_split = splits != 1;
   p.bn = static_cast<int>(bn);
   p.status = status_ptr(status);
+  p.m_limit = count_ptr(m_limit, a);
+  p.k_limit = count_ptr(k_limit, a);
   plg::gemm_bf16(p, cur_stream());
 }
 
@@ -378,6 +393,312 @@ void router_topk_b(const at::Tensor& logits, int64_t k, bool renorm, const c10::
                    probs.has_value() ? probs->data_ptr<float>() : nullptr, w.data_ptr<float>(),
                    idx.data_ptr<int64_t>(), counts.has_value() ? counts->data_ptr<int>() : nullptr,
                    cur_stream());
+}
+
+// ---- token log-probabilities of a linear head
+const int64_t* labels_ptr(const at::Tensor& labels) {
+  check_cuda(labels, "labels");
+  TORCH_CHECK(labels.scalar_type() == at::kLong && labels.is_contiguous(), "labels must be contiguous int64");
+  return labels.data_ptr<int64_t>();
+}
+
+int* int_ptr(const at::Tensor& t, int64_t n, const char* name) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() >= n, name,
+              " must be contiguous int32 with at least ", n, " elements");
+  return t.data_ptr<int>();
+}
+
+float* float_ptr(const at::Tensor& t, int64_t n, const char* name) {
+  check_cuda(t, name);
+  TORCH_CHECK(is_f32(t) && t.is_contiguous() && t.numel() >= n, name,
+              " must be contiguous fp32 with at least ", n, " elements");
+  return t.data_ptr<float>();
+}
+
+void head_compact_b(const at::Tensor& labels, int64_t V, int64_t ignore_index, at::Tensor& row_map,
+                    at::Tensor& inverse, at::Tensor& count, at::Tensor& out) {
+  const int64_t T = labels.numel();
+  TORCH_CHECK(T <= INT32_MAX - 256, "linear_token_logprobs: too many tokens in one call");
+  const c10::cuda::CUDAGuard guard(labels.device());
+  plg::head_compact(labels_ptr(labels), T, V, ignore_index, int_ptr(row_map, T, "row_map"),
+                    int_ptr(inverse, T, "inverse"), int_ptr(count, 1, "count"), float_ptr(out, T, "out"),
+                    cur_stream());
+}
+
+void head_gather_b(const at::Tensor& h, const at::Tensor& row_map, const at::Tensor& count, at::Tensor& out) {
+  check_cuda(h, "hidden");
+  TORCH_CHECK(h.dim() == 2 && h.stride(1) == 1 && (is_bf16(h) || is_f32(h)), "hidden must be [T, D] bf16 or fp32");
+  TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.dim() == 2 && out.size(1) == h.size(1) &&
+                  out.size(0) >= h.size(0), "head_gather: out must be contiguous bf16 [>= T, D]");
+  const c10::cuda::CUDAGuard guard(h.device());
+  plg::head_gather(h.data_ptr(), is_f32(h), h.stride(0), static_cast<int>(h.size(1)),
+                   int_ptr(row_map, h.size(0), "row_map"), int_ptr(count, 1, "count"), out.data_ptr(),
+                   static_cast<int>(out.size(0)), cur_stream());
+}
+
+plg::HeadProblem head_problem(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
+                              const c10::optional<at::Tensor>& row_map,
+                              const c10::optional<at::Tensor>& count, double softcap, double temperature,
+                              const c10::optional<at::Tensor>& status) {
+  check_cuda(h, "hidden");
+  check_cuda(w, "weight");
+  TORCH_CHECK(is_bf16(h) && is_bf16(w) && h.dim() == 2 && w.dim() == 2 && h.stride(1) == 1 &&
+                  w.stride(1) == 1 && h.size(1) == w.size(1),
+              "linear_token_logprobs: hidden [T, D] and weight [V, D] in bf16 with unit inner stride");
+  TORCH_CHECK(row_map.has_value() == count.has_value(), "linear_token_logprobs: row_map goes with count");
+  TORCH_CHECK(h.size(0) <= INT32_MAX - 256 && w.size(0) <= INT32_MAX - 256,
+              "linear_token_logprobs: too many rows in one call");
+  plg::HeadProblem p;
+  p.rows = static_cast<int>(h.size(0));
+  p.N = static_cast<int>(w.size(0));
+  p.D = static_cast<int>(h.size(1));
+  p.h = h.data_ptr();
+  p.ldh = h.stride(0);
+  p.w = w.data_ptr();
+  p.ldw = w.stride(0);
+  p.bn = plg::head_tile_n(p.rows, p.N);
+  p.labels = labels_ptr(labels);
+  if (row_map.has_value()) {
+    p.row_map = int_ptr(*row_map, labels.numel(), "row_map");
+    p.n_rows = count_ptr(count, h);
+  } else {
+    TORCH_CHECK(labels.numel() == p.rows, "linear_token_logprobs: one label per row");
+  }
+  p.softcap = static_cast<float>(softcap);
+  p.temperature = static_cast<float>(temperature);
+  p.status = status_ptr(status);
+  return p;
+}
+
+// out[token] = log-probability of its label; lse2 [rows] (optional) for the gradient
+void head_logprobs_b(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels, int64_t ignore_index,
+                     const c10::optional<at::Tensor>& row_map, const c10::optional<at::Tensor>& count,
+                     double softcap, double temperature, at::Tensor& out,
+                     const c10::optional<at::Tensor>& lse2, const c10::optional<at::Tensor>& status) {
+  const c10::cuda::CUDAGuard guard(h.device());
+  const plg::HeadProblem p = head_problem(h, w, labels, row_map, count, softcap, temperature, status);
+  const int64_t parts = 2 * ((p.N + p.bn - 1) / p.bn);
+  // workspace: the rows' (reference, sum) pairs and their labels' logits
+  at::Tensor part = at::empty({static_cast<int64_t>(p.rows) * (2 * parts + 1)}, out.options());
+  float* target = part.data_ptr<float>() + 2 * parts * p.rows;
+  plg::head_stats(p, part.data_ptr(), target, cur_stream());
+  plg::head_join(p, part.data_ptr(), target, p.N, ignore_index, float_ptr(out, labels.numel(), "out"),
+                 lse2.has_value() ? float_ptr(*lse2, p.rows, "lse2") : nullptr, cur_stream());
+}
+
+// g [rows, N] bf16 = gout[token] * d out / d logits of the vocabulary range starting at v0
+void head_grad_b(const at::Tensor& h, const at::Tensor& w, int64_t v0, const at::Tensor& labels,
+                 const at::Tensor& row_map, const at::Tensor& count, double softcap, double temperature,
+                 const at::Tensor& lse2, const at::Tensor& gout, at::Tensor& g,
+                 const c10::optional<at::Tensor>& status) {
+  const c10::cuda::CUDAGuard guard(h.device());
+  plg::HeadProblem p = head_problem(h, w, labels, row_map, count, softcap, temperature, status);
+  TORCH_CHECK(is_bf16(g) && g.dim() == 2 && g.size(0) == p.rows && g.size(1) == p.N && g.stride(1) == 1,
+              "head_grad: g must be bf16 [rows, N]");
+  p.label0 = v0;
+  plg::head_grad(p, float_ptr(lse2, p.rows, "lse2"), float_ptr(gout, labels.numel(), "gout"), g.data_ptr(),
+                 g.stride(0), cur_stream());
+}
+
+void head_scatter_b(const at::Tensor& src, const at::Tensor& inverse, at::Tensor& dh) {
+  check_cuda(dh, "dh");
+  TORCH_CHECK(dh.dim() == 2 && dh.is_contiguous() && (is_bf16(dh) || is_f32(dh)) && src.dim() == 2 &&
+                  src.size(1) == dh.size(1) && dh.size(1) % 8 == 0,
+              "head_scatter: dh contiguous [T, D] bf16 or fp32, src [rows, D]");
+  const c10::cuda::CUDAGuard guard(dh.device());
+  plg::head_scatter(float_ptr(src, src.numel(), "src"), int_ptr(inverse, dh.size(0), "inverse"),
+                    dh.data_ptr(), is_f32(dh), dh.size(0), static_cast<int>(dh.size(1)), cur_stream());
+}
+
+// ---- objectives over token log-probabilities and router logits
+// a [..., S] tensor whose last dimension is contiguous (any stride when S < 2)
+void check_tokens(const at::Tensor& t, at::IntArrayRef shape, const char* name) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
+  TORCH_CHECK(t.size(-1) < 2 || t.stride(-1) == 1, name, " must have contiguous tokens");
+}
+
+const uint8_t* mask_ptr(const at::Tensor& m) {
+  TORCH_CHECK(m.scalar_type() == at::kBool, "mask must be bool");
+  return reinterpret_cast<const uint8_t*>(m.data_ptr<bool>());
+}
+
+plg::PrefArgs pref_args(const at::Tensor& mask) {
+  TORCH_CHECK(mask.dim() == 3 && mask.size(0) == 2, "preference_loss: mask must be [2, P, S]");
+  check_tokens(mask, mask.sizes(), "mask");
+  TORCH_CHECK(mask.size(1) <= INT32_MAX / 2 && mask.size(2) <= INT32_MAX / 2, "preference_loss: too large");
+  plg::PrefArgs a;
+  a.mask = mask_ptr(mask);
+  a.mk_side = mask.stride(0);
+  a.mk_pair = mask.stride(1);
+  a.P = static_cast<int>(mask.size(1));
+  a.S = static_cast<int>(mask.size(2));
+  return a;
+}
+
+// out: fp32 [4 P + 1]: row_scale [2, P], rewards [2, P], loss
+void preference_fwd(const at::Tensor& logps, const c10::optional<at::Tensor>& ref, const at::Tensor& mask,
+                    int64_t kind, double beta, double smoothing, bool normalized, at::Tensor& out) {
+  const c10::cuda::CUDAGuard guard(mask.device());
+  plg::PrefArgs a = pref_args(mask);
+  check_tokens(logps, mask.sizes(), "logps");
+  TORCH_CHECK(is_f32(logps), "preference_loss: logps must be fp32");
+  a.logps = logps.data_ptr<float>();
+  a.lp_side = logps.stride(0);
+  a.lp_pair = logps.stride(1);
+  if (ref.has_value()) {
+    check_tokens(*ref, mask.sizes(), "ref_logps");
+    TORCH_CHECK(is_f32(*ref) || is_bf16(*ref), "preference_loss: ref_logps must be fp32 or bf16");
+    a.ref = ref->data_ptr();
+    a.ref_bf16 = is_bf16(*ref);
+    a.ref_side = ref->stride(0);
+    a.ref_pair = ref->stride(1);
+  }
+  a.kind = static_cast<int>(kind);
+  a.beta = static_cast<float>(beta);
+  a.smoothing = static_cast<float>(smoothing);
+  a.normalized = normalized;
+  float* o = float_ptr(out, 4LL * a.P + 1, "out");
+  // workspace: partial sums, block losses, ticket
+  const int64_t nb = plg::pref_blocks(a.P), np = 2LL * a.P * plg::pref_chunks(a.S);
+  at::Tensor ws = at::empty({8 * (np + nb + 1)}, mask.options().dtype(at::kByte));
+  char* w = static_cast<char*>(ws.data_ptr());
+  plg::pref_forward(a, w, reinterpret_cast<double*>(w + 8 * np), reinterpret_cast<unsigned*>(w + 8 * (np + nb)),
+                    o, o + 4LL * a.P, o + 2LL * a.P, cur_stream());
+}
+
+void preference_bwd(const at::Tensor& mask, const at::Tensor& row_scale, const at::Tensor& gout, at::Tensor& grad) {
+  const c10::cuda::CUDAGuard guard(mask.device());
+  const plg::PrefArgs a = pref_args(mask);
+  plg::pref_backward(a, float_ptr(row_scale, 2LL * a.P, "row_scale"), float_ptr(gout, 1, "gout"),
+                     float_ptr(grad, mask.numel(), "grad"), cur_stream());
+}
+
+// out: fp32 [3]: loss, mean KL, clipped share; grad [R, S] (optional)
+void policy_fwd(const at::Tensor& logps, const c10::optional<at::Tensor>& old, const at::Tensor& adv,
+                const at::Tensor& mask, const c10::optional<at::Tensor>& ref, double clip_low, double clip_high,
+                double kl_coef, bool by_sequence, const c10::optional<at::Tensor>& grad, at::Tensor& out) {
+  TORCH_CHECK(mask.dim() == 2, "policy_loss: mask must be [R, S]");
+  const c10::cuda::CUDAGuard guard(mask.device());
+  check_tokens(mask, mask.sizes(), "mask");
+  check_tokens(logps, mask.sizes(), "logps");
+  TORCH_CHECK(mask.size(0) <= INT32_MAX / 2 && mask.size(1) <= INT32_MAX / 2, "policy_loss: too large");
+  TORCH_CHECK(is_f32(logps), "policy_loss: logps must be fp32");
+  plg::PolicyArgs a;
+  a.R = static_cast<int>(mask.size(0));
+  a.S = static_cast<int>(mask.size(1));
+  a.mask = mask_ptr(mask);
+  a.mk_row = mask.stride(0);
+  a.logps = logps.data_ptr<float>();
+  a.lp_row = logps.stride(0);
+  if (old.has_value()) {
+    check_tokens(*old, mask.sizes(), "old_logps");
+    TORCH_CHECK(is_f32(*old) || is_bf16(*old), "policy_loss: old_logps must be fp32 or bf16");
+    a.old = old->data_ptr();
+    a.old_bf16 = is_bf16(*old);
+    a.old_row = old->stride(0);
+  }
+  if (ref.has_value()) {
+    check_tokens(*ref, mask.sizes(), "ref_logps");
+    TORCH_CHECK(is_f32(*ref) || is_bf16(*ref), "policy_loss: ref_logps must be fp32 or bf16");
+    a.ref = ref->data_ptr();
+    a.ref_bf16 = is_bf16(*ref);
+    a.ref_row = ref->stride(0);
+  }
+  check_cuda(adv, "advantages");
+  TORCH_CHECK(is_f32(adv) && (adv.dim() == 1 || adv.dim() == 2) && adv.size(0) == a.R,
+              "policy_loss: advantages must be fp32 [R] or [R, S]");
+  if (adv.dim() == 2) {
+    check_tokens(adv, mask.sizes(), "advantages");
+    a.adv_tok = 1;
+  }
+  a.adv = adv.data_ptr<float>();
+  a.adv_row = adv.stride(0);
+  a.hi = static_cast<float>(1.0 + clip_high);
+  a.lo = static_cast<float>(1.0 - clip_low);
+  a.log_hi = static_cast<float>(std::log1p(clip_high));
+  a.log_lo = static_cast<float>(std::log1p(-clip_low));
+  a.kl_coef = static_cast<float>(kl_coef);
+  a.by_sequence = by_sequence;
+  // workspace: block counts, block sums, row counts, ticket
+  const int64_t cb = plg::policy_count_blocks(a.R, a.S), sb = plg::policy_blocks(a.R, a.S);
+  at::Tensor ws = at::empty({16 * cb + 24 * sb + 4LL * a.R + 4}, mask.options().dtype(at::kByte));
+  char* w = static_cast<char*>(ws.data_ptr());
+  int* counts = reinterpret_cast<int*>(w + 16 * cb + 24 * sb);
+  plg::policy_forward(a, counts, w, reinterpret_cast<double*>(w + 16 * cb),
+                      reinterpret_cast<unsigned*>(counts + a.R),
+                      grad.has_value() ? float_ptr(*grad, mask.numel(), "grad") : nullptr,
+                      float_ptr(out, 3, "out"), cur_stream());
+}
+
+void scale_unless_one_b(at::Tensor& x, const at::Tensor& s) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  plg::scale_unless_one(float_ptr(x, x.numel(), "x"), x.numel(), float_ptr(s, 1, "s"), cur_stream());
+}
+
+plg::RouterArgs router_args(const std::vector<at::Tensor>& logits, const std::vector<at::Tensor>& idx,
+                            const c10::optional<at::Tensor>& mask) {
+  TORCH_CHECK(!logits.empty() && logits.size() <= plg::kRouterMaxLayers && idx.size() == logits.size(),
+              "router_balance_loss: 1..", plg::kRouterMaxLayers, " layers, one index tensor for each");
+  plg::RouterArgs a{};
+  const at::Tensor& x0 = logits[0];
+  check_cuda(x0, "router_logits");
+  TORCH_CHECK(x0.dim() == 2 && idx[0].dim() == 2, "router_balance_loss: logits [T, E] and indices [T, k]");
+  a.L = static_cast<int>(logits.size());
+  a.T = x0.size(0);
+  a.E = static_cast<int>(x0.size(1));
+  a.k = static_cast<int>(idx[0].size(1));
+  for (int l = 0; l < a.L; ++l) {
+    const at::Tensor &x = logits[l], &i = idx[l];
+    TORCH_CHECK(x.device() == x0.device() && x.sizes() == x0.sizes() && x.scalar_type() == x0.scalar_type() &&
+                    (is_bf16(x) || is_f32(x)) && (x.stride(1) == 1 || a.E == 1),
+                "router_balance_loss: the layers' logits must be bf16 or fp32 [T, E], alike");
+    TORCH_CHECK(i.device() == x0.device() && i.scalar_type() == at::kLong && i.is_contiguous() && i.dim() == 2 &&
+                    i.size(0) == a.T && i.size(1) == a.k,
+                "router_balance_loss: indices must be contiguous int64 [T, k], alike");
+    a.logits[l] = x.data_ptr();
+    a.ld[l] = x.stride(0);
+    a.idx[l] = i.data_ptr<int64_t>();
+  }
+  if (mask.has_value()) {
+    check_tokens(*mask, {a.T}, "mask");
+    TORCH_CHECK(mask->is_contiguous(), "mask must be contiguous");
+    a.mask = mask_ptr(*mask);
+  }
+  return a;
+}
+
+// out: fp32 [E + 2]: slope [E + 1], loss; lse [L, T]; counts int64 [E]
+void router_balance_fwd(const std::vector<at::Tensor>& logits, const std::vector<at::Tensor>& idx,
+                        const c10::optional<at::Tensor>& mask, double balance, double zcoef, at::Tensor& lse,
+                        at::Tensor& counts, at::Tensor& out) {
+  const c10::cuda::CUDAGuard guard(lse.device());
+  const plg::RouterArgs a = router_args(logits, idx, mask);
+  TORCH_CHECK(counts.is_cuda() && counts.scalar_type() == at::kLong && counts.is_contiguous() &&
+                  counts.numel() == a.E, "router_balance_loss: counts must be int64 [E]");
+  float* o = float_ptr(out, a.E + 2, "out");
+  const int64_t blocks = plg::router_blocks(a.L * a.T);
+  at::Tensor ws = at::empty({blocks * (16 + 8LL * a.E)}, lse.options().dtype(at::kByte));
+  char* w = static_cast<char*>(ws.data_ptr());
+  float* pp = reinterpret_cast<float*>(w + 16 * blocks);
+  plg::router_balance_forward(a, is_bf16(logits[0]), static_cast<float>(balance), static_cast<float>(zcoef),
+                              float_ptr(lse, a.L * a.T, "lse"), pp, reinterpret_cast<int*>(pp + blocks * a.E),
+                              reinterpret_cast<double*>(w), o + a.E + 1, counts.data_ptr<int64_t>(), o,
+                              cur_stream());
+}
+
+void router_balance_bwd(const std::vector<at::Tensor>& logits, const std::vector<at::Tensor>& idx,
+                        const c10::optional<at::Tensor>& mask, const at::Tensor& lse, const at::Tensor& slope,
+                        const at::Tensor& gout, at::Tensor& grad) {
+  const c10::cuda::CUDAGuard guard(lse.device());
+  const plg::RouterArgs a = router_args(logits, idx, mask);
+  check_cuda(grad, "grad");
+  TORCH_CHECK(grad.is_contiguous() && grad.scalar_type() == logits[0].scalar_type() &&
+                  grad.numel() == a.L * a.T * a.E, "router_balance_loss: grad must be [L, T, E] in the logits' type");
+  plg::router_balance_backward(a, is_bf16(logits[0]), float_ptr(lse, a.L * a.T, "lse"),
+                               float_ptr(slope, a.E + 1, "slope"), float_ptr(gout, 1, "gout"), grad.data_ptr(),
+                               cur_stream());
 }
 
 void exp2_poly_eval_b(const at::Tensor& x, at::Tensor& poly, at::Tensor& ref) {
@@ -842,7 +1163,20 @@ void set_peer_wait_deadline(int64_t ns) {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "pluggy_b200 sm_100a kernels";
-  m.def("gemm", &gemm);
+  m.def("gemm", &gemm, py::arg("a"), py::arg("a_mn_major"), py::arg("b"), py::arg("b_mn_major"),
+        py::arg("c"), py::arg("d"), py::arg("alpha"), py::arg("beta"), py::arg("splits"), py::arg("bn"),
+        py::arg("status"), py::arg("m_limit") = py::none(), py::arg("k_limit") = py::none());
+  m.def("preference_fwd", &preference_fwd);
+  m.def("preference_bwd", &preference_bwd);
+  m.def("policy_fwd", &policy_fwd);
+  m.def("scale_unless_one", &scale_unless_one_b);
+  m.def("router_balance_fwd", &router_balance_fwd);
+  m.def("router_balance_bwd", &router_balance_bwd);
+  m.def("head_compact", &head_compact_b);
+  m.def("head_gather", &head_gather_b);
+  m.def("head_logprobs", &head_logprobs_b);
+  m.def("head_grad", &head_grad_b);
+  m.def("head_scatter", &head_scatter_b);
   m.def("gemm_grouped", &gemm_grouped, py::arg("a"), py::arg("b"), py::arg("b_mn_major"), py::arg("c"),
         py::arg("mode"), py::arg("table"), py::arg("groups"), py::arg("b_rows"), py::arg("alpha"),
         py::arg("beta"), py::arg("status") = py::none());

@@ -65,7 +65,18 @@ struct Args {
   const int* grp_koff;   // mode 2: [groups + 1] row offsets of the k ranges (multiples of BK)
   long long grp_c_rows;  // mode 2: rows of C per group (C is [groups * M, N])
   int grp_count;         // mode 2: number of groups
+  const int* m_limit;    // device row count of C (null: M)
+  const int* k_limit;    // device length of the sum (null: K)
 };
+
+// m tiles and k blocks in use under the device limits
+__device__ __forceinline__ void limited_extent(const Args& args, int tile_m, int& m_tiles,
+                                               int& k_blocks) {
+  m_tiles = args.m_tiles;
+  k_blocks = args.k_blocks;
+  if (args.m_limit != nullptr) m_tiles = min(m_tiles, (max(*args.m_limit, 0) + tile_m - 1) / tile_m);
+  if (args.k_limit != nullptr) k_blocks = min(k_blocks, (max(*args.k_limit, 0) + BK - 1) / BK);
+}
 
 // destination of row `row` under the reduce-scatter epilogue; static indices only
 // (a dynamically indexed kernel parameter would be copied to local memory)
@@ -301,9 +312,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_smem;
 
-  const int total_tiles = args.m_tiles * args.n_tiles;
+  int m_tiles, k_blocks;
+  limited_extent(args, BM, m_tiles, k_blocks);
+  const int total_tiles = m_tiles * args.n_tiles;
   const int total_work = total_tiles * (args.grp_mode == 2 ? args.grp_count : args.splits);
-  const int kb_per_split = (args.k_blocks + args.splits - 1) / args.splits;
+  const int kb_per_split = (k_blocks + args.splits - 1) / args.splits;
 
   // work unit -> tile (mt, nt), k-block range and group g; false: no work (mode 1
   // m tile beyond the last group). Every role decodes the same units.
@@ -318,20 +331,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       sp = w - tile * args.splits;
     }
     if (args.raster_m) {
-      mt = tile % args.m_tiles;
-      nt = tile / args.m_tiles;
+      mt = tile % m_tiles;
+      nt = tile / m_tiles;
     } else {
       nt = tile % args.n_tiles;
       mt = tile / args.n_tiles;
     }
-    if (args.rs_mshift) mt = (mt + args.rs_mshift) % args.m_tiles;
+    if (args.rs_mshift) mt = (mt + args.rs_mshift) % m_tiles;
     if (args.grp_mode == 2) {
       kb0 = args.grp_koff[g] / BK;
       kb1 = args.grp_koff[g + 1] / BK;
       return true;
     }
     kb0 = sp * kb_per_split;
-    kb1 = min(args.k_blocks, kb0 + kb_per_split);
+    kb1 = min(k_blocks, kb0 + kb_per_split);
     if (args.grp_mode == 1) {
       g = args.grp_tile[mt];
       return g >= 0;
@@ -564,22 +577,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_smem;
 
-  const int total_tiles = args.m_tiles * args.n_tiles;  // 256 x 256 tiles
+  int m_tiles, k_blocks;
+  limited_extent(args, 2 * BM, m_tiles, k_blocks);
+  const int total_tiles = m_tiles * args.n_tiles;  // 256 x 256 tiles
   const int total_work = total_tiles * args.splits;
-  const int kb_per_split = (args.k_blocks + args.splits - 1) / args.splits;
+  const int kb_per_split = (k_blocks + args.splits - 1) / args.splits;
   auto decode = [&](int w, int& mt, int& nt, int& kb0, int& kb1) {
     const int tile = w / args.splits;
     const int sp = w - tile * args.splits;
     if (args.raster_m) {
-      mt = tile % args.m_tiles;
-      nt = tile / args.m_tiles;
+      mt = tile % m_tiles;
+      nt = tile / m_tiles;
     } else {
       nt = tile % args.n_tiles;
       mt = tile / args.n_tiles;
     }
-    if (args.rs_mshift) mt = (mt + args.rs_mshift) % args.m_tiles;
+    if (args.rs_mshift) mt = (mt + args.rs_mshift) % m_tiles;
     kb0 = sp * kb_per_split;
-    kb1 = min(args.k_blocks, kb0 + kb_per_split);
+    kb1 = min(k_blocks, kb0 + kb_per_split);
   };
 
   if (warp == 0) {
@@ -717,7 +732,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const long long row = (long long)mt * 2 * BM + rank * BM + row_in_tile;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
-      store_acc_row<BN>(args, t_row, row, row < args.M, nt * BN, kb0, epi_stage + q * 32 * 128);
+      store_acc_row<BN>(args, t_row, row, row < args.M, nt * BN, kb0, epi_stage + q * 32 * 128,
+                        kb1 <= kb0);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(&acce_bar[buf], 0);
@@ -832,6 +848,8 @@ static void launch(const GemmProblem& p, cudaStream_t stream) {
   a.n_tiles = (p.N + BN - 1) / BN;
   a.k_blocks = (p.K + BK - 1) / BK;
   a.status = p.status;
+  a.m_limit = p.m_limit;
+  a.k_limit = p.k_limit;
   set_rs_fields(p, a, BM);
   a.grp_mode = p.grp_mode;
   a.grp_tile = p.grp_tile;
@@ -891,6 +909,8 @@ static void launch_pair(const GemmProblem& p, cudaStream_t stream) {
   a.n_tiles = (p.N + BN - 1) / BN;
   a.k_blocks = (p.K + BK - 1) / BK;
   a.status = p.status;
+  a.m_limit = p.m_limit;
+  a.k_limit = p.k_limit;
   set_rs_fields(p, a, 2 * BM);
   auto kern = gemm_pair_kernel<A_MN, B_MN>;
   set_max_smem_once(reinterpret_cast<const void*>(kern), C_::kSmemBytes);
@@ -963,6 +983,8 @@ void gemm_bf16(const GemmProblem& p, cudaStream_t stream) {
     if (p.grp_mode == 2 && p.D != nullptr && p.D != p.C)
       throw std::invalid_argument("gemm grouped mode 2: the addend can only be C itself");
   }
+  if ((p.m_limit != nullptr || p.k_limit != nullptr) && (p.grp_mode || p.rs_n || p.allow_split))
+    throw std::invalid_argument("gemm: device row counts need an ungrouped product without split-K");
   const bool wide = p.N >= 256 && p.bn != 128;
   // large problems: 256 x 256 tiles on SM pairs (bn == 256 keeps the one-SM kernel)
   const bool pair = wide && p.bn == 0 && p.M >= 256 && num_sms() >= 2 && !p.grp_mode;

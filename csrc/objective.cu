@@ -1,0 +1,879 @@
+// Losses over per-token log-probabilities (paired preference loss, clipped policy loss with
+// a KL term) and over MoE router logits (balance and z loss), forward and backward.
+//
+// All of them stream their inputs once and are bound by memory (or, at a few thousand
+// tokens, by launch latency). Every sum runs in a fixed order: per-warp or per-block
+// partial sums go to a workspace and one block joins them, so results repeat bit for bit.
+// Masked places are skipped by selection, never by a product with 0, so that whatever they
+// hold (infinities, NaN) reaches neither a loss nor a gradient.
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+#include "common.cuh"
+#include "ops.h"
+
+namespace plg {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kWarpTokens = 1024;  // tokens of one row that a warp takes at a time
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_f(const float* p, float (&v)[VEC]) {
+  if (VEC == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+    v[0] = *p;
+  }
+}
+
+// VEC values at element `i` of an fp32 or bf16 row
+template <int VEC>
+__device__ __forceinline__ void load_any(const void* p, bool bf16, long long i, float (&v)[VEC]) {
+  if (!bf16) {
+    load_f<VEC>(static_cast<const float*>(p) + i, v);
+  } else if (VEC == 4) {
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i);
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+  } else {
+    v[0] = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_mask(const uint8_t* p, bool (&m)[VEC]) {
+  if (VEC == 4) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) m[j] = ((u >> (8 * j)) & 0xffu) != 0;
+  } else {
+    m[0] = *p != 0;
+  }
+}
+
+// ------------------------------------------------------------------ preference loss
+// Row r = side * P + pair of [2, P, S] tensors.
+template <int VEC>
+__global__ void __launch_bounds__(256) pref_sums_kernel(const PrefArgs a, float2* __restrict__ part,
+                                                        int chunks, unsigned* __restrict__ ticket) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+  const int lane = threadIdx.x & 31;
+  const long long units = 2LL * a.P * chunks;
+  const long long nw = static_cast<long long>(gridDim.x) * 8;
+  for (long long u = blockIdx.x * 8LL + (threadIdx.x >> 5); u < units; u += nw) {
+    const long long r = u / chunks;
+    const int t0 = static_cast<int>(u - r * chunks) * kWarpTokens;
+    const int t1 = min(a.S, t0 + kWarpTokens);
+    const int side = r >= a.P ? 1 : 0;
+    const long long pair = r - static_cast<long long>(side) * a.P;
+    const float* lp = a.logps + side * a.lp_side + pair * a.lp_pair;
+    const long long ro = side * a.ref_side + pair * a.ref_pair;
+    const uint8_t* mk = a.mask + side * a.mk_side + pair * a.mk_pair;
+    float s = 0.f;
+    int n = 0;
+#pragma unroll 4
+    for (int t = t0 + lane * VEC; t < t1; t += 32 * VEC) {
+      float x[VEC], y[VEC];
+      bool m[VEC];
+      load_f<VEC>(lp + t, x);
+      load_mask<VEC>(mk + t, m);
+      if (a.ref != nullptr) {
+        load_any<VEC>(a.ref, a.ref_bf16, ro + t, y);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] -= y[j];
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        s += m[j] ? x[j] : 0.f;
+        n += m[j] ? 1 : 0;
+      }
+    }
+    s = warp_sum(s);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) part[u] = make_float2(s, __int_as_float(n));
+  }
+}
+
+// One warp per pair joins its chunks; the last block sums the blocks' losses.
+//   h = s_0 - s_1;  sigmoid: (1 - eps) softplus(-b h) + eps softplus(b h);
+//   hinge: max(0, 1 - b h);  ipo: (h - 1 / (2 b))^2
+__global__ void __launch_bounds__(256) pref_pairs_kernel(const PrefArgs a, const float2* __restrict__ part,
+                                                         int chunks, double* __restrict__ block_loss,
+                                                         unsigned* __restrict__ ticket,
+                                                         float* __restrict__ row_scale,
+                                                         float* __restrict__ loss,
+                                                         float* __restrict__ rewards) {
+  __shared__ double s_loss[8];
+  __shared__ bool s_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double acc = 0.0;
+  for (long long i = blockIdx.x * 8LL + warp; i < a.P; i += gridDim.x * 8LL) {
+    double s[2];
+    float inv[2];
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const float2* p = part + (side * static_cast<long long>(a.P) + i) * chunks;
+      double t = 0.0;
+      long long n = 0;
+      for (int c = lane; c < chunks; c += 32) {
+        const float2 v = p[c];
+        t += v.x;
+        n += __float_as_int(v.y);
+      }
+      t = warp_sum_d(t);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      inv[side] = a.normalized && n > 1 ? 1.f / static_cast<float>(n) : 1.f;
+      s[side] = a.normalized && n > 1 ? t / static_cast<double>(n) : t;
+    }
+    const float h = static_cast<float>(s[0] - s[1]);
+    float l, d;  // loss and dloss / dh
+    if (a.kind == 0) {
+      const float x = a.beta * h;
+      const float soft = log1pf(expf(-fabsf(x)));
+      l = (1.f - a.smoothing) * (soft + fmaxf(-x, 0.f));
+      if (a.smoothing > 0.f) l += a.smoothing * (soft + fmaxf(x, 0.f));
+      // d softplus(-x) = -sigmoid(-x), d softplus(x) = sigmoid(x)
+      const float e = expf(-fabsf(x)), r = 1.f / (1.f + e);
+      const float sig = x >= 0.f ? r : e * r, sig_neg = x >= 0.f ? e * r : r;
+      d = a.beta * (a.smoothing * sig - (1.f - a.smoothing) * sig_neg);
+    } else if (a.kind == 1) {
+      const float x = 1.f - a.beta * h;
+      l = x > 0.f ? x : (x <= 0.f ? 0.f : x);  // NaN stays NaN
+      d = x > 0.f ? -a.beta : (x <= 0.f ? 0.f : x);
+    } else {
+      const float x = h - 0.5f / a.beta;
+      l = x * x;
+      d = 2.f * x;
+    }
+    if (lane == 0) {
+      const float c = d / static_cast<float>(a.P);
+      row_scale[i] = c * inv[0];
+      row_scale[a.P + i] = -c * inv[1];
+      rewards[i] = static_cast<float>(a.beta * s[0]);
+      rewards[a.P + i] = static_cast<float>(a.beta * s[1]);
+      acc += l;
+    }
+  }
+  if (lane == 0) s_loss[warp] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int w = 0; w < 8; ++w) t += s_loss[w];
+    block_loss[blockIdx.x] = t;
+    __threadfence();
+    s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (s_last && warp == 0) {
+    __threadfence();
+    double t = 0.0;
+    for (int b = lane; b < gridDim.x; b += 32) t += static_cast<volatile double*>(block_loss)[b];
+    t = warp_sum_d(t);
+    if (lane == 0) *loss = static_cast<float>(t / a.P);
+  }
+}
+
+// grad[r, t] = gout * row_scale[r] where the mask holds, else 0 (contiguous [2, P, S])
+template <int VEC>
+__global__ void __launch_bounds__(256) pref_grad_kernel(const PrefArgs a, const float* __restrict__ row_scale,
+                                                        const float* __restrict__ gout,
+                                                        float* __restrict__ grad, int chunks) {
+  const int lane = threadIdx.x & 31;
+  const long long units = 2LL * a.P * chunks;
+  const long long nw = static_cast<long long>(gridDim.x) * 8;
+  const float g = *gout;
+  for (long long u = blockIdx.x * 8LL + (threadIdx.x >> 5); u < units; u += nw) {
+    const long long r = u / chunks;
+    const int t0 = static_cast<int>(u - r * chunks) * kWarpTokens;
+    const int t1 = min(a.S, t0 + kWarpTokens);
+    const int side = r >= a.P ? 1 : 0;
+    const uint8_t* mk = a.mask + side * a.mk_side + (r - static_cast<long long>(side) * a.P) * a.mk_pair;
+    const float c = g * row_scale[r];
+    float* out = grad + r * a.S;
+#pragma unroll 4
+    for (int t = t0 + lane * VEC; t < t1; t += 32 * VEC) {
+      bool m[VEC];
+      load_mask<VEC>(mk + t, m);
+      if (VEC == 4)
+        *reinterpret_cast<float4*>(out + t) =
+            make_float4(m[0] ? c : 0.f, m[1 % VEC] ? c : 0.f, m[2 % VEC] ? c : 0.f, m[3 % VEC] ? c : 0.f);
+      else
+        out[t] = m[0] ? c : 0.f;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------- policy loss
+// counts[r] = tokens of row r; block_counts[b] = (tokens, rows with any) of block b's rows.
+// A row is counted by one warp, or by the whole block when rows are long.
+template <bool BLOCK_ROW>
+__global__ void __launch_bounds__(256) policy_counts_kernel(const PolicyArgs a, int* __restrict__ counts,
+                                                            longlong2* __restrict__ block_counts,
+                                                            unsigned* __restrict__ ticket) {
+  __shared__ int s_n[8];
+  __shared__ long long s_tok[8];
+  __shared__ int s_rows[8];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = BLOCK_ROW ? threadIdx.x : lane;
+  constexpr int kGroup = BLOCK_ROW ? 256 : 32;
+  constexpr int kRows = BLOCK_ROW ? 1 : 8;
+  long long tokens = 0;
+  int rows = 0;
+  for (long long r0 = blockIdx.x * static_cast<long long>(kRows); r0 < a.R; r0 += gridDim.x * static_cast<long long>(kRows)) {
+    const long long r = r0 + (BLOCK_ROW ? 0 : warp);
+    int n = 0;
+    if (r < a.R) {
+      const uint8_t* mk = a.mask + r * a.mk_row;
+      // bytes up to the first 16-byte boundary, 16 at a time, then the rest
+      const int head = min(a.S, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(mk) & 15)) & 15));
+      const int vecs = (a.S - head) / 16;
+      for (int t = sub; t < head; t += kGroup) n += mk[t] != 0;
+      const uint4* mv = reinterpret_cast<const uint4*>(mk + head);
+#pragma unroll 4
+      for (int i = sub; i < vecs; i += kGroup) {
+        const uint4 u = mv[i];
+        // a bool tensor's bytes are 0 or 1, but any nonzero byte counts once
+        n += __popc(__vcmpne4(u.x, 0) & 0x01010101u) + __popc(__vcmpne4(u.y, 0) & 0x01010101u) +
+             __popc(__vcmpne4(u.z, 0) & 0x01010101u) + __popc(__vcmpne4(u.w, 0) & 0x01010101u);
+      }
+      for (int t = head + vecs * 16 + sub; t < a.S; t += kGroup) n += mk[t] != 0;
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (BLOCK_ROW) {
+      __syncthreads();
+      if (lane == 0) s_n[warp] = n;
+      __syncthreads();
+      n = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) n += s_n[w];
+    }
+    if (r < a.R && (BLOCK_ROW ? threadIdx.x : lane) == 0) {
+      counts[r] = n;
+      tokens += n;
+      rows += n > 0;
+    }
+  }
+  if (lane == 0) {
+    s_tok[warp] = tokens;
+    s_rows[warp] = rows;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) {
+      tokens += s_tok[w];
+      rows += s_rows[w];
+    }
+    block_counts[blockIdx.x] = make_longlong2(tokens, rows);
+  }
+}
+
+// e^d - 1 - d: the KL term per token. For small d the difference cancels, so its Taylor
+// series is summed instead (|d| < 1/4: the first dropped term is below 1e-8 of the result).
+__device__ __forceinline__ float kl_term(float d, float em1) {
+  if (fabsf(d) >= 0.25f) return em1 - d;
+  float p = 1.f / 5040.f;
+  p = fmaf(p, d, 1.f / 720.f);
+  p = fmaf(p, d, 1.f / 120.f);
+  p = fmaf(p, d, 1.f / 24.f);
+  p = fmaf(p, d, 1.f / 6.f);
+  p = fmaf(p, d, 0.5f);
+  return d * d * p;
+}
+
+// Per token, with r = logps - old and d = ref - logps:
+//   loss = -A e^r (the bound instead of e^r once A pushes r past it) + kl_coef (e^d - 1 - d)
+//   grad = -A e^r (0 past the bound) - kl_coef (e^d - 1)
+// each times the token's weight in the mean, known from the counts.
+template <int VEC>
+__global__ void __launch_bounds__(256) policy_kernel(const PolicyArgs a, const int* __restrict__ counts,
+                                                     const longlong2* __restrict__ block_counts, int nblocks,
+                                                     double* __restrict__ block_sums,
+                                                     unsigned* __restrict__ ticket, float* __restrict__ grad,
+                                                     float* __restrict__ out, int chunks) {
+  __shared__ long long s_cnt[2][8];
+  __shared__ double s_sum[3][8];
+  __shared__ bool s_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long tokens = 0, rows = 0;
+  for (int b = threadIdx.x; b < nblocks; b += 256) {
+    const longlong2 v = block_counts[b];
+    tokens += v.x;
+    rows += v.y;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+    rows += __shfl_xor_sync(0xffffffffu, rows, o);
+  }
+  if (lane == 0) {
+    s_cnt[0][warp] = tokens;
+    s_cnt[1][warp] = rows;
+  }
+  __syncthreads();
+  tokens = rows = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    tokens += s_cnt[0][w];
+    rows += s_cnt[1][w];
+  }
+  const double inv_tokens = 1.0 / static_cast<double>(tokens > 0 ? tokens : 1);
+  const double inv_rows = 1.0 / static_cast<double>(rows > 0 ? rows : 1);
+
+  double loss = 0.0, kl = 0.0, clipped = 0.0;
+  const long long units = static_cast<long long>(a.R) * chunks;
+  const long long nw = static_cast<long long>(gridDim.x) * 8;
+  for (long long u = blockIdx.x * 8LL + warp; u < units; u += nw) {
+    const long long r = u / chunks;
+    const int t0 = static_cast<int>(u - r * chunks) * kWarpTokens;
+    const int t1 = min(a.S, t0 + kWarpTokens);
+    const float* lp = a.logps + r * a.lp_row;
+    const uint8_t* mk = a.mask + r * a.mk_row;
+    const float row_adv = a.adv_tok == 0 ? a.adv[r * a.adv_row] : 0.f;
+    const float w = static_cast<float>(a.by_sequence ? inv_rows / max(counts[r], 1) : inv_tokens);
+    float sl = 0.f, sk = 0.f;
+    int sc = 0;
+#pragma unroll 2
+    for (int t = t0 + lane * VEC; t < t1; t += 32 * VEC) {
+      float x[VEC], o[VEC], f[VEC], A[VEC], g[VEC];
+      bool m[VEC];
+      load_f<VEC>(lp + t, x);
+      load_mask<VEC>(mk + t, m);
+      if (a.old != nullptr) load_any<VEC>(a.old, a.old_bf16, r * a.old_row + t, o);
+      if (a.ref != nullptr) load_any<VEC>(a.ref, a.ref_bf16, r * a.ref_row + t, f);
+      if (a.adv_tok != 0) load_f<VEC>(a.adv + r * a.adv_row + t, A);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float adv = a.adv_tok != 0 ? A[j] : row_adv;
+        const float lr = a.old != nullptr ? x[j] - o[j] : 0.f;
+        const float ratio = a.old != nullptr ? expf(lr) : 1.f;
+        const bool up = adv > 0.f && lr > a.log_hi, dn = adv < 0.f && lr < a.log_lo;
+        float l = -(up ? a.hi : dn ? a.lo : ratio) * adv;
+        float d = (up || dn) ? 0.f : -adv * ratio;
+        if (a.ref != nullptr) {
+          const float df = f[j] - x[j], em1 = expm1f(df), k3 = kl_term(df, em1);
+          sk += m[j] ? k3 : 0.f;
+          l = fmaf(a.kl_coef, k3, l);
+          d = fmaf(-a.kl_coef, em1, d);
+        }
+        sl += m[j] ? l : 0.f;
+        sc += (m[j] && (up || dn)) ? 1 : 0;
+        g[j] = m[j] ? d * w : 0.f;
+      }
+      if (grad != nullptr) {
+        float* gp = grad + r * a.S + t;
+        if (VEC == 4)
+          *reinterpret_cast<float4*>(gp) = make_float4(g[0], g[1 % VEC], g[2 % VEC], g[3 % VEC]);
+        else
+          *gp = g[0];
+      }
+    }
+    loss += static_cast<double>(sl) * w;
+    kl += sk;
+    clipped += sc;
+  }
+  loss = warp_sum_d(loss);
+  kl = warp_sum_d(kl);
+  clipped = warp_sum_d(clipped);
+  if (lane == 0) {
+    s_sum[0][warp] = loss;
+    s_sum[1][warp] = kl;
+    s_sum[2][warp] = clipped;
+  }
+  __syncthreads();
+  if (threadIdx.x < 3) {
+    double t = 0.0;
+    for (int w = 0; w < 8; ++w) t += s_sum[threadIdx.x][w];
+    block_sums[blockIdx.x * 3 + threadIdx.x] = t;
+    __threadfence();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (s_last && warp < 3) {
+    __threadfence();
+    double t = 0.0;
+    for (int b = lane; b < gridDim.x; b += 32) t += static_cast<volatile double*>(block_sums)[b * 3 + warp];
+    t = warp_sum_d(t);
+    if (lane == 0) out[warp] = static_cast<float>(warp == 0 ? t : t * inv_tokens);
+  }
+}
+
+// x *= *s, unless *s is 1 (the usual gradient of a loss): then nothing is read or written
+template <int VEC>
+__global__ void __launch_bounds__(256) scale_unless_one_kernel(float* __restrict__ x, long long n,
+                                                               const float* __restrict__ s) {
+  const float c = *s;
+  if (c == 1.f) return;
+  const long long step = static_cast<long long>(gridDim.x) * 256 * VEC;
+  for (long long i = (blockIdx.x * 256LL + threadIdx.x) * VEC; i < n; i += step) {
+    if (VEC == 4 && i + 4 <= n) {
+      float4 v = *reinterpret_cast<float4*>(x + i);
+      v.x *= c; v.y *= c; v.z *= c; v.w *= c;
+      *reinterpret_cast<float4*>(x + i) = v;
+    } else {
+      for (long long j = i; j < min(n, i + VEC); ++j) x[j] *= c;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------ MoE router
+// A row of E logits is held by a group of G lanes, NV vectors of VEC per lane (column
+// (v G + lane) VEC + j). One row then costs log2(G) shuffle steps shared by 32 / G rows.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+template <typename T, int VEC, int G, int NV>
+__device__ __forceinline__ void load_row(const T* p, int sub, int E, float (&x)[NV * VEC]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * G + sub) * VEC;
+    if (c < E) {  // E is a multiple of VEC
+      const Pack<T, VEC> u = *reinterpret_cast<const Pack<T, VEC>*>(p + c);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[v * VEC + j] = static_cast<float>(u.v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[v * VEC + j] = -INFINITY;
+    }
+  }
+}
+
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+constexpr int kRouterThreads = 512;
+
+// Per block: column sums of the probabilities, the sum of lse^2, the kept tokens and the
+// histogram of the chosen experts over the block's rows; lse of every row for the backward.
+template <typename T, int VEC, int G, int NV>
+__global__ void __launch_bounds__(kRouterThreads) router_sums_kernel(const __grid_constant__ RouterArgs a,
+                                                                     float* __restrict__ lse_out,
+                                                                     float* __restrict__ part_p,
+                                                                     int* __restrict__ part_n,
+                                                                     double* __restrict__ part_z) {
+  constexpr int kEl = NV * VEC, kCover = G * kEl, kGroups = 32 / G, kWarps = kRouterThreads / 32;
+  __shared__ float s_p[kCover];
+  __shared__ int s_hist[kCover];
+  __shared__ double s_z[kWarps];
+  __shared__ int s_kept[kWarps], s_bad;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane & (G - 1), grp = lane / G;
+  for (int i = threadIdx.x; i < kCover; i += kRouterThreads) {
+    s_p[i] = 0.f;
+    s_hist[i] = 0;
+  }
+  if (threadIdx.x == 0) s_bad = 0;
+  __syncthreads();
+  float acc[kEl];
+#pragma unroll
+  for (int i = 0; i < kEl; ++i) acc[i] = 0.f;
+  double z = 0.0;
+  int kept = 0;
+  // contiguous rows per warp, kGroups at a time
+  const long long total = static_cast<long long>(a.L) * a.T;
+  const long long nw = static_cast<long long>(gridDim.x) * kWarps;
+  const long long wid = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  const long long r_begin = total * wid / nw, r_end = total * (wid + 1) / nw;
+  int layer = static_cast<int>((r_begin + grp) / a.T);
+  long long t = (r_begin + grp) - static_cast<long long>(layer) * a.T;
+  for (long long r0 = r_begin; r0 < r_end; r0 += kGroups) {
+    const long long r = r0 + grp;
+    const bool in = r < r_end;
+    const bool keep = in && (a.mask == nullptr || a.mask[t] != 0);
+    float x[kEl];
+#pragma unroll
+    for (int i = 0; i < kEl; ++i) x[i] = -INFINITY;
+    if (in) {
+      load_row<T, VEC, G, NV>(static_cast<const T*>(a.logits[layer]) + t * a.ld[layer], sub, a.E, x);
+      if (keep) {
+        const int64_t* ip = a.idx[layer] + t * a.k;
+        for (int j = sub; j < a.k; j += G) {
+          const int64_t e = ip[j];
+          if (e >= 0 && e < a.E) atomicAdd(&s_hist[e], 1);
+          else s_bad = 1;
+        }
+      }
+    }
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < kEl; ++i) m = fmaxf(m, x[i]);
+    m = group_max<G>(m);
+    const float ml = m * kLog2e;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEl; ++i) {
+      x[i] = fast_exp2(fmaf(x[i], kLog2e, -ml));
+      s += x[i];
+    }
+    s = group_sum<G>(s);
+    const float inv = 1.f / s, lse = m + kLn2 * log2f(s);
+    if (keep) {
+#pragma unroll
+      for (int i = 0; i < kEl; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
+      if (sub == 0) {
+        z += static_cast<double>(lse) * lse;
+        ++kept;
+      }
+    }
+    if (in && sub == 0) lse_out[r] = lse;
+    t += kGroups;
+    while (t >= a.T) {
+      t -= a.T;
+      ++layer;
+    }
+  }
+  // the warps add their column sums in turn: a fixed order
+#pragma unroll
+  for (int i = 0; i < kEl; ++i) {
+#pragma unroll
+    for (int o = 16; o >= G; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+  }
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp && grp == 0) {
+#pragma unroll
+      for (int i = 0; i < kEl; ++i) s_p[((i / VEC) * G + sub) * VEC + i % VEC] += acc[i];
+    }
+    __syncthreads();
+  }
+  z = warp_sum_d(z);
+  kept = __reduce_add_sync(0xffffffffu, kept);
+  if (lane == 0) {
+    s_z[warp] = z;
+    s_kept[warp] = kept;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.E; i += kRouterThreads) {
+    part_p[static_cast<long long>(blockIdx.x) * a.E + i] = s_p[i];
+    part_n[static_cast<long long>(blockIdx.x) * a.E + i] = s_hist[i];
+  }
+  if (threadIdx.x == 0) {
+    long long n = 0;
+    z = 0.0;
+    for (int w = 0; w < kWarps; ++w) {
+      z += s_z[w];
+      n += s_kept[w];
+    }
+    part_z[blockIdx.x * 2] = s_bad ? __longlong_as_double(0x7ff8000000000000LL) : z;
+    part_z[blockIdx.x * 2 + 1] = static_cast<double>(n);
+  }
+}
+
+// One block joins the partial sums: loss, counts, and the backward's constants
+//   slope[e] = c_b E / n * f_e  and  slope[E] = 2 c_z / n
+__global__ void __launch_bounds__(1024) router_join_kernel(const float* __restrict__ part_p,
+                                                           const int* __restrict__ part_n,
+                                                           const double* __restrict__ part_z, int blocks,
+                                                           int E, float balance, float zcoef,
+                                                           float* __restrict__ loss,
+                                                           int64_t* __restrict__ counts,
+                                                           float* __restrict__ slope) {
+  __shared__ double s_p[32][33];
+  __shared__ long long s_n[32][33];
+  __shared__ double s_red[32], s_tot[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp == 0) {
+    double z = 0.0, n = 0.0;
+    for (int b = lane; b < blocks; b += 32) {
+      z += part_z[2 * b];
+      n += part_z[2 * b + 1];
+    }
+    z = warp_sum_d(z);
+    n = warp_sum_d(n);
+    if (lane == 0) {
+      s_tot[0] = z;
+      s_tot[1] = n > 0.0 ? n : 1.0;
+    }
+  }
+  // cols chunks of 32 columns at a time, 32 / cols warps striding over the blocks of each
+  const int all = (E + 31) / 32;
+  int cols = 1;
+  while (cols < 32 && cols < all) cols *= 2;
+  const int per = 32 / cols;
+  double dot = 0.0;
+  for (int c0 = 0; c0 < all; c0 += cols) {
+    const int c = (c0 + warp / per) * 32 + lane;
+    double p = 0.0;
+    long long n = 0;
+    if (c < E) {
+#pragma unroll 8
+      for (int b = warp % per; b < blocks; b += per) {
+        p += part_p[static_cast<long long>(b) * E + c];
+        n += part_n[static_cast<long long>(b) * E + c];
+      }
+    }
+    __syncthreads();
+    s_p[warp][lane] = p;
+    s_n[warp][lane] = n;
+    __syncthreads();
+    if (warp % per == 0 && c < E) {
+      for (int w = 1; w < per; ++w) {
+        p += s_p[warp + w][lane];
+        n += s_n[warp + w][lane];
+      }
+      const double tokens = s_tot[1], f = static_cast<double>(n) / tokens;
+      counts[c] = n;
+      slope[c] = static_cast<float>(balance * E / tokens * f);
+      dot += f * (p / tokens);
+    }
+  }
+  dot = warp_sum_d(dot);
+  if (lane == 0) s_red[warp] = dot;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int w = 0; w < 32; ++w) t += s_red[w];
+    const double tokens = s_tot[1];
+    // NaN in s_tot[0] marks a chosen index outside [0, E)
+    const bool bad = !(s_tot[0] == s_tot[0]);
+    *loss = static_cast<float>(balance * E * t + (zcoef != 0.f || bad ? zcoef * s_tot[0] / tokens : 0.0));
+    slope[E] = static_cast<float>(2.0 * zcoef / tokens);
+  }
+}
+
+// dlogit = gout p (slope_e - <p, slope> + slope_E lse), 0 in masked rows
+template <typename T, int VEC, int G, int NV>
+__global__ void __launch_bounds__(kRouterThreads) router_grad_kernel(const __grid_constant__ RouterArgs a,
+                                                                     const float* __restrict__ lse_in,
+                                                                     const float* __restrict__ slope,
+                                                                     const float* __restrict__ gout,
+                                                                     T* __restrict__ grad) {
+  constexpr int kEl = NV * VEC, kGroups = 32 / G, kWarps = kRouterThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane & (G - 1), grp = lane / G;
+  const float go = *gout, zs = slope[a.E] * go;
+  float f[kEl];
+#pragma unroll
+  for (int i = 0; i < kEl; ++i) {
+    const int c = ((i / VEC) * G + sub) * VEC + i % VEC;
+    f[i] = c < a.E ? slope[c] * go : 0.f;
+  }
+  const long long total = static_cast<long long>(a.L) * a.T;
+  const long long nw = static_cast<long long>(gridDim.x) * kWarps;
+  const long long wid = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  const long long r_begin = total * wid / nw, r_end = total * (wid + 1) / nw;
+  int layer = static_cast<int>((r_begin + grp) / a.T);
+  long long t = (r_begin + grp) - static_cast<long long>(layer) * a.T;
+  for (long long r0 = r_begin; r0 < r_end; r0 += kGroups) {
+    const long long r = r0 + grp;
+    const bool in = r < r_end;
+    const bool keep = in && (a.mask == nullptr || a.mask[t] != 0);
+    float x[kEl];
+    float lse = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEl; ++i) x[i] = -INFINITY;
+    if (keep) {
+      load_row<T, VEC, G, NV>(static_cast<const T*>(a.logits[layer]) + t * a.ld[layer], sub, a.E, x);
+      lse = lse_in[r];
+    }
+    const float l2 = lse * kLog2e;
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEl; ++i) {
+      x[i] = fast_exp2(fmaf(x[i], kLog2e, -l2));
+      d = fmaf(x[i], f[i], d);
+    }
+    d = group_sum<G>(d);
+    const float c = zs * lse - d;
+    if (in) {
+      T* g = grad + r * a.E;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int col = (v * G + sub) * VEC;
+        if (col < a.E) {
+          Pack<T, VEC> u;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            u.v[j] = static_cast<T>(keep ? x[v * VEC + j] * (f[v * VEC + j] + c) : 0.f);
+          *reinterpret_cast<Pack<T, VEC>*>(g + col) = u;
+        }
+      }
+    }
+    t += kGroups;
+    while (t >= a.T) {
+      t -= a.T;
+      ++layer;
+    }
+  }
+}
+
+int warp_grid(long long units) {
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((units + 7) / 8, 148 * 8)));
+}
+
+int chunks_of(int S) { return (S + kWarpTokens - 1) / kWarpTokens; }
+
+// 4 tokens at a time need every row to start on a boundary of 4 elements
+bool aligned4(const void* p, int bytes, std::initializer_list<long long> strides) {
+  if (reinterpret_cast<uintptr_t>(p) % (4 * bytes)) return false;
+  for (long long s : strides)
+    if (s % 4) return false;
+  return true;
+}
+
+// the widest layout for E columns: 16-byte vectors when rows allow them, 16 values a lane
+template <typename T, typename F>
+void router_dispatch(int E, bool vec, F&& launch) {
+  constexpr int V = 16 / sizeof(T), N = 16 / V;
+  if (vec) {
+    if (E <= 16) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, N>{});
+    else if (E <= 32) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, N>{});
+    else if (E <= 64) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, N>{});
+    else if (E <= 128) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 8>{}, std::integral_constant<int, N>{});
+    else if (E <= 256) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 16>{}, std::integral_constant<int, N>{});
+    else if (E <= 512) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, N>{});
+    else launch(std::integral_constant<int, V>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 2 * N>{});
+  } else {
+    if (E <= 128) launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+    else if (E <= 256) launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
+    else if (E <= 512) launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
+    else launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 32>{});
+  }
+}
+
+template <typename T>
+bool router_vec(const RouterArgs& a) {
+  constexpr int V = 16 / sizeof(T);
+  if (a.E % V) return false;
+  for (int l = 0; l < a.L; ++l)
+    if (a.ld[l] % V || (reinterpret_cast<uintptr_t>(a.logits[l]) & 15)) return false;
+  return true;
+}
+
+}  // namespace
+
+int pref_chunks(int S) { return std::max(1, chunks_of(S)); }
+
+int pref_blocks(int P) { return std::max(1, std::min((P + 7) / 8, 148)); }
+
+void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* ticket, float* row_scale,
+                  float* loss, float* rewards, cudaStream_t st) {
+  if (a.P <= 0) return;
+  const int chunks = pref_chunks(a.S);
+  const bool vec = a.S % 4 == 0 && aligned4(a.logps, 4, {a.lp_side, a.lp_pair}) &&
+                   aligned4(a.mask, 1, {a.mk_side, a.mk_pair}) &&
+                   (a.ref == nullptr || aligned4(a.ref, a.ref_bf16 ? 2 : 4, {a.ref_side, a.ref_pair}));
+  const int grid = warp_grid(2LL * a.P * chunks);
+  if (vec) pref_sums_kernel<4><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, ticket);
+  else pref_sums_kernel<1><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, ticket);
+  PLG_CUDA_CHECK(cudaGetLastError());
+  pref_pairs_kernel<<<pref_blocks(a.P), 256, 0, st>>>(a, static_cast<const float2*>(part), chunks, block_loss,
+                                                      ticket, row_scale, loss, rewards);
+  PLG_CUDA_CHECK(cudaGetLastError());
+}
+
+void pref_backward(const PrefArgs& a, const float* row_scale, const float* gout, float* grad, cudaStream_t st) {
+  if (a.P <= 0 || a.S <= 0) return;
+  const int chunks = pref_chunks(a.S);
+  const bool vec = a.S % 4 == 0 && aligned4(a.mask, 1, {a.mk_side, a.mk_pair}) && aligned4(grad, 4, {});
+  const int grid = warp_grid(2LL * a.P * chunks);
+  if (vec) pref_grad_kernel<4><<<grid, 256, 0, st>>>(a, row_scale, gout, grad, chunks);
+  else pref_grad_kernel<1><<<grid, 256, 0, st>>>(a, row_scale, gout, grad, chunks);
+  PLG_CUDA_CHECK(cudaGetLastError());
+}
+
+int policy_count_blocks(int R, int S) {
+  const long long b = S > 2048 ? R : (R + 7) / 8;
+  return static_cast<int>(std::max<long long>(1, std::min<long long>(b, 148 * 4)));
+}
+
+int policy_blocks(int R, int S) { return warp_grid(static_cast<long long>(R) * std::max(1, chunks_of(S))); }
+
+void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double* block_sums,
+                    unsigned* ticket, float* grad, float* out, cudaStream_t st) {
+  if (a.R <= 0) return;
+  const int cb = policy_count_blocks(a.R, a.S);
+  longlong2* bc = static_cast<longlong2*>(block_counts);
+  if (a.S > 2048) policy_counts_kernel<true><<<cb, 256, 0, st>>>(a, counts, bc, ticket);
+  else policy_counts_kernel<false><<<cb, 256, 0, st>>>(a, counts, bc, ticket);
+  PLG_CUDA_CHECK(cudaGetLastError());
+  const int chunks = std::max(1, chunks_of(a.S));
+  const bool vec = a.S % 4 == 0 && aligned4(a.logps, 4, {a.lp_row}) && aligned4(a.mask, 1, {a.mk_row}) &&
+                   (a.old == nullptr || aligned4(a.old, a.old_bf16 ? 2 : 4, {a.old_row})) &&
+                   (a.ref == nullptr || aligned4(a.ref, a.ref_bf16 ? 2 : 4, {a.ref_row})) &&
+                   (a.adv_tok == 0 || aligned4(a.adv, 4, {a.adv_row})) && aligned4(grad, 4, {});
+  const int grid = policy_blocks(a.R, a.S);
+  if (vec) policy_kernel<4><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket, grad, out, chunks);
+  else policy_kernel<1><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket, grad, out, chunks);
+  PLG_CUDA_CHECK(cudaGetLastError());
+}
+
+void scale_unless_one(float* x, long long n, const float* s, cudaStream_t st) {
+  if (n <= 0) return;
+  const int grid = static_cast<int>(std::min<long long>((n + 1023) / 1024, 148 * 8));
+  if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) scale_unless_one_kernel<4><<<grid, 256, 0, st>>>(x, n, s);
+  else scale_unless_one_kernel<1><<<grid, 256, 0, st>>>(x, n, s);
+  PLG_CUDA_CHECK(cudaGetLastError());
+}
+
+int router_blocks(long long rows) {
+  // at least 64 rows a block, at most two blocks an SM (their partial sums are joined by one)
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((rows + 63) / 64, 296)));
+}
+
+void router_balance_forward(const RouterArgs& a, bool bf16, float balance, float zcoef, float* lse,
+                            float* part_p, int* part_n, double* part_z, float* loss, int64_t* counts,
+                            float* slope, cudaStream_t st) {
+  if (a.E < 1 || a.E > kRouterMaxExperts || a.L < 1 || a.L > kRouterMaxLayers || a.k < 0)
+    throw std::invalid_argument("router_balance_loss: 1..1024 experts and 1..128 layers in one call");
+  const long long rows = static_cast<long long>(a.L) * a.T;
+  const int blocks = router_blocks(rows);
+  if (rows > 0) {
+    auto run = [&](auto* tag, bool vec) {
+      using T = std::remove_pointer_t<decltype(tag)>;
+      router_dispatch<T>(a.E, vec, [&](auto V, auto G, auto N) {
+        router_sums_kernel<T, V.value, G.value, N.value><<<blocks, kRouterThreads, 0, st>>>(a, lse, part_p, part_n,
+                                                                                          part_z);
+      });
+    };
+    if (bf16) run(static_cast<__nv_bfloat16*>(nullptr), router_vec<__nv_bfloat16>(a));
+    else run(static_cast<float*>(nullptr), router_vec<float>(a));
+    PLG_CUDA_CHECK(cudaGetLastError());
+  }
+  router_join_kernel<<<1, 1024, 0, st>>>(part_p, part_n, part_z, rows > 0 ? blocks : 0, a.E, balance, zcoef, loss,
+                                         counts, slope);
+  PLG_CUDA_CHECK(cudaGetLastError());
+}
+
+void router_balance_backward(const RouterArgs& a, bool bf16, const float* lse, const float* slope,
+                             const float* gout, void* grad, cudaStream_t st) {
+  const long long rows = static_cast<long long>(a.L) * a.T;
+  if (rows <= 0) return;
+  const int blocks = router_blocks(rows);
+  auto run = [&](auto* tag, bool vec) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    vec = vec && (reinterpret_cast<uintptr_t>(grad) & 15) == 0;
+    router_dispatch<T>(a.E, vec, [&](auto V, auto G, auto N) {
+      router_grad_kernel<T, V.value, G.value, N.value><<<blocks, kRouterThreads, 0, st>>>(a, lse, slope, gout,
+                                                                                        static_cast<T*>(grad));
+    });
+  };
+  if (bf16) run(static_cast<__nv_bfloat16*>(nullptr), router_vec<__nv_bfloat16>(a));
+  else run(static_cast<float*>(nullptr), router_vec<float>(a));
+  PLG_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace plg

@@ -50,6 +50,11 @@ struct GemmProblem {
   long long grp_b_rows = 0;
   const int* grp_koff = nullptr;
   int grp_count = 0;
+  // Device row counts (ungrouped, no split-K): rows of C past *m_limit are not computed, the
+  // sum stops at the 64-row block holding row *k_limit - 1 (A and B finite to its end; a
+  // count of 0 writes zeros).
+  const int* m_limit = nullptr;
+  const int* k_limit = nullptr;
 };
 void gemm_bf16(const GemmProblem& p, cudaStream_t stream);
 
@@ -139,6 +144,116 @@ void ce_rows(void* logits, long long ld, const int64_t* labels, long long rows, 
 // vocabulary): with stats_out [rows][3], only (max, sum of exp, owned target
 // logit or 0) are written and the logits are left alone; with lse_in [rows] (the
 // full-vocabulary lse), only the in-place gradient pass runs.
+
+// ---------------------------------------------------------------- token log-probabilities
+// One product of a linear head over packed rows: a[r, v] = <h_r, w_v>, columns being the
+// vocabulary entries [label0, label0 + N). n_rows (device int, optional) limits the rows;
+// row_map (optional) gives each row's token, whose label is labels[token].
+struct HeadProblem {
+  int rows = 0, N = 0, D = 0;
+  const void* h = nullptr;  // bf16 [rows, D]
+  long long ldh = 0;
+  const void* w = nullptr;  // bf16 [N, D]
+  long long ldw = 0;
+  int bn = 256;             // columns of a tile (head_tile_n)
+  const int* n_rows = nullptr;
+  const int* row_map = nullptr;
+  const int64_t* labels = nullptr;
+  long long label0 = 0;
+  float temperature = 1.f, softcap = 0.f;
+  int* status = nullptr;
+};
+int head_pairs();                       // CTA pairs of the persistent grid
+int head_tile_n(int rows, int N);
+// per row and half tile (reference, sum) pairs: part is float2 [rows][2 * ceil(N / bn)];
+// target [rows] receives the label's logit (after the softcap, before the temperature)
+void head_stats(const HeadProblem& p, void* part, float* target, cudaStream_t stream);
+// out[token] = log-probability of its label (0 where ignored, NaN outside [0, V));
+// lse2 [rows] (optional) = log2 of the row's sum of exponentials
+void head_join(const HeadProblem& p, const void* part, const float* target, long long V,
+               long long ignore_index, float* out, float* lse2, cudaStream_t stream);
+// bf16 G[r, v] = gout[token] * d out / d a[r, v]; zero rows from n_rows to the tile's end
+void head_grad(const HeadProblem& p, const float* lse2, const float* gout, void* G, long long ldg,
+               cudaStream_t stream);
+// row_map [T], inverse [T] (token -> row or -1), count [1], and out = 0 / NaN of the rest
+void head_compact(const int64_t* labels, long long T, long long V, long long ignore_index, int* row_map,
+                  int* inverse, int* count, float* out, cudaStream_t stream);
+// packed bf16 rows of h (bf16 or fp32), zero rows up to a multiple of 256 (at most cap_rows)
+void head_gather(const void* h, bool fp32, long long ldh, int D, const int* row_map, const int* count,
+                 void* out, int cap_rows, cudaStream_t stream);
+void head_scatter(const float* src, const int* inverse, void* dh, bool fp32, long long tokens, int D,
+                  cudaStream_t stream);
+
+// ---------------------------------------------------------------- objectives
+// Paired preference loss over [2, P, S] token log-probabilities (side 0 chosen, 1 rejected;
+// strides in elements, tokens contiguous). ref null: no reference model.
+struct PrefArgs {
+  const float* logps = nullptr;
+  long long lp_side = 0, lp_pair = 0;
+  const void* ref = nullptr;  // fp32 or bf16
+  bool ref_bf16 = false;
+  long long ref_side = 0, ref_pair = 0;
+  const uint8_t* mask = nullptr;
+  long long mk_side = 0, mk_pair = 0;
+  int P = 0, S = 0;
+  int kind = 0;               // 0 sigmoid, 1 hinge, 2 ipo
+  float beta = 0.1f, smoothing = 0.f;
+  bool normalized = false;    // mean over a sequence's tokens instead of the sum
+};
+int pref_chunks(int S);       // part holds float2 [2 * P * chunks]
+int pref_blocks(int P);       // block_loss holds that many doubles
+// row_scale [2, P] = d loss / d logps of each row's tokens; rewards [2, P] = beta * sums
+void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* ticket, float* row_scale,
+                  float* loss, float* rewards, cudaStream_t stream);
+void pref_backward(const PrefArgs& a, const float* row_scale, const float* gout, float* grad,
+                   cudaStream_t stream);
+
+// Clipped policy loss over [R, S] token log-probabilities (strides in elements, tokens
+// contiguous; adv_tok 0: one advantage for each row).
+struct PolicyArgs {
+  const float* logps = nullptr;
+  long long lp_row = 0;
+  const void* old = nullptr;  // null: the ratio is 1
+  bool old_bf16 = false;
+  long long old_row = 0;
+  const void* ref = nullptr;  // null: no KL term
+  bool ref_bf16 = false;
+  long long ref_row = 0;
+  const float* adv = nullptr;
+  long long adv_row = 0;
+  int adv_tok = 0;
+  const uint8_t* mask = nullptr;
+  long long mk_row = 0;
+  int R = 0, S = 0;
+  float hi = 1.2f, lo = 0.8f, log_hi = 0.f, log_lo = 0.f, kl_coef = 0.f;
+  bool by_sequence = false;   // mean over sequences of their means, else over all tokens
+};
+int policy_count_blocks(int R, int S);  // block_counts holds that many (2 x int64)
+int policy_blocks(int R, int S);        // block_sums holds 3 doubles for each
+// grad [R, S] (optional) = d loss / d logps; out [3] = loss, mean KL, clipped share
+void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double* block_sums,
+                    unsigned* ticket, float* grad, float* out, cudaStream_t stream);
+void scale_unless_one(float* x, long long n, const float* s, cudaStream_t stream);
+
+// Balance and z loss of L routers over [T, E] logits (row stride ld[l], columns contiguous)
+// with the experts idx[l] [T, k] that each token was sent to.
+constexpr int kRouterMaxLayers = 128, kRouterMaxExperts = 1024;
+struct RouterArgs {
+  const void* logits[kRouterMaxLayers];
+  const int64_t* idx[kRouterMaxLayers];
+  long long ld[kRouterMaxLayers];
+  const uint8_t* mask;  // [T] tokens that count (null: all)
+  long long T;
+  int L, E, k;
+};
+int router_blocks(long long rows);
+// lse [L, T]; workspaces part_p, part_n [blocks, E], part_z [blocks, 2]; slope [E + 1]
+void router_balance_forward(const RouterArgs& a, bool bf16, float balance, float zcoef, float* lse,
+                            float* part_p, int* part_n, double* part_z, float* loss, int64_t* counts,
+                            float* slope, cudaStream_t stream);
+// grad [L, T, E] in the logits' type
+void router_balance_backward(const RouterArgs& a, bool bf16, const float* lse, const float* slope,
+                             const float* gout, void* grad, cudaStream_t stream);
 
 // ---------------------------------------------------------------- optimizer
 struct TensorRef { void* p; long long n; };

@@ -1,0 +1,166 @@
+"""Log-probabilities of given tokens under a linear head (the LM head), without its logits.
+
+``linear_token_logprobs(hidden, weight, labels)`` returns, for every token,
+
+    z = softcap(hidden @ weight^T) / temperature
+    out = z[label] - log(sum(exp(z)))             (0 where the label is ignore_index)
+
+in fp32, differentiable in ``hidden`` and ``weight``. It is what a preference or a policy
+loss reads of the policy, and with gradients off it scores tokens under a frozen
+reference model or one sampled token at a time.
+
+CUDA path (csrc/logprob.cu): the product's tcgen05 epilogue reduces every accumulator
+tile to a (maximum, sum of exponentials) pair per row, so no logits are written; the
+backward recomputes them one vocabulary range at a time as the bf16 gradient
+``g_t * (onehot - softmax)``, whose two products give the gradients. Ranges are split over
+the vocabulary rather than over the tokens so that each row of the weight's gradient is
+written once, in its final type, instead of being summed over chunks of tokens. Tokens
+with ignored labels are packed away on the device first: they cost no products, and
+values in their hidden rows reach no output.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from pluggy_b200.ops._ext import ext, status_word
+
+# bytes of the bf16 gradient workspace of one vocabulary range (backward)
+GRAD_WORKSPACE = 2 << 30
+# Scoring at most this many tokens skips the packing of the kept ones: up to 256 tokens
+# are one row of tiles, whose time is the head's one pass through memory.
+UNPACKED_ROWS = 256
+
+
+def token_logprobs_reference(hidden, weight, labels, ignore_index=-100, softcap=None,
+                             temperature=1.0):
+    """fp32 math in eager torch on [T, D] rows; ignored rows take no part in the graph."""
+    keep = (labels != ignore_index).nonzero().squeeze(1)
+    z = hidden[keep].float() @ weight.float().t()
+    if softcap:
+        z = torch.tanh(z / softcap) * softcap
+    z = z / temperature
+    lp = z.gather(1, labels[keep].unsqueeze(1)).squeeze(1) - torch.logsumexp(z, dim=-1)
+    return torch.zeros(labels.shape, dtype=torch.float32, device=hidden.device).index_put((keep,), lp)
+
+
+def _rows_aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` or a copy whose rows start on 16-byte boundaries (what the TMA loads need)."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _round_up(n: int, m: int) -> int:
+    return (n + m - 1) // m * m
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, ignore_index, w, softcap, temperature, train):
+        T, D = hidden.shape
+        V = w.shape[0]
+        dev = hidden.device
+        out = torch.empty(T, dtype=torch.float32, device=dev)
+        row_map = inverse = count = lse2 = None
+        rows = T
+        if train or T > UNPACKED_ROWS:
+            rows = _round_up(T, 256)
+            row_map, inverse = torch.empty((2, T), dtype=torch.int32, device=dev)
+            count = torch.empty(1, dtype=torch.int32, device=dev)
+            ext().head_compact(labels, V, ignore_index, row_map, inverse, count, out)
+            h = torch.empty((rows, D), dtype=torch.bfloat16, device=dev)
+            ext().head_gather(hidden, row_map, count, h)
+            lse2 = torch.empty(rows, dtype=torch.float32, device=dev) if train else None
+        else:
+            h = hidden.to(torch.bfloat16)
+        ext().head_logprobs(h, w, labels, ignore_index, row_map, count, softcap, temperature, out,
+                            lse2, status_word(dev))
+        if train:
+            ctx.save_for_backward(h, w, labels, row_map, inverse, count, lse2)
+            ctx.cfg = (softcap, temperature, hidden.dtype, weight.dtype, T)
+        return out
+
+    @staticmethod
+    def backward(ctx, gout):
+        h, w, labels, row_map, inverse, count, lse2 = ctx.saved_tensors
+        softcap, temperature, h_dtype, w_dtype, T = ctx.cfg
+        rows, D = h.shape
+        V = w.shape[0]
+        dev = h.device
+        need_h, need_w = ctx.needs_input_grad[:2]
+        gout = gout.contiguous()
+        status = status_word(dev)
+        # equal vocabulary ranges, whole 256-column tiles, within the workspace
+        ranges = max(1, -(-(rows * V * 2) // GRAD_WORKSPACE))
+        width = min(_round_up(V, 8), _round_up(-(-V // ranges), 256))
+        G = torch.empty((rows, width), dtype=torch.bfloat16, device=dev)
+        dh_rows = torch.empty((rows, D), dtype=torch.float32, device=dev) if need_h else None
+        dw = None
+        if need_w:
+            dw = torch.empty((V, D), dtype=w_dtype if w_dtype == torch.bfloat16 else torch.float32,
+                             device=dev)
+        for v0 in range(0, V, width):
+            wv = w[v0:v0 + width]
+            g = G[:, :wv.shape[0]]
+            ext().head_grad(h, wv, v0, labels, row_map, count, softcap, temperature, lse2, gout, g,
+                            status)
+            if need_h:
+                ext().gemm(g, False, wv, True, dh_rows, dh_rows if v0 else None, 1.0,
+                           1.0 if v0 else 0.0, 1, 0, status, count, None)
+            if need_w:
+                ext().gemm(g, True, h, True, dw[v0:v0 + width], None, 1.0, 0.0, 1, 0, status, None,
+                           count)
+        dh = None
+        if need_h:
+            dh = torch.empty((T, D), dtype=h_dtype, device=dev)
+            ext().head_scatter(dh_rows, inverse, dh)
+        return (dh, dw) + (None,) * 6
+
+
+def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
+                          ignore_index: int = -100, *, weight_lowp: torch.Tensor | None = None,
+                          softcap: float | None = None, temperature: float = 1.0) -> torch.Tensor:
+    """fp32 log-probability of every label under ``softmax(softcap(hidden weight^T) / temperature)``.
+
+    ``hidden`` [..., D] and ``weight`` [V, D] are bf16 or fp32, ``labels`` [...] int64 (already
+    shifted: ``labels[t]`` is scored against ``hidden[t]``). The result has labels' shape and is
+    0 where the label is ``ignore_index``; a label outside [0, V) gives NaN and no gradient.
+    On CUDA the products are bf16 with fp32 accumulation, as everywhere in this package (an
+    fp32 ``weight`` is cast, or ``weight_lowp``, its cached bf16 copy, is read instead), and D
+    must be a multiple of 8. The gradients have the inputs' types."""
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear_token_logprobs: hidden [..., D] and weight [V, D], got "
+                         f"{tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if labels.shape != hidden.shape[:-1] or labels.dtype != torch.int64:
+        raise ValueError(f"linear_token_logprobs: labels must be int64 {tuple(hidden.shape[:-1])}, got "
+                         f"{labels.dtype} {tuple(labels.shape)}")
+    if not temperature > 0 or (softcap is not None and softcap < 0):
+        raise ValueError("linear_token_logprobs: temperature must be positive, softcap not negative")
+    if weight.shape[0] == 0:
+        raise ValueError("linear_token_logprobs: an empty vocabulary")
+    for name, t in (("hidden", hidden), ("weight", weight)):
+        if t.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"linear_token_logprobs: {name} must be bf16 or fp32, got {t.dtype}")
+    if weight.device != hidden.device or labels.device != hidden.device:
+        raise ValueError("linear_token_logprobs: hidden, weight and labels must be on one device")
+    if weight_lowp is not None and (weight_lowp.shape != weight.shape
+                                    or weight_lowp.dtype != torch.bfloat16
+                                    or weight_lowp.device != weight.device):
+        raise ValueError("linear_token_logprobs: weight_lowp must be weight's bf16 copy")
+    D = hidden.shape[-1]
+    if not hidden.is_cuda:
+        flat = labels.reshape(-1)
+        return token_logprobs_reference(hidden.reshape(-1, D), weight, flat, ignore_index, softcap,
+                                        temperature).view(labels.shape)
+    if D % 8 or D == 0:
+        raise ValueError(f"linear_token_logprobs: D must be a multiple of 8 on CUDA, got {D}")
+    if labels.numel() == 0:
+        return (hidden.sum() + weight.sum()) * torch.zeros(labels.shape, device=hidden.device)
+    w = weight_lowp if weight_lowp is not None else weight.detach().to(torch.bfloat16)
+    h = hidden.reshape(-1, D)
+    h, w = _rows_aligned(h), _rows_aligned(w)
+    train = torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
+    out = _TokenLogprobs.apply(h, weight, labels.reshape(-1).contiguous(), int(ignore_index), w,
+                               float(softcap or 0.0), float(temperature), train)
+    return out.view(labels.shape)

@@ -80,3 +80,99 @@ def moe_expert_ffn(hidden, top_indices, top_weights, gate_up_proj, down_proj, *,
         return _expert_ffn_sorted(hidden, top_indices, top_weights, gate_up_proj, down_proj,
                                   gu_lowp, dn_lowp)
     return _expert_ffn_loop(hidden, top_indices, top_weights, gate_up_proj, down_proj)
+
+
+# ------------------------------------------------------------------ router losses
+MAX_ROUTER_LAYERS, MAX_ROUTER_EXPERTS = 128, 1024
+
+
+def router_balance_loss_reference(router_logits, top_indices, balance_coef=1.0, z_coef=0.0, mask=None):
+    """fp32 math in eager torch on lists of [T, E] logits and [T, k] indices."""
+    E = router_logits[0].shape[1]
+    x = torch.cat([g.float() for g in router_logits])
+    idx = torch.cat(list(top_indices))
+    if mask is not None:
+        keep = mask.repeat(len(router_logits)).nonzero().squeeze(1)
+        x, idx = x[keep], idx[keep]
+    n = max(1, x.shape[0])
+    counts = expert_histogram(idx, E)
+    lse = torch.logsumexp(x, dim=-1)
+    probs = torch.exp(x - lse.unsqueeze(1))
+    loss = balance_coef * E * (counts / n * probs.sum(0) / n).sum()
+    if z_coef:
+        loss = loss + z_coef * lse.square().sum() / n
+    return loss, counts
+
+
+class _RouterBalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, idx, mask, balance_coef, z_coef, *logits):
+        from pluggy_b200.ops._ext import ext
+
+        T, E = logits[0].shape
+        dev = logits[0].device
+        lse = torch.empty((len(logits), T), dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int64, device=dev)
+        out = torch.empty(E + 2, dtype=torch.float32, device=dev)
+        ext().router_balance_fwd(logits, idx, mask, balance_coef, z_coef, lse, counts, out)
+        ctx.save_for_backward(lse, out, *logits)
+        ctx.idx, ctx.mask = idx, mask
+        ctx.mark_non_differentiable(counts)
+        return out[E + 1], counts
+
+    @staticmethod
+    def backward(ctx, gout, _):
+        from pluggy_b200.ops._ext import ext
+
+        lse, slope, *logits = ctx.saved_tensors
+        grad = torch.empty((len(logits), *logits[0].shape), dtype=logits[0].dtype, device=lse.device)
+        ext().router_balance_bwd(logits, ctx.idx, ctx.mask, lse, slope, gout, grad)
+        return (None, None, None, None, *grad.unbind())
+
+
+def router_balance_loss(router_logits, top_indices, *, balance_coef: float = 1.0, z_coef: float = 0.0,
+                        mask: torch.Tensor | None = None):
+    """Balance and z loss of one or several MoE routers, and the tokens sent to each expert.
+
+    ``router_logits`` is [T, E] (bf16 or fp32) or a list of them, one for each layer, and
+    ``top_indices`` the routers' own choices, int64 [T, k] alike. Over the n tokens of all
+    layers (those where ``mask``, bool [T], holds), with p = softmax(logits) in fp32 and
+    counts[e] = how often expert e was chosen,
+
+        loss = balance_coef * E * sum_e (counts[e] / n) * mean(p[:, e]) + z_coef * mean(logsumexp^2)
+
+    Returns ``(loss, counts int64 [E])``; the gradient goes to the logits (the counts are
+    constants, as in the models' auxiliary loss). An index outside [0, E) makes the loss NaN.
+
+    CUDA path (csrc/objective.cu): all layers in one launch that keeps a row's probabilities
+    in registers and writes only its log-sum-exp, one small kernel for the loss, one launch
+    for all gradients; no probabilities and no concatenated logits in memory."""
+    single = isinstance(router_logits, torch.Tensor)
+    logits = [router_logits] if single else list(router_logits)
+    idx = [top_indices] if single else list(top_indices)
+    if not logits or len(idx) != len(logits):
+        raise ValueError(f"router_balance_loss: one index tensor for each router, got {len(logits)} and "
+                         f"{len(idx)}")
+    x0 = logits[0]
+    for x, i in zip(logits, idx):
+        if x.dim() != 2 or x.shape != x0.shape or x.dtype != x0.dtype or x.device != x0.device:
+            raise ValueError("router_balance_loss: the routers' logits must be [T, E], alike")
+        if i.shape != (x.shape[0], idx[0].shape[-1]) or i.dtype != torch.int64 or i.device != x.device:
+            raise ValueError(f"router_balance_loss: indices must be int64 [T, k], got {i.dtype} "
+                             f"{tuple(i.shape)}")
+    if x0.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"router_balance_loss: logits must be bf16 or fp32, got {x0.dtype}")
+    if x0.shape[1] == 0:
+        raise ValueError("router_balance_loss: no experts")
+    if mask is not None and (mask.shape != x0.shape[:1] or mask.dtype != torch.bool
+                             or mask.device != x0.device):
+        raise ValueError(f"router_balance_loss: mask must be bool [{x0.shape[0]}]")
+    if not x0.is_cuda:
+        return router_balance_loss_reference(logits, idx, balance_coef, z_coef, mask)
+    if len(logits) > MAX_ROUTER_LAYERS or x0.shape[1] > MAX_ROUTER_EXPERTS:
+        raise ValueError(f"router_balance_loss: at most {MAX_ROUTER_LAYERS} layers of "
+                         f"{MAX_ROUTER_EXPERTS} experts on CUDA")
+    logits = [x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous() for x in logits]
+    return _RouterBalanceLoss.apply([i.contiguous() for i in idx],
+                                    None if mask is None else mask.contiguous(), float(balance_coef),
+                                    float(z_coef), *logits)

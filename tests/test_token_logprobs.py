@@ -1,0 +1,288 @@
+"""Token log-probabilities of a linear head against the definition in 64 bits.
+
+Tolerances. The kernel's operands are the bf16 values that the reference reads too, so a
+logit is off by its fp32 accumulation alone: at most D additions of relative error 2^-23
+in the order of sum_k |h_k w_k|, which random signs keep near sqrt(D); 2^-22 sqrt(D)
+sum|h w| bounds it and its use in the log-sum-exp with room to spare, and the result's own
+rounding and exponentials add a few 2^-23 of its size. The gradients' operand G is rounded
+to bf16, whose 8-bit significand makes that 2^-8 of each term at most, and so are gradients of
+bf16 inputs (2^-8 of the result): |d grad| <= 2^-7 |G| |operand| per element covers both.
+"""
+
+import pytest
+import torch
+
+from pluggy_b200.ops import linear_token_logprobs
+
+GPU = pytest.mark.gpu
+IGN = -100
+
+
+@pytest.fixture
+def status():
+    yield
+    if torch.cuda.is_available():
+        from pluggy_b200.ops import _ext
+
+        torch.cuda.synchronize()
+        _ext.check_status()
+
+
+def make(T, D, V, dev, ignored=0.3, seed=0, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed + T + 7 * D + 13 * V)
+    h = torch.randn(T, D, generator=g).to(dtype).to(dev)
+    w = (torch.randn(V, D, generator=g) * (3.0 / D ** 0.5)).to(dtype).to(dev)
+    y = torch.randint(0, V, (T,), generator=g)
+    y[torch.rand(T, generator=g) < ignored] = IGN
+    return h, w, y.to(dev), torch.randn(T, generator=g).to(dev)
+
+
+def exact(h, w, y, gout, softcap=None, tau=1.0):
+    """(logps, dh, dw, |G| |w|, |G|^T |h|, logit bound) in 64 bits; ignored rows left out."""
+    keep = y != IGN
+    H = torch.where(keep[:, None], h.double(), 0.0)
+    W = w.double()
+    a = H @ W.t()
+    z = (softcap * torch.tanh(a / softcap) if softcap else a) / tau
+    lse = torch.logsumexp(z, 1)
+    at = y.clamp_min(0)
+    r = torch.arange(len(y), device=y.device)
+    lp = torch.where(keep, z[r, at] - lse, 0.0)
+    G = -torch.exp(z - lse[:, None])
+    G[r, at] += 1.0
+    G *= (torch.where(keep, gout.double(), 0.0) / tau)[:, None]
+    if softcap:
+        G *= 1 - torch.tanh(a / softcap) ** 2
+    bound = (H.abs() @ W.abs().t()).max() / tau
+    return lp, G @ W, G.t() @ H, G.abs() @ W.abs(), G.abs().t() @ H.abs(), bound
+
+
+def check_case(h, w, y, gout, softcap=None, tau=1.0, **kw):
+    D = h.shape[1]
+    h = h.requires_grad_(True)
+    w = w.requires_grad_(True)
+    lp = linear_token_logprobs(h, w, y, softcap=softcap, temperature=tau, **kw)
+    assert lp.dtype == torch.float32 and lp.shape == y.shape
+    dh, dw = torch.autograd.grad(lp, (h, w), gout)
+    assert dh.dtype == h.dtype and dw.dtype == w.dtype
+    with torch.no_grad():
+        lp2 = linear_token_logprobs(h, w, y, softcap=softcap, temperature=tau, **kw)
+        ref, rdh, rdw, bdh, bdw, bound = exact(h, w, y, gout, softcap, tau)
+    tol = 2.0 ** -22 * D ** 0.5 * bound + 2.0 ** -20 * ref.abs()
+    assert ((lp - ref).abs() <= tol).all()
+    assert ((lp2 - ref).abs() <= tol).all()
+    assert (lp[y == IGN] == 0).all()
+    assert ((dh - rdh).abs() <= 2.0 ** -7 * bdh + 1e-6).all()
+    assert ((dw - rdw).abs() <= 2.0 ** -7 * bdw + 1e-6).all()
+    return lp, dh, dw
+
+
+@pytest.mark.parametrize("softcap,tau", [(None, 1.0), (5.0, 0.7)])
+@pytest.mark.parametrize("T,D,V", [(1, 8, 1), (7, 24, 33), (40, 64, 301)])
+def test_cpu_matches_definition(T, D, V, softcap, tau):
+    check_case(*make(T, D, V, "cpu", dtype=torch.float32), softcap, tau)
+
+
+CASES = [(1, 64, 1), (1, 1024, 4099), (2, 8, 33), (31, 72, 255), (127, 256, 1000), (128, 64, 256),
+         (129, 520, 257), (256, 128, 511), (257, 128, 513), (700, 256, 8191), (1025, 136, 2049),
+         (3000, 64, 5001)]
+
+
+@GPU
+@pytest.mark.parametrize("T,D,V", CASES)
+@pytest.mark.parametrize("softcap,tau", [(None, 1.0), (4.0, 0.6)])
+def test_kernel_matches_definition(T, D, V, softcap, tau, status):
+    check_case(*make(T, D, V, "cuda"), softcap, tau)
+
+
+@GPU
+@pytest.mark.parametrize("ignored", [0.0, 1.0])
+@pytest.mark.parametrize("T", [1, 300])
+def test_kernel_all_or_no_rows_ignored(T, ignored, status):
+    lp, dh, dw = check_case(*make(T, 128, 700, "cuda", ignored=ignored))
+    if ignored == 1.0:
+        assert (lp == 0).all() and (dh == 0).all() and (dw == 0).all()
+
+
+@GPU
+def test_kernel_vocabulary_ranges(monkeypatch, status):
+    """A workspace of a few columns: the gradients of many vocabulary ranges add up."""
+    from pluggy_b200.ops import logprob
+
+    monkeypatch.setattr(logprob, "GRAD_WORKSPACE", 512 * 2 * 600)
+    check_case(*make(512, 128, 2100, "cuda"))
+
+
+@GPU
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_ignored_rows_do_not_reach_anything(bad, status):
+    """NaN and infinities in the hidden rows of ignored tokens change nothing."""
+    h, w, y, g = make(600, 128, 1000, "cuda")
+    clean = check_case(h.clone(), w.clone(), y, g)
+    h2 = h.clone()
+    h2[y == IGN] = bad
+    h2.requires_grad_(True)
+    w2 = w.clone().requires_grad_(True)
+    gb = torch.where(y == IGN, torch.full_like(g, float("nan")), g)
+    lp = linear_token_logprobs(h2, w2, y)
+    dh, dw = torch.autograd.grad(lp, (h2, w2), gb)
+    for a, b in zip((lp, dh, dw), clean):
+        assert torch.equal(a, b)
+
+
+@GPU
+def test_kernel_extreme_logits(status):
+    """Logits of +-1e4 keep finite log-probabilities; equal logits give -log V."""
+    D, V = 64, 500
+    h = torch.zeros(3, D, device="cuda", dtype=torch.bfloat16)
+    w = torch.zeros(V, D, device="cuda", dtype=torch.bfloat16)
+    h[0, 0], h[1, 0], w[7, 0] = 100.0, -100.0, 100.0
+    y = torch.tensor([7, 7, 3], device="cuda")
+    lp = linear_token_logprobs(h, w, y)
+    ref = exact(h, w, y, torch.ones(3, device="cuda"))[0]
+    assert ((lp - ref).abs() <= 2.0 ** -20 * (1 + ref.abs())).all()
+
+
+@GPU
+def test_kernel_minus_infinity_logits(status):
+    """A vocabulary entry at -inf (a masked logit) has probability 0 and gradient 0."""
+    D, V = 64, 300
+    h, w, y, g = make(200, D, V, "cuda", ignored=0.0)
+    h = h.abs()  # positive, so that a weight row of -inf gives -inf logits
+    y = y.clamp_max(V - 2)
+    w2 = w.clone()
+    w2[V - 1] = float("-inf")
+    lp = linear_token_logprobs(h, w2, y)
+    ref, *_, bound = exact(h, w[:V - 1], y, g)
+    assert ((lp - ref).abs() <= 2.0 ** -22 * 8 * bound + 2.0 ** -20 * ref.abs()).all()
+
+
+@GPU
+def test_kernel_types_views_and_shapes(status):
+    """fp32 inputs (cast to bf16 for the products), a cached bf16 weight, [B, S] labels and
+    strided hidden states."""
+    h, w, y, g = make(6 * 50, 128, 900, "cuda")
+    hf = h.float().view(6, 50, 128).requires_grad_(True)
+    wf = w.float().requires_grad_(True)
+    lp = linear_token_logprobs(hf, wf, y.view(6, 50), weight_lowp=w)
+    dh, dw = torch.autograd.grad(lp, (hf, wf), g.view(6, 50))
+    assert dh.dtype == dw.dtype == torch.float32 and dh.shape == hf.shape
+    ref, rdh, rdw, bdh, bdw, bound = exact(h, w, y, g)
+    assert ((lp.view(-1) - ref).abs() <= 2.0 ** -22 * 12 * bound + 2.0 ** -20 * ref.abs()).all()
+    assert ((dh.view(-1, 128) - rdh).abs() <= 2.0 ** -7 * bdh + 1e-6).all()
+    assert ((dw - rdw).abs() <= 2.0 ** -7 * bdw + 1e-6).all()
+    big = torch.zeros(300, 3, 128, device="cuda", dtype=torch.bfloat16)
+    big[:, 1] = h
+    assert torch.equal(linear_token_logprobs(big[:, 1], w, y), lp.view(-1).detach())
+    odd = torch.zeros(300 * 128 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(300, 128)
+    odd.copy_(h)
+    assert torch.equal(linear_token_logprobs(odd, w, y), lp.view(-1).detach())
+
+
+@GPU
+def test_kernel_only_one_gradient_asked(status):
+    h, w, y, g = make(400, 64, 700, "cuda")
+    both = check_case(h.clone(), w.clone(), y, g)
+    hr = h.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(linear_token_logprobs(hr, w, y), hr, g)[0], both[1])
+    wr = w.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(linear_token_logprobs(h, wr, y), wr, g)[0], both[2])
+
+
+@GPU
+def test_kernel_gradient_matches_differences(status):
+    """Central differences along a direction. hidden and weight lie on a grid of 2^-4 (below
+    2) and the step is 2^-6, so every perturbed value is a bf16 value. The difference's own
+    error is step^2 / 6 times a third derivative of order |u|^3 ~ (step-scaled logit change)^3."""
+    gen = torch.Generator().manual_seed(5)
+    T, D, V, step = 64, 32, 200, 2.0 ** -6
+    h = (torch.randint(-16, 17, (T, D), generator=gen) / 16).cuda()
+    w = (torch.randint(-16, 17, (V, D), generator=gen) / 16).cuda()
+    y = torch.randint(0, V, (T,), generator=gen).cuda()
+    u = (torch.randint(0, 2, (T, D), generator=gen) * 2.0 - 1.0).cuda()
+    u *= torch.rand(T, D, generator=gen).cuda() < 0.25
+    hb, wb = h.bfloat16().requires_grad_(True), w.bfloat16()
+    lp = linear_token_logprobs(hb, wb, y)
+    (dh,) = torch.autograd.grad(lp.sum(), hb)
+    up = linear_token_logprobs((h + step * u).bfloat16(), wb, y).double()
+    dn = linear_token_logprobs((h - step * u).bfloat16(), wb, y).double()
+    diff = (up - dn) / (2 * step)
+    want = (dh.double() * u).sum(1)
+    # |u w| <= 8 per logit: third derivative of log-sum-exp <= 8^3; plus fp32 noise / step and
+    # bf16 rounding of the gradient (2^-7 of sum |dh|, |G| |W| <= 2 x 8)
+    tol = step ** 2 / 6 * 8.0 ** 3 + 2.0 ** -20 * 10 / step + 2.0 ** -7 * 16
+    assert ((diff - want).abs() <= tol).all()
+
+
+@GPU
+def test_kernel_is_repeatable(status):
+    h, w, y, g = make(900, 256, 3000, "cuda")
+    a = check_case(h.clone(), w.clone(), y, g)
+    b = check_case(h.clone(), w.clone(), y, g)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+
+
+@GPU
+def test_kernel_on_another_stream(status):
+    h, w, y, g = make(500, 128, 1000, "cuda")
+    a = check_case(h.clone(), w.clone(), y, g)[0].detach()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = linear_token_logprobs(h, w, y)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(a, b)
+
+
+@GPU
+def test_label_outside_the_vocabulary_is_nan(status):
+    h, w, y, g = make(300, 64, 100, "cuda", ignored=0.0)
+    y2 = y.clone()
+    y2[5], y2[6] = 100, -7
+    for kw in ({}, {"train": True}):
+        hr = h.clone().requires_grad_(bool(kw))
+        lp = linear_token_logprobs(hr, w, y2)
+        assert torch.isnan(lp[5:7]).all() and torch.isfinite(lp[7:]).all() and torch.isfinite(lp[:5]).all()
+    (dh,) = torch.autograd.grad(lp, hr, g)
+    assert (dh[5:7] == 0).all() and torch.isfinite(dh).all()
+    assert torch.isnan(linear_token_logprobs(h[5:7], w, y2[5:7])).all()
+
+
+def test_refusals():
+    h, w, y = torch.zeros(4, 16), torch.zeros(9, 16), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="hidden"):
+        linear_token_logprobs(h, torch.zeros(9, 8), y)
+    with pytest.raises(ValueError, match="labels"):
+        linear_token_logprobs(h, w, y[:3])
+    with pytest.raises(ValueError, match="labels"):
+        linear_token_logprobs(h, w, y.int())
+    with pytest.raises(ValueError, match="temperature"):
+        linear_token_logprobs(h, w, y, temperature=0.0)
+    with pytest.raises(ValueError, match="softcap"):
+        linear_token_logprobs(h, w, y, softcap=-1.0)
+    with pytest.raises(ValueError, match="empty"):
+        linear_token_logprobs(h, torch.zeros(0, 16), y)
+    with pytest.raises(TypeError, match="bf16 or fp32"):
+        linear_token_logprobs(h.double(), w, y)
+    with pytest.raises(ValueError, match="weight_lowp"):
+        linear_token_logprobs(h, w, y, weight_lowp=w)
+
+
+def test_no_tokens():
+    lp = linear_token_logprobs(torch.zeros(2, 0, 16, requires_grad=True), torch.zeros(9, 16),
+                               torch.zeros(2, 0, dtype=torch.int64))
+    assert lp.shape == (2, 0)
+
+
+@GPU
+def test_refusals_on_the_gpu(status):
+    y = torch.zeros(4, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="multiple of 8"):
+        linear_token_logprobs(torch.zeros(4, 12, device="cuda"), torch.zeros(9, 12, device="cuda"), y)
+    with pytest.raises(ValueError, match="one device"):
+        linear_token_logprobs(torch.zeros(4, 16, device="cuda"), torch.zeros(9, 16), y)
+    lp = linear_token_logprobs(torch.zeros(0, 16, device="cuda", requires_grad=True),
+                               torch.zeros(9, 16, device="cuda"), y[:0])
+    assert lp.shape == (0,)
+    lp.sum().backward()
