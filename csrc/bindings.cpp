@@ -31,8 +31,8 @@ int* status_ptr(const c10::optional<at::Tensor>& s) {
 // a device row count (int32, one element) or null
 const int* count_ptr(const c10::optional<at::Tensor>& c, const at::Tensor& like) {
   if (!c.has_value()) return nullptr;
-  TORCH_CHECK(c->scalar_type() == at::kInt && c->numel() == 1 && c->device() == like.device(),
-              "a device row count is one int32 on the operands' device");
+  TORCH_CHECK(c->scalar_type() == at::kInt && c->numel() >= 1 && c->device() == like.device(),
+              "a device row count is an int32 (its tensor's first) on the operands' device");
   return c->data_ptr<int>();
 }
 
@@ -422,19 +422,8 @@ void head_compact_b(const at::Tensor& labels, int64_t V, int64_t ignore_index, a
   TORCH_CHECK(T <= INT32_MAX - 256, "linear_token_logprobs: too many tokens in one call");
   const c10::cuda::CUDAGuard guard(labels.device());
   plg::head_compact(labels_ptr(labels), T, V, ignore_index, int_ptr(row_map, T, "row_map"),
-                    int_ptr(inverse, T, "inverse"), int_ptr(count, 1, "count"), float_ptr(out, T, "out"),
+                    int_ptr(inverse, T, "inverse"), int_ptr(count, 2, "count"), float_ptr(out, T, "out"),
                     cur_stream());
-}
-
-void head_gather_b(const at::Tensor& h, const at::Tensor& row_map, const at::Tensor& count, at::Tensor& out) {
-  check_cuda(h, "hidden");
-  TORCH_CHECK(h.dim() == 2 && h.stride(1) == 1 && (is_bf16(h) || is_f32(h)), "hidden must be [T, D] bf16 or fp32");
-  TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.dim() == 2 && out.size(1) == h.size(1) &&
-                  out.size(0) >= h.size(0), "head_gather: out must be contiguous bf16 [>= T, D]");
-  const c10::cuda::CUDAGuard guard(h.device());
-  plg::head_gather(h.data_ptr(), is_f32(h), h.stride(0), static_cast<int>(h.size(1)),
-                   int_ptr(row_map, h.size(0), "row_map"), int_ptr(count, 1, "count"), out.data_ptr(),
-                   static_cast<int>(out.size(0)), cur_stream());
 }
 
 plg::HeadProblem head_problem(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
@@ -461,7 +450,7 @@ plg::HeadProblem head_problem(const at::Tensor& h, const at::Tensor& w, const at
   p.labels = labels_ptr(labels);
   if (row_map.has_value()) {
     p.row_map = int_ptr(*row_map, labels.numel(), "row_map");
-    p.n_rows = count_ptr(count, h);
+    p.n_rows = int_ptr(*count, 2, "count");
   } else {
     TORCH_CHECK(labels.numel() == p.rows, "linear_token_logprobs: one label per row");
   }
@@ -471,44 +460,100 @@ plg::HeadProblem head_problem(const at::Tensor& h, const at::Tensor& w, const at
   return p;
 }
 
-// out[token] = log-probability of its label; lse2 [rows] (optional) for the gradient
+void* x_ptr(const at::Tensor& x, int64_t rows, int64_t cols) {
+  check_cuda(x, "x");
+  TORCH_CHECK(is_bf16(x) && x.dim() == 2 && x.size(0) == rows && x.size(1) == cols && x.stride(1) == 1,
+              "linear_token_logprobs: x must be bf16 [rows, N]");
+  return x.data_ptr();
+}
+
+// packed rows of hidden; ref (optional) [rows]: the reference of a kept X
+void head_gather_b(const at::Tensor& hidden, const at::Tensor& w, const at::Tensor& labels,
+                   const at::Tensor& row_map, const at::Tensor& count, double softcap, double temperature,
+                   at::Tensor& out, const c10::optional<at::Tensor>& ref) {
+  check_cuda(hidden, "hidden");
+  TORCH_CHECK(hidden.dim() == 2 && hidden.stride(1) == 1 && (is_bf16(hidden) || is_f32(hidden)),
+              "hidden must be [T, D] bf16 or fp32");
+  TORCH_CHECK(out.is_contiguous() && out.size(0) >= hidden.size(0), "head_gather: out must be [>= T, D]");
+  TORCH_CHECK(out.size(1) == hidden.size(1), "head_gather: out must be [>= T, D]");
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  const plg::HeadProblem p = head_problem(out, w, labels, row_map, count, softcap, temperature, c10::nullopt);
+  plg::head_gather(p, hidden.data_ptr(), is_f32(hidden), hidden.stride(0), out.data_ptr(),
+                   static_cast<int>(out.size(0)), ref.has_value() ? float_ptr(*ref, p.rows, "ref") : nullptr,
+                   cur_stream());
+}
+
+// out[token] = log-probability of its label; for the gradient, lse2 and label_grad [rows],
+// and with a kept x its reference ref [rows]
 void head_logprobs_b(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels, int64_t ignore_index,
                      const c10::optional<at::Tensor>& row_map, const c10::optional<at::Tensor>& count,
                      double softcap, double temperature, at::Tensor& out,
-                     const c10::optional<at::Tensor>& lse2, const c10::optional<at::Tensor>& status) {
+                     const c10::optional<at::Tensor>& lse2, const c10::optional<at::Tensor>& label_grad,
+                     const c10::optional<at::Tensor>& ref, const c10::optional<at::Tensor>& x,
+                     const c10::optional<at::Tensor>& status) {
   const c10::cuda::CUDAGuard guard(h.device());
   const plg::HeadProblem p = head_problem(h, w, labels, row_map, count, softcap, temperature, status);
+  TORCH_CHECK(ref.has_value() == x.has_value() && lse2.has_value() == label_grad.has_value() &&
+                  (!x.has_value() || (lse2.has_value() && count.has_value())),
+              "head_logprobs: x goes with ref, both with the gradient's row statistics and packed rows");
   const int64_t parts = 2 * ((p.N + p.bn - 1) / p.bn);
   // workspace: the rows' (reference, sum) pairs and their labels' logits
   at::Tensor part = at::empty({static_cast<int64_t>(p.rows) * (2 * parts + 1)}, out.options());
   float* target = part.data_ptr<float>() + 2 * parts * p.rows;
-  plg::head_stats(p, part.data_ptr(), target, cur_stream());
-  plg::head_join(p, part.data_ptr(), target, p.N, ignore_index, float_ptr(out, labels.numel(), "out"),
-                 lse2.has_value() ? float_ptr(*lse2, p.rows, "lse2") : nullptr, cur_stream());
+  const float* rp = ref.has_value() ? float_ptr(*ref, p.rows, "ref") : nullptr;
+  plg::head_stats(p, part.data_ptr(), target, rp, x.has_value() ? x_ptr(*x, p.rows, p.N) : nullptr,
+                  x.has_value() ? x->stride(0) : 0, cur_stream());
+  plg::head_join(p, part.data_ptr(), target, p.N, ignore_index, float_ptr(out, labels.numel(), "out"), rp,
+                 lse2.has_value() ? float_ptr(*lse2, p.rows, "lse2") : nullptr,
+                 label_grad.has_value() ? float_ptr(*label_grad, p.rows, "label_grad") : nullptr,
+                 count.has_value() ? count->data_ptr<int>() + 1 : nullptr, cur_stream());
 }
 
-// g [rows, N] bf16 = gout[token] * d out / d logits of the vocabulary range starting at v0
-void head_grad_b(const at::Tensor& h, const at::Tensor& w, int64_t v0, const at::Tensor& labels,
-                 const at::Tensor& row_map, const at::Tensor& count, double softcap, double temperature,
-                 const at::Tensor& lse2, const at::Tensor& gout, at::Tensor& g,
-                 const c10::optional<at::Tensor>& status) {
+// x [rows, N] = gradient rows over the vocabulary range starting at v0; if_flagged: only when
+// count[1] is set
+void head_recompute_b(const at::Tensor& h, const at::Tensor& w, int64_t v0, const at::Tensor& labels,
+                      const at::Tensor& row_map, const at::Tensor& count, double softcap, double temperature,
+                      const at::Tensor& lse2, const at::Tensor& label_grad, const at::Tensor& gout,
+                      bool if_flagged, at::Tensor& x, const c10::optional<at::Tensor>& status) {
   const c10::cuda::CUDAGuard guard(h.device());
   plg::HeadProblem p = head_problem(h, w, labels, row_map, count, softcap, temperature, status);
-  TORCH_CHECK(is_bf16(g) && g.dim() == 2 && g.size(0) == p.rows && g.size(1) == p.N && g.stride(1) == 1,
-              "head_grad: g must be bf16 [rows, N]");
   p.label0 = v0;
-  plg::head_grad(p, float_ptr(lse2, p.rows, "lse2"), float_ptr(gout, labels.numel(), "gout"), g.data_ptr(),
-                 g.stride(0), cur_stream());
+  plg::head_recompute(p, float_ptr(lse2, p.rows, "lse2"), float_ptr(label_grad, p.rows, "label_grad"),
+                      float_ptr(gout, labels.numel(), "gout"), if_flagged ? count.data_ptr<int>() + 1 : nullptr,
+                      x_ptr(x, p.rows, p.N), x.stride(0), cur_stream());
 }
 
-void head_scatter_b(const at::Tensor& src, const at::Tensor& inverse, at::Tensor& dh) {
+// completes a kept x; factor [rows, 2], hs [rows, D]
+void head_scale_rows_b(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
+                       const at::Tensor& row_map, const at::Tensor& count, double temperature,
+                       const at::Tensor& lse2, const at::Tensor& label_grad, const at::Tensor& ref,
+                       const at::Tensor& gout, at::Tensor& x, at::Tensor& factor, at::Tensor& hs) {
+  const c10::cuda::CUDAGuard guard(h.device());
+  const plg::HeadProblem p = head_problem(h, w, labels, row_map, count, 0.0, temperature, c10::nullopt);
+  TORCH_CHECK(is_bf16(hs) && hs.is_contiguous() && hs.sizes() == h.sizes(), "head_scale_rows: hs must be like h");
+  plg::head_scale_rows(p, float_ptr(lse2, p.rows, "lse2"), float_ptr(label_grad, p.rows, "label_grad"),
+                       float_ptr(ref, p.rows, "ref"), float_ptr(gout, labels.numel(), "gout"),
+                       x_ptr(x, p.rows, p.N), x.stride(0), float_ptr(factor, 2LL * p.rows, "factor"),
+                       hs.data_ptr(), cur_stream());
+}
+
+void head_scatter_b(const at::Tensor& src, const c10::optional<at::Tensor>& factor, const at::Tensor& w,
+                    const at::Tensor& labels, const at::Tensor& inverse, at::Tensor& dh) {
   check_cuda(dh, "dh");
   TORCH_CHECK(dh.dim() == 2 && dh.is_contiguous() && (is_bf16(dh) || is_f32(dh)) && src.dim() == 2 &&
-                  src.size(1) == dh.size(1) && dh.size(1) % 8 == 0,
-              "head_scatter: dh contiguous [T, D] bf16 or fp32, src [rows, D]");
+                  src.size(1) == dh.size(1) && dh.size(1) % 8 == 0 && labels.numel() == dh.size(0) &&
+                  is_bf16(w) && w.dim() == 2 && w.size(1) == dh.size(1),
+              "head_scatter: dh contiguous [T, D] bf16 or fp32, src [rows, D], w bf16 [V, D]");
   const c10::cuda::CUDAGuard guard(dh.device());
-  plg::head_scatter(float_ptr(src, src.numel(), "src"), int_ptr(inverse, dh.size(0), "inverse"),
-                    dh.data_ptr(), is_f32(dh), dh.size(0), static_cast<int>(dh.size(1)), cur_stream());
+  plg::HeadProblem p;
+  p.D = static_cast<int>(dh.size(1));
+  p.w = w.data_ptr();
+  p.ldw = w.stride(0);
+  p.labels = labels_ptr(labels);
+  plg::head_scatter(p, float_ptr(src, src.numel(), "src"),
+                    factor.has_value() ? float_ptr(*factor, 2 * src.size(0), "factor") : nullptr,
+                    int_ptr(inverse, dh.size(0), "inverse"), dh.data_ptr(), is_f32(dh), dh.size(0),
+                    cur_stream());
 }
 
 // ---- objectives over token log-probabilities and router logits
@@ -1175,7 +1220,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("head_compact", &head_compact_b);
   m.def("head_gather", &head_gather_b);
   m.def("head_logprobs", &head_logprobs_b);
-  m.def("head_grad", &head_grad_b);
+  m.def("head_recompute", &head_recompute_b);
+  m.def("head_scale_rows", &head_scale_rows_b);
   m.def("head_scatter", &head_scatter_b);
   m.def("gemm_grouped", &gemm_grouped, py::arg("a"), py::arg("b"), py::arg("b_mn_major"), py::arg("c"),
         py::arg("mode"), py::arg("table"), py::arg("groups"), py::arg("b_rows"), py::arg("alpha"),

@@ -303,6 +303,16 @@ __device__ __forceinline__ void tma_reduce_add_4d(const CUtensorMap* map, const 
         "r"(w)
       : "memory");
 }
+// 2-D tiled store of a shared-memory box, tracked by the issuing thread's bulk
+// async-group. Coordinates must be non-negative and x a multiple of 16 bytes; the parts
+// of the box outside the tensor are not written.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* smem_src, int32_t x,
+                                             int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+      ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(smem_src)), "r"(x), "r"(y)
+      : "memory");
+}
 __device__ __forceinline__ void bulk_commit_group() {
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }

@@ -3,16 +3,26 @@
 //   a[t, v]  = <h_t, w_v>                       tcgen05 product, fp32 accumulators
 //   z[t, v]  = softcap(a) / temperature         softcap(a) = cap * tanh(a / cap), or a
 //   out[t]   = z[t, y_t] - log sum_v exp z[t, v]
-//   dout/dz  = onehot(y_t) - softmax(z_t)
+//   d out[t] / d a[t, v] = (onehot(y_t) - p[t, v]) * softcap'(a) / temperature,  p = softmax(z)
 //
-// The logits never reach memory in the forward pass: the product's epilogue turns each
-// accumulator row of a tile into a running (reference, sum of 2^(z log2e - reference))
-// pair, and a second small kernel joins a row's pairs in a fixed order. The gradient pass
-// recomputes the tile and stores bf16 G = g_t * dout/dz, the operand of the two gradient
-// products (dh = G W, dW = G^T h, gemm_tcgen05.cu).
+// The logits never reach memory: the product's epilogue turns each accumulator row of a
+// tile into a running (reference, sum of 2^(z log2e - reference)) pair, and a second small
+// kernel joins a row's pairs in a fixed order.
 //
-// Rows whose label is ignore_index are left out of the products: compact_rows lists the
-// others on the device, gather_rows packs their hidden rows, and every later kernel reads
+// Gradient. dh = G W and dW = G^T h with G[t, v] = g_t * d out[t] / d a[t, v], in bf16. The
+// plain way recomputes each tile of the product in the backward pass (head_kernel STORE):
+// 8 T V D operations in all. Large problems need 6: dh = diag(c) X W and dW = X^T diag(c) h
+// hold for any X whose rows are G's up to factors c_t, so the forward pass already stores
+//   X[t, v] = bf16(2^(z log2e - r_t) * softcap'(a)),   r_t = z[t, y_t] log2e + 40
+// with a reference r_t that one dot product gives beforehand, and the backward pass writes
+// the label's entry and folds c_t = -(g_t / temperature) 2^(r_t - lse2_t) into the hidden rows
+// (for dW) and into the result (for dh). Since lse2 >= z_y log2e, the entries that matter
+// lie above 2^-100 and below 2^(-out log2e - 40): bf16's range holds them unless out < -97 or
+// so. If any row is beyond that, a flag in device memory makes the backward pass recompute.
+// What it costs: c_t h_t is rounded to bf16 once more (2^-8 of a term of dW).
+//
+// Rows whose label is ignore_index are left out of the products: compact_kernel lists
+// the others on the device, gather_kernel packs their hidden rows, and every later kernel reads
 // the row count from device memory, so nothing is read back to the host and a NaN or an
 // infinity in an ignored row reaches neither gradient.
 #include <algorithm>
@@ -30,18 +40,28 @@ constexpr int kBK = 64;   // one 128-byte swizzle row of bf16
 constexpr int kMaxBN = 256;
 constexpr int kStages = 6;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kThreads = 128 + 32 * kEpiWarps;  // a warpgroup of loads and MMAs, two of epilogue
+// Registers of the warpgroups where the epilogue holds a whole accumulator row part: the
+// launch has 168 for each of 384 threads, and 80 + 2 * 208 < 3 * 168.
+constexpr int kLoadRegs = 80, kEpiRegs = 208;
 constexpr int kABytes = kBM * kBK * 2;
 constexpr int kMaxStageBytes = kABytes + (kMaxBN / 2) * kBK * 2;
-constexpr int kSmemBytes = kStages * kMaxStageBytes + 1024 + 256;
+// per epilogue warp: two 32 x 32 bf16 boxes on their way to X
+constexpr int kBoxBytes = 32 * 32 * 2;
+constexpr int kSmemBytes = kStages * kMaxStageBytes + kEpiWarps * 2 * kBoxBytes + 1024 + 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-
-enum HeadMode { kStats = 0, kGrad = 1 };
+constexpr float kRefOffset = 40.f;   // r_t - z_y log2e
+constexpr float kRefLimit = 100.f;   // lse2 - r_t beyond which X is recomputed
+// Reduction length of one accumulator of the statistics: the tensor cores truncate each
+// addition, a bias of about 1e-9 of the sum per column of D (measured: 2.5e-6 of a logit at
+// D = 2560, 5e-7 at 512, where an fp32 chain's own rounding is as large), so longer sums
+// are cut into pieces that the epilogue adds in fp32.
+constexpr int kSegBlocks = 512 / kBK;
 
 struct HeadArgs {
-  int rows, N, k_blocks;
-  int bn, m_tiles, n_tiles, group_m;
+  int rows, N, k_blocks, segs;
+  int bn, n_tiles, group_m;
   const int* n_rows;            // device row count (null: rows)
   const int* row_map;           // compact row -> token (null: identity)
   const int64_t* labels;        // per token
@@ -49,30 +69,41 @@ struct HeadArgs {
   float k;                      // log2(e) / temperature
   float cap, inv_cap;
   int* status;
-  float2* part;                 // stats: [rows][2 * n_tiles]
-  float* target;                // stats: [rows] accumulator (after the softcap) of the label
-  const float* lse2;            // grad: [rows] log2 of the sum of 2^(z log2e)
-  const float* gout;            // grad: per token
+  float2* part;                 // statistics: [rows][2 * n_tiles]
+  float* target;                // statistics: [rows] a (after the softcap) of the label
+  const float* ref;             // X: [rows] r_t
+  const float* label_grad;      // X alone: [rows] (1 - p_y) softcap'(a_y)
+  const float* gout;            // X alone: per token
   float inv_temp;
-  __nv_bfloat16* G;
-  long long ldg;
+  const int* only_if;           // X alone: nothing to do unless this device flag is set
 };
 
 __device__ __forceinline__ float ex2(float x) { return fast_exp2(x); }
 
+// y = v where lane index `at` is i: a predicated move, which keeps a register array that is
+// searched for one element from becoming an indexed array in local memory
+__device__ __forceinline__ void pick_if(float& y, float v, int at, int i) {
+  asm("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %2, %3;\n\t@p mov.f32 %0, %1;\n\t}"
+      : "+f"(y)
+      : "f"(v), "r"(at), "r"(i));
+}
+
 // Persistent CTA-pair kernel: 256 x bn tiles with tcgen05.mma.cta_group::2. CTA rank r
 // holds rows [128 r, 128 r + 128) of the tile and loads those of A and half of B's bn
-// columns. Warp 0 loads (TMA), warp 1 of rank 0 issues the MMAs, 8 warps per CTA drain the
+// columns. Warp 0 loads (TMA), warp 1 of rank 0 issues the MMAs, warps 4 to 11 drain the
 // accumulator (two warps per 32-row quadrant, alternate 32-column chunks), double
-// buffered in TMEM against the next tile's main loop.
-template <int MODE, bool CAP>
+// buffered in TMEM against the next main loop. STATS: the rows' (reference, sum) pairs;
+// STORE: X, staged per warp and written by TMA; SEG: more than one accumulator piece.
+template <bool STATS, bool STORE, bool CAP, bool SEG>
 __global__ void __launch_bounds__(kThreads, 1)
     head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                const HeadArgs args) {
+                const __grid_constant__ CUtensorMap tmX, const HeadArgs args) {
+  if (!STATS && args.only_if != nullptr && *args.only_if == 0) return;  // uniform over the grid
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kStages * kMaxStageBytes);
+  uint8_t* boxes = smem + kStages * kMaxStageBytes;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(boxes + kEpiWarps * 2 * kBoxBytes);
   uint64_t* full_bar = bar;                  // [kStages] (rank 0's are used)
   uint64_t* empty_bar = bar + kStages;       // [kStages]
   uint64_t* accf_bar = bar + 2 * kStages;    // [2]
@@ -105,6 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
+    if (STORE) tma_prefetch_desc(&tmX);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_base_smem, 512);
@@ -118,6 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int rows = args.n_rows != nullptr ? min(*args.n_rows, args.rows) : args.rows;
   const int m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
   const int total = m_tiles * args.n_tiles;
+  const int segs = SEG ? args.segs : 1;
   // m tiles walk fastest within a group of group_m of them, so the group's rows stay in L2
   // while the head streams past once per group
   auto decode = [&](int w, int& mt, int& nt) {
@@ -130,228 +163,290 @@ __global__ void __launch_bounds__(kThreads, 1)
     mt = m0 + (r - nt * gm);
   };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      uint32_t armed_mask = 0, parity_mask = 0;
-      for (int w = pair; w < total && ok; w += npairs) {
-        int mt, nt;
-        decode(w, mt, nt);
-        const int m0 = mt * 2 * kBM + static_cast<int>(rank) * kBM;
-        const int n0 = nt * bn + static_cast<int>(rank) * (bn / 2);
-        for (int kb = 0; kb < args.k_blocks; ++kb) {
-          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag)) {
-            record_status(args.status, kTimeoutSmemEmpty);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          uint8_t* sA = smem + stage * kMaxStageBytes;
-          if (leader) {
-            mbar_arrive_expect_tx(&full_bar[stage], 2 * stage_bytes);
-            armed_mask |= 1u << stage;
-            parity_mask = (parity_mask & ~(1u << stage)) | (phase << stage);
-          }
-          tma_load_2d_pair(sA, &tmA, &full_bar[stage], kb * kBK, m0);
-          tma_load_2d_pair(sA + kABytes, &tmB, &full_bar[stage], kb * kBK, n0);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+  if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    if (SEG) setmaxnreg_inc<kEpiRegs>();  // heads its warpgroups' branch
+    const int q = warp & 3;           // TMEM lane quadrant this warp may access
+    const int half = (warp - 4) >> 2;  // which of the quadrant's two warps
+    const int chunks = bn / 32;
+    uint8_t* box = boxes + (warp - 4) * 2 * kBoxBytes;
+    int local = 0, nbox = 0;
+    bool ok = true;
+    for (int w = pair; w < total && ok; w += npairs) {
+      int mt, nt;
+      decode(w, mt, nt);
+      const int row0 = mt * 2 * kBM + static_cast<int>(rank) * kBM + q * 32;  // the warp's first row
+      const int row = row0 + lane;
+      const bool live = row < rows;
+      // this row's label as a column of this launch, and its constants
+      long long lab = -1;
+      float rref = 0.f, lgrad = 0.f, coef = 0.f;
+      if (live) {
+        const int tok = args.row_map != nullptr ? args.row_map[row] : row;
+        lab = args.labels[tok] - args.label0;
+        if (STORE) rref = args.ref[row];
+        if (STORE && !STATS) {
+          coef = args.gout[tok] * args.inv_temp;
+          lgrad = args.label_grad[row] * coef;
         }
       }
-      if (!ok) {
-        // unwind: let the copies in flight land before the CTA can exit
-        if (leader) {
-          for (int s = 0; s < kStages; ++s)
-            if (((armed_mask >> s) & 1u) &&
-                !mbar_wait_bounded(&full_bar[s], (parity_mask >> s) & 1u, nullptr))
-              record_status(args.status, kTimeoutDrain);
-        } else {
-          const uint64_t t0 = globaltimer_ns();
-          while (globaltimer_ns() - t0 < 2000000ull) {
-          }
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ----------------------------------------------------------------- MMA
-    if (lane == 0 && leader) {
-      const uint32_t idesc = make_idesc_bf16_f32(2 * kBM, bn, false, false);
-      int stage = 0;
-      uint32_t phase = 0;
-      int local = 0;
-      bool ok = true;
-      for (int w = pair; w < total && ok; w += npairs, ++local) {
+      // warps without any row in use skip the math (X gets its zero rows all the same)
+      const bool busy = STORE ? row0 < args.rows : row0 < rows;
+      float acc[SEG ? 4 : 1][32];
+      for (int seg = 0; seg < segs; ++seg, ++local) {
         const int buf = local & 1;
-        const uint32_t acc_phase = (local >> 1) & 1;
-        if (!mbar_wait_bounded(&acce_bar[buf], acc_phase ^ 1u, abort_flag)) {
-          record_status(args.status, kTimeoutAccEmpty);
+        if (!mbar_wait_bounded(&accf_bar[buf], (local >> 1) & 1, abort_flag)) {
+          record_status(args.status, kTimeoutAccFull);
           *abort_flag = 1;
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + buf * kMaxBN;
-        for (int kb = 0; kb < args.k_blocks; ++kb) {
-          if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag)) {
-            record_status(args.status, kTimeoutTmaFull);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sA = smem_u32(smem + stage * kMaxStageBytes);
-          const uint64_t da0 = make_smem_desc(sA, 16, 1024, kLayoutSW128);
-          const uint64_t db0 = make_smem_desc(sA + kABytes, 16, 1024, kLayoutSW128);
+        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * kMaxBN;
+        if (SEG && busy) {
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk)
-            tc_mma_ss_pair(d_tmem, desc_advance(da0, kk * 32), desc_advance(db0, kk * 32), idesc,
-                           (kb > 0 || kk > 0) ? 1u : 0u);
-          tc_commit_pair(&empty_bar[stage], 0x3);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
+          for (int j = 0; j < (SEG ? 4 : 1); ++j) {
+            if (half + 2 * j >= chunks) continue;
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              uint32_t r[16];
+              __syncwarp();
+              tmem_ld_32x32b_x16(t_row + (half + 2 * j) * 32 + h, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                acc[j][h + i] = __uint_as_float(r[i]) + (seg == 0 ? 0.f : acc[j][h + i]);
+            }
           }
         }
-        if (!ok) break;
-        tc_commit_pair(&accf_bar[buf], 0x3);
-      }
-      if (!ok) *abort_flag = 1;
-      tc_commit_pair(done_bar, 0x3);
-    }
-    if (lane == 0 && !mbar_wait_bounded(done_bar, 0, nullptr)) record_status(args.status, kTimeoutDrain);
-    __syncwarp();
-  } else {
-    // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;           // TMEM lane quadrant this warp may access
-    const int half = (warp - 2) >> 2;  // which of the quadrant's two warps
-    const int row_in_tile = q * 32 + lane;
-    const int chunks = bn / 32;
-    int local = 0;
-    for (int w = pair; w < total; w += npairs, ++local) {
-      int mt, nt;
-      decode(w, mt, nt);
-      const int buf = local & 1;
-      const uint32_t acc_phase = (local >> 1) & 1;
-      const int row = mt * 2 * kBM + static_cast<int>(rank) * kBM + row_in_tile;
-      const bool live = row < rows;
-      // this row's label as a column of this launch, and its factors
-      long long lab = -1;
-      float lse2 = 0.f, coef = 0.f;
-      if (live) {
-        const int tok = args.row_map != nullptr ? args.row_map[row] : row;
-        lab = args.labels[tok] - args.label0;
-        if (MODE == kGrad) {
-          lse2 = args.lse2[row];
-          coef = args.gout[tok] * args.inv_temp;
-        }
-      }
-      if (!mbar_wait_bounded(&accf_bar[buf], acc_phase, abort_flag)) {
-        record_status(args.status, kTimeoutAccFull);
-        *abort_flag = 1;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * kMaxBN;
-      const bool warp_live = row - lane < rows;  // any live row in this warp
-      if (MODE == kStats ? warp_live : row - lane < args.rows) {
-        float ref = -INFINITY, s0 = 0.f, s1 = 0.f;
-#pragma unroll 1
-        for (int c = half; c < chunks; c += 2) {
-          uint32_t r[32];
+        if (SEG) {  // the row part is in registers: the next main loop may have the accumulator
+          tc_fence_before();
           __syncwarp();
-          tmem_ld_32x32b_x32(t_row + c * 32, r);
-          tmem_ld_wait();
-          const int col0 = nt * bn + c * 32;
-          if (col0 >= args.N) continue;  // uniform over the grid's columns
-          float v[32];
+          if (lane == 0) mbar_arrive_cluster(&acce_bar[buf], 0);
+        }
+        if (busy && seg == segs - 1) {
+          float ref = -INFINITY, s0 = 0.f, s1 = 0.f, target = 0.f;
+          auto chunk = [&](int c, float (&v)[32]) __attribute__((always_inline)) {
+            const int col0 = nt * bn + c * 32;
+            if (col0 >= args.N) return;  // uniform over the warp
+            float slope[CAP && STORE ? 32 : 1];
+            if (CAP) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            v[i] = __uint_as_float(r[i]);
-            if (CAP && MODE == kStats) v[i] = args.cap * tanhf(v[i] * args.inv_cap);
-          }
-          const int lc = (lab >= col0 && lab < col0 + 32) ? static_cast<int>(lab - col0) : -1;
-          if (MODE == kStats) {
-            if (lc >= 0) {
-              float y = 0.f;
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i == lc) y = v[i];
-              if (col0 + lc < args.N) args.target[row] = y;
-            }
-            if (col0 + 32 > args.N) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (col0 + i >= args.N) v[i] = -INFINITY;
-            }
-            float m = fmax3(v[0], v[1], v[2]);
-#pragma unroll
-            for (int i = 3; i < 31; i += 2) m = fmax3(m, v[i], v[i + 1]);
-            m = fmaxf(m, v[31]);
-            const float nref = fmaxf(ref, m * args.k);
-            const float sub = nref == -INFINITY ? 0.f : nref;
-            const float f = ex2(ref - sub);
-            s0 *= f;
-            s1 *= f;
-            ref = nref;
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float e0, e1;
-              ffma2(e0, e1, v[i], v[i + 1], args.k, args.k, -sub, -sub);
-              fadd2(s0, s1, s0, s1, ex2(e0), ex2(e1));
-            }
-          } else {
-            uint32_t o[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float a0 = v[i], a1 = v[i + 1], d0 = coef, d1 = coef;
-              if (CAP) {
-                const float t0 = tanhf(a0 * args.inv_cap), t1 = tanhf(a1 * args.inv_cap);
-                a0 = args.cap * t0;
-                a1 = args.cap * t1;
-                d0 *= 1.f - t0 * t0;
-                d1 *= 1.f - t1 * t1;
+              for (int i = 0; i < 32; ++i) {
+                const float t = tanhf(v[i] * args.inv_cap);
+                v[i] = args.cap * t;
+                if (STORE) slope[i] = 1.f - t * t;
               }
-              float e0, e1;
-              ffma2(e0, e1, a0, a1, args.k, args.k, -lse2, -lse2);
-              float g0 = -ex2(e0), g1 = -ex2(e1);
-              if (i == lc) g0 += 1.f;
-              if (i + 1 == lc) g1 += 1.f;
-              o[i / 2] = pack_bf16x2(g0 * d0, g1 * d1);
             }
-            // rows past the count up to the tile's end are the products' zero padding
-            if (!live) {
+            const int lc = (lab >= col0 && lab < col0 + 32) ? static_cast<int>(lab - col0) : -1;
+            if (STATS) {
+              // With whole row parts in registers the pick runs unconditionally: a branch around
+              // it makes the compiler spill 80 registers, and the long main loop hides it.
+              if (SEG || __any_sync(0xffffffffu, lc >= 0)) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = 0u;
-            }
-            if (row < args.rows) {
-              __nv_bfloat16* gp = args.G + row * args.ldg + col0;
-              if (col0 + 32 <= args.N) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                  *reinterpret_cast<uint4*>(gp + 2 * i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-              } else {
+                for (int i = 0; i < 32; ++i) pick_if(target, v[i], lc, i);
+              }
+              if (col0 + 32 > args.N) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                  if (col0 + i < args.N) {
-                    const uint32_t u = (i & 1) ? (o[i / 2] >> 16) : (o[i / 2] & 0xffffu);
-                    reinterpret_cast<uint16_t*>(gp)[i] = static_cast<uint16_t>(u);
-                  }
+                  if (col0 + i >= args.N) v[i] = -INFINITY;
               }
+              float m = fmax3(v[0], v[1], v[2]);
+#pragma unroll
+              for (int i = 3; i < 31; i += 2) m = fmax3(m, v[i], v[i + 1]);
+              m = fmaxf(m, v[31]);
+              const float nref = fmaxf(ref, m * args.k);
+              const float sub = nref == -INFINITY ? 0.f : nref;
+              const float f = ex2(ref - sub);
+              s0 *= f;
+              s1 *= f;
+              ref = nref;
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float e0, e1;
+                ffma2(e0, e1, v[i], v[i + 1], args.k, args.k, -sub, -sub);
+                v[i] = ex2(e0);
+                v[i + 1] = ex2(e1);
+                fadd2(s0, s1, s0, s1, v[i], v[i + 1]);
+              }
+              if (STORE) {
+                const float to_ref = nref == -INFINITY ? 0.f : ex2(sub - rref);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) fmul2(v[i], v[i + 1], v[i], v[i + 1], to_ref, to_ref);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float e0, e1;
+                ffma2(e0, e1, v[i], v[i + 1], args.k, args.k, -rref, -rref);
+                v[i] = ex2(e0);
+                v[i + 1] = ex2(e1);
+              }
+            }
+            if (STORE) {
+              uint32_t o[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                if (CAP) {
+                  v[i] *= slope[i % (CAP && STORE ? 32 : 1)];
+                  v[i + 1] *= slope[(i + 1) % (CAP && STORE ? 32 : 1)];
+                }
+                if (!STATS) {
+                  v[i] = i == lc ? lgrad : -coef * v[i];
+                  v[i + 1] = i + 1 == lc ? lgrad : -coef * v[i + 1];
+                }
+                // rows past the count up to the tile's end: zero padding of the products
+                o[i / 2] = live ? pack_bf16x2(v[i], v[i + 1]) : 0u;
+              }
+              // 64-byte rows, 16-byte pieces swizzled as the tensor map expects them
+              uint8_t* b = box + (nbox & 1) * kBoxBytes;
+              if (lane == 0) bulk_wait_group_read<1>();
+              __syncwarp();
+              uint4* brow = reinterpret_cast<uint4*>(b + lane * 64);
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+                brow[p ^ ((lane >> 1) & 3)] = make_uint4(o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&tmX, b, col0, row0);
+                bulk_commit_group();
+              }
+              ++nbox;
+            }
+          };
+          if (SEG) {
+#pragma unroll
+            for (int j = 0; j < (SEG ? 4 : 1); ++j)
+              if (half + 2 * j < chunks) chunk(half + 2 * j, acc[j]);
+          } else {
+#pragma unroll 1
+            for (int c = half; c < chunks; c += 2) {
+              uint32_t r[32];
+              __syncwarp();
+              tmem_ld_32x32b_x32(t_row + c * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) acc[0][i] = __uint_as_float(r[i]);
+              chunk(c, acc[0]);
+            }
+          }
+          // the label's chunk was one of this warp's
+          if (STATS && lab >= nt * bn && lab < min((nt + 1) * bn, args.N) &&
+              ((static_cast<int>(lab) - nt * bn) / 32) % 2 == half)
+            args.target[row] = target;
+          if (STATS && live)
+            args.part[static_cast<long long>(row) * (2 * args.n_tiles) + 2 * nt + half] =
+                make_float2(ref, s0 + s1);
+        }
+        if (!SEG) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(&acce_bar[buf], 0);
+        }
+      }
+    }
+    // the staged boxes must have left shared memory (and reached X) before the CTA exits
+    if (STORE && lane == 0) bulk_wait_group<0>();
+  } else {
+    if (SEG) setmaxnreg_dec<kLoadRegs>();
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        uint32_t armed_mask = 0, parity_mask = 0;
+        for (int w = pair; w < total && ok; w += npairs) {
+          int mt, nt;
+          decode(w, mt, nt);
+          const int m0 = mt * 2 * kBM + static_cast<int>(rank) * kBM;
+          const int n0 = nt * bn + static_cast<int>(rank) * (bn / 2);
+          for (int kb = 0; kb < args.k_blocks; ++kb) {
+            if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+              record_status(args.status, kTimeoutSmemEmpty);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            uint8_t* sA = smem + stage * kMaxStageBytes;
+            if (leader) {
+              mbar_arrive_expect_tx(&full_bar[stage], 2 * stage_bytes);
+              armed_mask |= 1u << stage;
+              parity_mask = (parity_mask & ~(1u << stage)) | (phase << stage);
+            }
+            tma_load_2d_pair(sA, &tmA, &full_bar[stage], kb * kBK, m0);
+            tma_load_2d_pair(sA + kABytes, &tmB, &full_bar[stage], kb * kBK, n0);
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
             }
           }
         }
-        if (MODE == kStats && live)
-          args.part[static_cast<long long>(row) * (2 * args.n_tiles) + 2 * nt + half] =
-              make_float2(ref, s0 + s1);
+        if (!ok) {
+          // unwind: let the copies in flight land before the CTA can exit
+          if (leader) {
+            for (int s = 0; s < kStages; ++s)
+              if (((armed_mask >> s) & 1u) &&
+                  !mbar_wait_bounded(&full_bar[s], (parity_mask >> s) & 1u, nullptr))
+                record_status(args.status, kTimeoutDrain);
+          } else {
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 2000000ull) {
+            }
+          }
+        }
       }
-      tc_fence_before();
+    } else if (warp == 1) {
+      // ----------------------------------------------------------------- MMA
+      if (lane == 0 && leader) {
+        const uint32_t idesc = make_idesc_bf16_f32(2 * kBM, bn, false, false);
+        int stage = 0;
+        uint32_t phase = 0;
+        int local = 0;
+        bool ok = true;
+        for (int w = pair; w < total && ok; w += npairs) {
+          for (int seg = 0; seg < segs && ok; ++seg, ++local) {
+            const int kb0 = seg * args.k_blocks / segs, kb1 = (seg + 1) * args.k_blocks / segs;
+            const int buf = local & 1;
+            const uint32_t acc_phase = (local >> 1) & 1;
+            if (!mbar_wait_bounded(&acce_bar[buf], acc_phase ^ 1u, abort_flag)) {
+              record_status(args.status, kTimeoutAccEmpty);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + buf * kMaxBN;
+            for (int kb = kb0; kb < kb1; ++kb) {
+              if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag)) {
+                record_status(args.status, kTimeoutTmaFull);
+                *abort_flag = 1;
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t sA = smem_u32(smem + stage * kMaxStageBytes);
+              const uint64_t da0 = make_smem_desc(sA, 16, 1024, kLayoutSW128);
+              const uint64_t db0 = make_smem_desc(sA + kABytes, 16, 1024, kLayoutSW128);
+#pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk)
+                tc_mma_ss_pair(d_tmem, desc_advance(da0, kk * 32), desc_advance(db0, kk * 32), idesc,
+                               (kb > kb0 || kk > 0) ? 1u : 0u);
+              tc_commit_pair(&empty_bar[stage], 0x3);
+              if (++stage == kStages) {
+                stage = 0;
+                phase ^= 1u;
+              }
+            }
+            if (ok) tc_commit_pair(&accf_bar[buf], 0x3);
+          }
+        }
+        if (!ok) *abort_flag = 1;
+        tc_commit_pair(done_bar, 0x3);
+      }
+      if (lane == 0 && !mbar_wait_bounded(done_bar, 0, nullptr)) record_status(args.status, kTimeoutDrain);
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(&acce_bar[buf], 0);
     }
   }
 
@@ -378,6 +473,7 @@ __global__ void __launch_bounds__(kScan) compact_kernel(const int64_t* __restric
                                                         float* __restrict__ out) {
   __shared__ int s_warp[32];
   __shared__ int s_base;
+  if (blockIdx.x == 0 && threadIdx.x == 0) count[1] = 0;  // the flag that join_kernel may set
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long b0 = static_cast<long long>(blockIdx.x) * kScan;
   int before = 0;
@@ -418,64 +514,120 @@ __global__ void __launch_bounds__(kScan) compact_kernel(const int64_t* __restric
   if (t == T - 1) *count = off + (keep ? 1 : 0);
 }
 
-// packed bf16 hidden rows of the kept tokens; zero rows up to the next multiple of 256
+// Packed bf16 hidden rows of the kept tokens; zero rows up to the next multiple of 256.
+// With ref, also r_t = softcap(<h_t, w_{y_t}>) log2(e) / temperature + 40 of each row.
 template <typename T>
-__global__ void __launch_bounds__(256) gather_kernel(const T* __restrict__ h, long long ldh, int D,
+__global__ void __launch_bounds__(128) gather_kernel(const T* __restrict__ h, long long ldh, int D,
                                                      const int* __restrict__ row_map,
                                                      const int* __restrict__ count,
-                                                     __nv_bfloat16* __restrict__ out, int cap_rows) {
+                                                     __nv_bfloat16* __restrict__ out, int cap_rows,
+                                                     const __nv_bfloat16* __restrict__ w, long long ldw,
+                                                     const int64_t* __restrict__ labels, float k, float cap,
+                                                     float* __restrict__ ref) {
+  __shared__ float s_dot[2][4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = *count;
   const int pad = min(cap_rows, (n + 255) / 256 * 256);
+  int flip = 0;
   for (int r = blockIdx.x; r < pad; r += gridDim.x) {
     uint4* dst = reinterpret_cast<uint4*>(out + static_cast<long long>(r) * D);
     if (r >= n) {
       for (int i = threadIdx.x; i < D / 8; i += blockDim.x) dst[i] = make_uint4(0, 0, 0, 0);
       continue;
     }
-    const T* src = h + static_cast<long long>(row_map[r]) * ldh;
+    const int tok = row_map[r];
+    const T* src = h + static_cast<long long>(tok) * ldh;
+    const uint4* wr = ref != nullptr ? reinterpret_cast<const uint4*>(w + labels[tok] * ldw) : nullptr;
+    float dot = 0.f;
     for (int i = threadIdx.x; i < D / 8; i += blockDim.x) {
+      uint4 u;
       if (sizeof(T) == 2) {
-        dst[i] = reinterpret_cast<const uint4*>(src)[i];
+        u = reinterpret_cast<const uint4*>(src)[i];
       } else {
         const float4 a = reinterpret_cast<const float4*>(src)[2 * i];
         const float4 b = reinterpret_cast<const float4*>(src)[2 * i + 1];
-        dst[i] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y),
-                            pack_bf16x2(b.z, b.w));
+        u = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y),
+                       pack_bf16x2(b.z, b.w));
       }
+      dst[i] = u;
+      if (ref != nullptr) {
+        const uint4 v = wr[i];
+        const uint32_t* up = &u.x;
+        const uint32_t* vp = &v.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 a = unpack_bf16x2(up[j]), b = unpack_bf16x2(vp[j]);
+          dot = fmaf(a.x, b.x, fmaf(a.y, b.y, dot));
+        }
+      }
+    }
+    if (ref != nullptr) {
+      dot = warp_sum(dot);
+      if (lane == 0) s_dot[flip][warp] = dot;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        float a = s_dot[flip][0] + s_dot[flip][1] + s_dot[flip][2] + s_dot[flip][3];
+        if (cap > 0.f) a = cap * tanhf(a / cap);
+        ref[r] = fmaf(a, k, kRefOffset);
+      }
+      flip ^= 1;  // the next row's partial sums go to the other slots
     }
   }
 }
 
-// One warp per row joins the row's (reference, sum) pairs (lane-strided, then a fixed
-// shuffle tree: the same order every run) and writes out = z_label - lse.
+// Joins a row's (reference, sum) pairs (thread-strided, then fixed shuffle trees: the same
+// order every run) and writes out = z_label - lse. WARPS warps take a row: one where rows
+// are many, a block of 8 where a few rows' pairs are all there is to read.
+// For the gradient: lse2, (1 - p_y) softcap'(a_y), and the flag when X leaves bf16's range.
+template <int WARPS>
 __global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ part, int parts, int rows_,
                                                    const int* __restrict__ n_rows,
                                                    const int* __restrict__ row_map,
                                                    const int64_t* __restrict__ labels, long long V,
                                                    long long ignore_index,
-                                                   const float* __restrict__ target, float k,
-                                                   float* __restrict__ out, float* __restrict__ lse2) {
-  const int lane = threadIdx.x & 31;
-  const int nw = gridDim.x * (blockDim.x >> 5);
+                                                   const float* __restrict__ target, float k, float cap,
+                                                   float* __restrict__ out, const float* __restrict__ ref,
+                                                   float* __restrict__ lse2, float* __restrict__ label_grad,
+                                                   int* __restrict__ flag) {
+  __shared__ float2 s_part[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kRows = 8 / WARPS;  // rows of a block
+  const int sub = WARPS == 1 ? lane : threadIdx.x;
   const int rows = n_rows != nullptr ? min(*n_rows, rows_) : rows_;
-  for (int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); row < rows; row += nw) {
-    const float2* p = part + static_cast<long long>(row) * parts;
+  for (int r0 = blockIdx.x * kRows; r0 < rows; r0 += gridDim.x * kRows) {
+    const int row = r0 + (WARPS == 1 ? warp : 0);
     float m = -INFINITY, s = 0.f;
-    for (int i = lane; i < parts; i += 32) {
-      const float2 v = p[i];
-      const float nm = fmaxf(m, v.x), sub = nm == -INFINITY ? 0.f : nm;
-      s = s * ex2(m - sub) + v.y * ex2(v.x - sub);
-      m = nm;
+    if (row < rows) {
+      const float2* p = part + static_cast<long long>(row) * parts;
+#pragma unroll 4
+      for (int i = sub; i < parts; i += 32 * WARPS) {
+        const float2 v = p[i];
+        const float nm = fmaxf(m, v.x), off = nm == -INFINITY ? 0.f : nm;
+        s = s * ex2(m - off) + v.y * ex2(v.x - off);
+        m = nm;
+      }
     }
+    auto join = [&](float om, float os) {
+      const float nm = fmaxf(m, om), off = nm == -INFINITY ? 0.f : nm;
+      s = s * ex2(m - off) + os * ex2(om - off);
+      m = nm;
+    };
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float om = __shfl_xor_sync(0xffffffffu, m, o);
       const float os = __shfl_xor_sync(0xffffffffu, s, o);
-      const float nm = fmaxf(m, om), sub = nm == -INFINITY ? 0.f : nm;
-      s = s * ex2(m - sub) + os * ex2(om - sub);
-      m = nm;
+      join(om, os);
     }
-    if (lane == 0) {
+    if (WARPS > 1) {
+      __syncthreads();
+      if (lane == 0) s_part[warp] = make_float2(m, s);
+      __syncthreads();
+      m = s_part[0].x;
+      s = s_part[0].y;
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) join(s_part[i].x, s_part[i].y);
+    }
+    if (row < rows && sub == 0) {
       const int tok = row_map != nullptr ? row_map[row] : row;
       const int64_t y = labels[tok];
       const float l2 = log2f(s);
@@ -483,21 +635,93 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ pa
       if (y != ignore_index)
         v = (y >= 0 && y < V) ? kLn2 * (fmaf(target[row], k, -m) - l2) : __int_as_float(0x7fc00000);
       out[tok] = v;
-      if (lse2 != nullptr) lse2[row] = m + l2;
+      if (lse2 != nullptr) {
+        const float t = cap > 0.f ? target[row] / cap : 0.f;
+        lse2[row] = m + l2;
+        label_grad[row] = -expm1f(v) * (1.f - t * t);
+        if (ref != nullptr && !(m + l2 - ref[row] <= kRefLimit)) *flag = 1;
+      }
     }
   }
 }
 
-// dh[token] = fp32 compact gradient row in dh's type, zeros for the tokens left out
+// Completes a kept X. Per row: c_t, the bf16 row c_t h_t, the label's entry of X (rounded to
+// bf16) and, for dh, what that rounding left out. Under the flag X has been recomputed as the
+// gradient rows themselves: c_t = 1.
+__global__ void __launch_bounds__(128) scale_rows_kernel(const __nv_bfloat16* __restrict__ h, int D,
+                                                         const int* __restrict__ row_map,
+                                                         const int* __restrict__ count,
+                                                         const int64_t* __restrict__ labels,
+                                                         const float* __restrict__ lse2,
+                                                         const float* __restrict__ label_grad,
+                                                         const float* __restrict__ ref,
+                                                         const float* __restrict__ gout, float inv_temp,
+                                                         __nv_bfloat16* __restrict__ X, long long ldx,
+                                                         float2* __restrict__ factor,
+                                                         __nv_bfloat16* __restrict__ hs, int cap_rows) {
+  const int n = count[0];
+  const bool whole = count[1] != 0;
+  const int pad = min(cap_rows, (n + 255) / 256 * 256);
+  for (int r = blockIdx.x; r < pad; r += gridDim.x) {
+    uint4* dst = reinterpret_cast<uint4*>(hs + static_cast<long long>(r) * D);
+    if (r >= n) {
+      for (int i = threadIdx.x; i < D / 8; i += blockDim.x) dst[i] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const int tok = row_map[r];
+    float c = 1.f;
+    if (!whole) {
+      const float gap = lse2[r] - ref[r], g = gout[tok] * inv_temp;
+      c = -g * exp2f(-gap);
+      if (threadIdx.x == 0) {
+        const __nv_bfloat16 entry = __float2bfloat16(-label_grad[r] * exp2f(gap));
+        X[r * ldx + labels[tok]] = entry;
+        factor[r] = make_float2(c, g * label_grad[r] - c * __bfloat162float(entry));
+      }
+    } else if (threadIdx.x == 0) {
+      factor[r] = make_float2(1.f, 0.f);
+    }
+    const uint4* src = reinterpret_cast<const uint4*>(h + static_cast<long long>(r) * D);
+    for (int i = threadIdx.x; i < D / 8; i += blockDim.x) {
+      uint4 u = src[i];
+      uint32_t* up = &u.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = unpack_bf16x2(up[j]);
+        up[j] = pack_bf16x2(a.x * c, a.y * c);
+      }
+      dst[i] = u;
+    }
+  }
+}
+
+// dh[token] in dh's type from the compact fp32 rows, zeros for the tokens left out; with a
+// kept X, c_t times the row plus the left-out part of the label's entry times its weight row
 template <typename T>
 __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ src,
+                                                      const float2* __restrict__ factor,
+                                                      const __nv_bfloat16* __restrict__ w, long long ldw,
+                                                      const int64_t* __restrict__ labels,
                                                       const int* __restrict__ inverse,
                                                       T* __restrict__ dh, long long tokens, int D) {
   for (long long t = blockIdx.x; t < tokens; t += gridDim.x) {
     const int r = inverse[t];
     const float4* s = reinterpret_cast<const float4*>(src + static_cast<long long>(r < 0 ? 0 : r) * D);
+    const float2 c = r < 0 || factor == nullptr ? make_float2(1.f, 0.f) : factor[r];
+    const uint2* wr = c.y != 0.f ? reinterpret_cast<const uint2*>(w + labels[t] * ldw) : nullptr;
     for (int i = threadIdx.x; i < D / 4; i += blockDim.x) {
-      const float4 v = r < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : s[i];
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r >= 0) {
+        v = s[i];
+        v.x *= c.x; v.y *= c.x; v.z *= c.x; v.w *= c.x;
+        if (wr != nullptr) {
+          const float2 a = unpack_bf16x2(wr[i].x), b = unpack_bf16x2(wr[i].y);
+          v.x = fmaf(c.y, a.x, v.x);
+          v.y = fmaf(c.y, a.y, v.y);
+          v.z = fmaf(c.y, b.x, v.z);
+          v.w = fmaf(c.y, b.y, v.w);
+        }
+      }
       if (sizeof(T) == 2)
         reinterpret_cast<uint2*>(dh + t * D)[i] = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
       else
@@ -506,14 +730,15 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ 
   }
 }
 
-CUtensorMap head_map(const void* base, long long rows, long long cols, long long ld, int box_rows) {
+CUtensorMap head_map(const void* base, long long rows, long long cols, long long ld, int box_cols, int box_rows) {
   CUtensorMap m;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * 2)};
-  cuuint32_t box[2] = {kBK, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = encode_tensor_map(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
-                                 strides, box, estr, CU_TENSOR_MAP_SWIZZLE_128B);
+                                 strides, box, estr,
+                                 box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
   if (r != CUDA_SUCCESS)
     throw std::runtime_error("linear_token_logprobs: cuTensorMapEncodeTiled failed with code " +
                              std::to_string(r));
@@ -527,12 +752,23 @@ int sm_count() {
   return n;
 }
 
-template <int MODE, bool CAP>
-void launch_head(const HeadProblem& p, HeadArgs a, cudaStream_t st) {
-  auto kern = head_kernel<MODE, CAP>;
+template <bool STATS, bool STORE, bool CAP, bool SEG>
+void launch_head(const HeadProblem& p, const HeadArgs& a, void* X, long long ldx, cudaStream_t st) {
+  auto kern = head_kernel<STATS, STORE, CAP, SEG>;
   set_max_smem_once(reinterpret_cast<const void*>(kern), kSmemBytes);
-  const CUtensorMap ta = head_map(p.h, p.rows, p.D, p.ldh, kBM);
-  const CUtensorMap tb = head_map(p.w, p.N, p.D, p.ldw, a.bn / 2);
+  if (SEG) {
+    // the register split waits forever unless the launch owns what the epilogue asks for
+    static const int regs = [&] {
+      cudaFuncAttributes f;
+      PLG_CUDA_CHECK(cudaFuncGetAttributes(&f, kern));
+      return f.numRegs;
+    }();
+    if (kLoadRegs * 128 + kEpiRegs * 32 * kEpiWarps > regs * kThreads)
+      throw std::runtime_error("linear_token_logprobs: the kernel was built with too few registers");
+  }
+  const CUtensorMap ta = head_map(p.h, p.rows, p.D, p.ldh, kBK, kBM);
+  const CUtensorMap tb = head_map(p.w, p.N, p.D, p.ldw, kBK, a.bn / 2);
+  const CUtensorMap tx = STORE ? head_map(X, p.rows, p.N, ldx, 32, 32) : ta;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = kSmemBytes;
@@ -544,10 +780,27 @@ void launch_head(const HeadProblem& p, HeadArgs a, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const long long work = static_cast<long long>(a.m_tiles) * a.n_tiles;
+  const long long work = static_cast<long long>((p.rows + 2 * kBM - 1) / (2 * kBM)) * a.n_tiles;
   const int pairs = static_cast<int>(std::min<long long>(work, head_pairs()));
   cfg.gridDim = dim3(2 * pairs, 1, 1);
-  PLG_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, a));
+  PLG_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, tx, a));
+}
+
+template <bool STATS, bool STORE>
+void dispatch_head(const HeadProblem& p, const HeadArgs& a, void* X, long long ldx, cudaStream_t st) {
+  const bool cap = p.softcap > 0.f;
+  if (STATS && a.segs > 1) {
+    if (cap) launch_head<STATS, STORE, true, STATS>(p, a, X, ldx, st);
+    else launch_head<STATS, STORE, false, STATS>(p, a, X, ldx, st);
+  } else {
+    if (cap) launch_head<STATS, STORE, true, false>(p, a, X, ldx, st);
+    else launch_head<STATS, STORE, false, false>(p, a, X, ldx, st);
+  }
+}
+
+void check_x(const void* X, long long ldx) {
+  if (ldx % 8 || (reinterpret_cast<uintptr_t>(X) & 15))
+    throw std::invalid_argument("linear_token_logprobs: the gradient rows must be 16-byte aligned");
 }
 
 void check_head(const HeadProblem& p) {
@@ -563,8 +816,8 @@ HeadArgs base_args(const HeadProblem& p) {
   a.rows = p.rows;
   a.N = p.N;
   a.k_blocks = (p.D + kBK - 1) / kBK;
+  a.segs = (a.k_blocks + kSegBlocks - 1) / kSegBlocks;
   a.bn = p.bn;
-  a.m_tiles = (p.rows + 2 * kBM - 1) / (2 * kBM);
   a.n_tiles = (p.N + a.bn - 1) / a.bn;
   // the rows of a group of m tiles take at most 32 MB of L2
   const long long tile_bytes = 2LL * kBM * p.D * 2;
@@ -574,7 +827,6 @@ HeadArgs base_args(const HeadProblem& p) {
   a.labels = p.labels;
   a.label0 = p.label0;
   a.k = kLog2e / p.temperature;
-  a.inv_temp = 1.f / p.temperature;
   a.cap = p.softcap;
   a.inv_cap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
   a.status = p.status;
@@ -604,39 +856,64 @@ int head_tile_n(int rows, int N) {
   return best;
 }
 
-void head_stats(const HeadProblem& p, void* part, float* target, cudaStream_t st) {
+void head_stats(const HeadProblem& p, void* part, float* target, const float* ref, void* X, long long ldx,
+                cudaStream_t st) {
   if (p.rows <= 0) return;
   check_head(p);
   HeadArgs a = base_args(p);
   a.part = static_cast<float2*>(part);
   a.target = target;
-  if (p.softcap > 0.f) launch_head<kStats, true>(p, a, st);
-  else launch_head<kStats, false>(p, a, st);
+  if (X != nullptr) {
+    check_x(X, ldx);
+    a.ref = ref;
+    dispatch_head<true, true>(p, a, X, ldx, st);
+  } else {
+    dispatch_head<true, false>(p, a, nullptr, 0, st);
+  }
 }
 
 void head_join(const HeadProblem& p, const void* part, const float* target, long long V,
-               long long ignore_index, float* out, float* lse2, cudaStream_t st) {
+               long long ignore_index, float* out, const float* ref, float* lse2, float* label_grad,
+               int* flag, cudaStream_t st) {
   if (p.rows <= 0) return;
   const int parts = 2 * ((p.N + p.bn - 1) / p.bn);
-  const int blocks = std::min((p.rows + 7) / 8, 148 * 8);
-  join_kernel<<<blocks, 256, 0, st>>>(static_cast<const float2*>(part), parts, p.rows, p.n_rows, p.row_map,
-                                      p.labels, V, ignore_index, target, kLog2e / p.temperature, out, lse2);
+  const float2* pp = static_cast<const float2*>(part);
+  const float k = kLog2e / p.temperature;
+  // a warp per row fills the machine from about 148 * 8 rows on
+  if (p.rows >= 1024)
+    join_kernel<1><<<std::min((p.rows + 7) / 8, 148 * 8), 256, 0, st>>>(
+        pp, parts, p.rows, p.n_rows, p.row_map, p.labels, V, ignore_index, target, k, p.softcap, out, ref, lse2,
+        label_grad, flag);
+  else
+    join_kernel<8><<<p.rows, 256, 0, st>>>(pp, parts, p.rows, p.n_rows, p.row_map, p.labels, V, ignore_index,
+                                           target, k, p.softcap, out, ref, lse2, label_grad, flag);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
-void head_grad(const HeadProblem& p, const float* lse2, const float* gout, void* G, long long ldg,
-               cudaStream_t st) {
+void head_recompute(const HeadProblem& p, const float* lse2, const float* label_grad, const float* gout,
+                    const int* only_if, void* X, long long ldx, cudaStream_t st) {
   if (p.rows <= 0) return;
   check_head(p);
-  if (ldg % 8 || (reinterpret_cast<uintptr_t>(G) & 15))
-    throw std::invalid_argument("linear_token_logprobs: the gradient rows must be 16-byte aligned");
+  check_x(X, ldx);
   HeadArgs a = base_args(p);
-  a.lse2 = lse2;
+  a.ref = lse2;
+  a.label_grad = label_grad;
   a.gout = gout;
-  a.G = static_cast<__nv_bfloat16*>(G);
-  a.ldg = ldg;
-  if (p.softcap > 0.f) launch_head<kGrad, true>(p, a, st);
-  else launch_head<kGrad, false>(p, a, st);
+  a.inv_temp = 1.f / p.temperature;
+  a.only_if = only_if;
+  dispatch_head<false, true>(p, a, X, ldx, st);
+}
+
+void head_scale_rows(const HeadProblem& p, const float* lse2, const float* label_grad, const float* ref,
+                     const float* gout, void* X, long long ldx, float* factor, void* hs, cudaStream_t st) {
+  if (p.rows <= 0) return;
+  if (p.ldh != p.D || p.D % 8)
+    throw std::invalid_argument("linear_token_logprobs: packed rows of a multiple of 8 columns");
+  scale_rows_kernel<<<std::min(p.rows, 148 * 16), 128, 0, st>>>(
+      static_cast<const __nv_bfloat16*>(p.h), p.D, p.row_map, p.n_rows, p.labels, lse2, label_grad, ref, gout,
+      1.f / p.temperature, static_cast<__nv_bfloat16*>(X), ldx, reinterpret_cast<float2*>(factor),
+      static_cast<__nv_bfloat16*>(hs), p.rows);
+  PLG_CUDA_CHECK(cudaGetLastError());
 }
 
 void head_compact(const int64_t* labels, long long T, long long V, long long ignore_index, int* row_map,
@@ -647,32 +924,40 @@ void head_compact(const int64_t* labels, long long T, long long V, long long ign
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
-void head_gather(const void* h, bool fp32, long long ldh, int D, const int* row_map, const int* count,
-                 void* out, int cap_rows, cudaStream_t st) {
+void head_gather(const HeadProblem& p, const void* h, bool fp32, long long ldh, void* out, int cap_rows,
+                 float* ref, cudaStream_t st) {
   if (cap_rows <= 0) return;
-  if (D % 8 || ldh % 8 || ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(out)) & 15))
-    throw std::invalid_argument("linear_token_logprobs: D and hidden's row stride must be multiples of 8, "
+  const int D = p.D;
+  if (D % 8 || ldh % 8 || p.ldw % 8 ||
+      ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p.w)) & 15))
+    throw std::invalid_argument("linear_token_logprobs: D and the row strides must be multiples of 8, "
                                 "rows 16-byte aligned");
   const int blocks = std::min(cap_rows, 148 * 16);
+  const float k = kLog2e / p.temperature;
+  const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(p.w);
   if (fp32)
-    gather_kernel<float><<<blocks, 256, 0, st>>>(static_cast<const float*>(h), ldh, D, row_map, count,
-                                                 static_cast<__nv_bfloat16*>(out), cap_rows);
+    gather_kernel<float><<<blocks, 128, 0, st>>>(static_cast<const float*>(h), ldh, D, p.row_map, p.n_rows,
+                                                 static_cast<__nv_bfloat16*>(out), cap_rows, w, p.ldw, p.labels, k,
+                                                 p.softcap, ref);
   else
-    gather_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(h), ldh, D,
-                                                         row_map, count,
-                                                         static_cast<__nv_bfloat16*>(out), cap_rows);
+    gather_kernel<__nv_bfloat16><<<blocks, 128, 0, st>>>(static_cast<const __nv_bfloat16*>(h), ldh, D, p.row_map,
+                                                         p.n_rows, static_cast<__nv_bfloat16*>(out), cap_rows, w,
+                                                         p.ldw, p.labels, k, p.softcap, ref);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
-void head_scatter(const float* src, const int* inverse, void* dh, bool fp32, long long tokens, int D,
-                  cudaStream_t st) {
+void head_scatter(const HeadProblem& p, const float* src, const float* factor, const int* inverse, void* dh,
+                  bool fp32, long long tokens, cudaStream_t st) {
   if (tokens <= 0) return;
   const int blocks = static_cast<int>(std::min<long long>(tokens, 148 * 16));
+  const float2* f = reinterpret_cast<const float2*>(factor);
+  const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(p.w);
   if (fp32)
-    scatter_kernel<float><<<blocks, 256, 0, st>>>(src, inverse, static_cast<float*>(dh), tokens, D);
+    scatter_kernel<float><<<blocks, 256, 0, st>>>(src, f, w, p.ldw, p.labels, inverse, static_cast<float*>(dh),
+                                                  tokens, p.D);
   else
-    scatter_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(src, inverse, static_cast<__nv_bfloat16*>(dh),
-                                                          tokens, D);
+    scatter_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(src, f, w, p.ldw, p.labels, inverse,
+                                                          static_cast<__nv_bfloat16*>(dh), tokens, p.D);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 

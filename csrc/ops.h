@@ -166,23 +166,35 @@ struct HeadProblem {
 int head_pairs();                       // CTA pairs of the persistent grid
 int head_tile_n(int rows, int N);
 // per row and half tile (reference, sum) pairs: part is float2 [rows][2 * ceil(N / bn)];
-// target [rows] receives the label's logit (after the softcap, before the temperature)
-void head_stats(const HeadProblem& p, void* part, float* target, cudaStream_t stream);
-// out[token] = log-probability of its label (0 where ignored, NaN outside [0, V));
-// lse2 [rows] (optional) = log2 of the row's sum of exponentials
+// target [rows] receives the label's logit (after the softcap, before the temperature).
+// X (optional) bf16 [rows, ldx]: the gradient rows up to a factor, relative to ref [rows]
+void head_stats(const HeadProblem& p, void* part, float* target, const float* ref, void* X, long long ldx,
+                cudaStream_t stream);
+// out[token] = log-probability of its label (0 where ignored, NaN outside [0, V)). For the
+// gradient (lse2 null: none): lse2 [rows] = log2 of the row's sum of exponentials,
+// label_grad [rows] = (1 - p_y) softcap'(a_y), flag = 1 if a row of X left bf16's range
 void head_join(const HeadProblem& p, const void* part, const float* target, long long V,
-               long long ignore_index, float* out, float* lse2, cudaStream_t stream);
-// bf16 G[r, v] = gout[token] * d out / d a[r, v]; zero rows from n_rows to the tile's end
-void head_grad(const HeadProblem& p, const float* lse2, const float* gout, void* G, long long ldg,
-               cudaStream_t stream);
-// row_map [T], inverse [T] (token -> row or -1), count [1], and out = 0 / NaN of the rest
+               long long ignore_index, float* out, const float* ref, float* lse2, float* label_grad,
+               int* flag, cudaStream_t stream);
+// X = the gradient rows themselves; nothing happens unless *only_if (when given)
+void head_recompute(const HeadProblem& p, const float* lse2, const float* label_grad, const float* gout,
+                    const int* only_if, void* X, long long ldx, cudaStream_t stream);
+// Completes a kept X: the labels' entries, hs [rows, D] = bf16(c h) (zero rows up to the
+// tile's end) and factor [rows][2] = c and the part of the label's entry that X lacks
+void head_scale_rows(const HeadProblem& p, const float* lse2, const float* label_grad, const float* ref,
+                     const float* gout, void* X, long long ldx, float* factor, void* hs, cudaStream_t stream);
+// row_map [T], inverse [T] (token -> row or -1), count [2] = {rows, 0}, and out = 0 / NaN of
+// the tokens left out
 void head_compact(const int64_t* labels, long long T, long long V, long long ignore_index, int* row_map,
                   int* inverse, int* count, float* out, cudaStream_t stream);
-// packed bf16 rows of h (bf16 or fp32), zero rows up to a multiple of 256 (at most cap_rows)
-void head_gather(const void* h, bool fp32, long long ldh, int D, const int* row_map, const int* count,
-                 void* out, int cap_rows, cudaStream_t stream);
-void head_scatter(const float* src, const int* inverse, void* dh, bool fp32, long long tokens, int D,
-                  cudaStream_t stream);
+// packed bf16 rows of h (bf16 or fp32), zero rows up to a multiple of 256 (at most cap_rows);
+// ref [rows] (optional): the reference of X
+void head_gather(const HeadProblem& p, const void* h, bool fp32, long long ldh, void* out, int cap_rows,
+                 float* ref, cudaStream_t stream);
+// dh[token] = src row (with factor: times c, plus the missing part times the label's weight
+// row), 0 for the tokens left out
+void head_scatter(const HeadProblem& p, const float* src, const float* factor, const int* inverse, void* dh,
+                  bool fp32, long long tokens, cudaStream_t stream);
 
 // ---------------------------------------------------------------- objectives
 // Paired preference loss over [2, P, S] token log-probabilities (side 0 chosen, 1 rejected;

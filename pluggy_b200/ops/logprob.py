@@ -14,9 +14,11 @@ tile to a (maximum, sum of exponentials) pair per row, so no logits are written;
 backward recomputes them one vocabulary range at a time as the bf16 gradient
 ``g_t * (onehot - softmax)``, whose two products give the gradients. Ranges are split over
 the vocabulary rather than over the tokens so that each row of the weight's gradient is
-written once, in its final type, instead of being summed over chunks of tokens. Tokens
-with ignored labels are packed away on the device first: they cost no products, and
-values in their hidden rows reach no output.
+written once, in its final type, instead of being summed over chunks of tokens. Large
+problems save that second product of hidden and weight: the forward stores bf16
+exponentials, which are the gradient's rows up to a factor for each row. Tokens with ignored
+labels are packed away on the device first: they cost no products, and values in their
+hidden rows reach no output.
 """
 
 from __future__ import annotations
@@ -25,8 +27,12 @@ import torch
 
 from pluggy_b200.ops._ext import ext, status_word
 
-# bytes of the bf16 gradient workspace of one vocabulary range (backward)
-GRAD_WORKSPACE = 2 << 30
+# Bytes of the bf16 matrix, two for each trained token and vocabulary entry, that a call keeps
+# from its forward to its backward, or recomputes at a time
+WORKSPACE = 8 << 30
+# tokens * vocabulary * D from which the matrix is kept: below it the product that this saves
+# takes less than 0.1 ms, and recomputing rounds the weight's gradient once less
+KEEP_PRODUCT = 1 << 36
 # Scoring at most this many tokens skips the packing of the kept ones: up to 256 tokens
 # are one row of tiles, whose time is the head's one pass through memory.
 UNPACKED_ROWS = 256
@@ -57,70 +63,85 @@ def _round_up(n: int, m: int) -> int:
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, labels, ignore_index, w, softcap, temperature, train):
+    def forward(ctx, hidden, weight, labels, ignore_index, w, softcap, temperature, workspace, train):
         T, D = hidden.shape
         V = w.shape[0]
         dev = hidden.device
         out = torch.empty(T, dtype=torch.float32, device=dev)
-        row_map = inverse = count = lse2 = None
-        rows = T
+        row_map = inverse = count = lse2 = label_grad = ref = x = None
         if train or T > UNPACKED_ROWS:
             rows = _round_up(T, 256)
             row_map, inverse = torch.empty((2, T), dtype=torch.int32, device=dev)
-            count = torch.empty(1, dtype=torch.int32, device=dev)
+            count = torch.empty(2, dtype=torch.int32, device=dev)
             ext().head_compact(labels, V, ignore_index, row_map, inverse, count, out)
             h = torch.empty((rows, D), dtype=torch.bfloat16, device=dev)
-            ext().head_gather(hidden, row_map, count, h)
-            lse2 = torch.empty(rows, dtype=torch.float32, device=dev) if train else None
+            if train:
+                lse2, label_grad, ref = torch.empty((3, rows), dtype=torch.float32, device=dev)
+                if 2 * rows * V <= workspace and T * V * D >= KEEP_PRODUCT:
+                    x = torch.empty((rows, _round_up(V, 8)), dtype=torch.bfloat16, device=dev)[:, :V]
+                else:
+                    ref = None
+            ext().head_gather(hidden, w, labels, row_map, count, softcap, temperature, h, ref)
         else:
             h = hidden.to(torch.bfloat16)
         ext().head_logprobs(h, w, labels, ignore_index, row_map, count, softcap, temperature, out,
-                            lse2, status_word(dev))
+                            lse2, label_grad, ref, x, status_word(dev))
         if train:
-            ctx.save_for_backward(h, w, labels, row_map, inverse, count, lse2)
-            ctx.cfg = (softcap, temperature, hidden.dtype, weight.dtype, T)
+            ctx.save_for_backward(h, w, labels, row_map, inverse, count, lse2, label_grad, ref, x)
+            ctx.cfg = (softcap, temperature, workspace, hidden.dtype, weight.dtype, T)
         return out
 
     @staticmethod
     def backward(ctx, gout):
-        h, w, labels, row_map, inverse, count, lse2 = ctx.saved_tensors
-        softcap, temperature, h_dtype, w_dtype, T = ctx.cfg
+        h, w, labels, row_map, inverse, count, lse2, label_grad, ref, x = ctx.saved_tensors
+        softcap, temperature, workspace, h_dtype, w_dtype, T = ctx.cfg
         rows, D = h.shape
         V = w.shape[0]
         dev = h.device
         need_h, need_w = ctx.needs_input_grad[:2]
-        gout = gout.contiguous()
         status = status_word(dev)
-        # equal vocabulary ranges, whole 256-column tiles, within the workspace
-        ranges = max(1, -(-(rows * V * 2) // GRAD_WORKSPACE))
-        width = min(_round_up(V, 8), _round_up(-(-V // ranges), 256))
-        G = torch.empty((rows, width), dtype=torch.bfloat16, device=dev)
+
+        gout = gout.contiguous()
+
+        def recompute(v0, wv, xv, if_flagged):
+            ext().head_recompute(h, wv, v0, labels, row_map, count, softcap, temperature, lse2,
+                                 label_grad, gout, if_flagged, xv, status)
+
+        width, factor, hs = V, None, h
+        if x is not None:
+            recompute(0, w, x, True)  # runs only if a row of x left bf16's range
+            factor = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+            hs = torch.empty_like(h)
+            ext().head_scale_rows(h, w, labels, row_map, count, temperature, lse2, label_grad, ref,
+                                  gout, x, factor, hs)
+        else:
+            if 2 * rows * V > workspace:  # ranges of whole 256-column tiles within the workspace
+                width = max(1, workspace // (2 * rows * 256)) * 256
+            x = torch.empty((rows, _round_up(min(width, V), 8)), dtype=torch.bfloat16, device=dev)
         dh_rows = torch.empty((rows, D), dtype=torch.float32, device=dev) if need_h else None
-        dw = None
-        if need_w:
-            dw = torch.empty((V, D), dtype=w_dtype if w_dtype == torch.bfloat16 else torch.float32,
-                             device=dev)
+        dw = torch.empty((V, D), dtype=w_dtype, device=dev) if need_w else None
         for v0 in range(0, V, width):
             wv = w[v0:v0 + width]
-            g = G[:, :wv.shape[0]]
-            ext().head_grad(h, wv, v0, labels, row_map, count, softcap, temperature, lse2, gout, g,
-                            status)
+            xv = x[:, :wv.shape[0]]
+            if factor is None:
+                recompute(v0, wv, xv, False)
             if need_h:
-                ext().gemm(g, False, wv, True, dh_rows, dh_rows if v0 else None, 1.0,
+                ext().gemm(xv, False, wv, True, dh_rows, dh_rows if v0 else None, 1.0,
                            1.0 if v0 else 0.0, 1, 0, status, count, None)
             if need_w:
-                ext().gemm(g, True, h, True, dw[v0:v0 + width], None, 1.0, 0.0, 1, 0, status, None,
+                ext().gemm(xv, True, hs, True, dw[v0:v0 + width], None, 1.0, 0.0, 1, 0, status, None,
                            count)
         dh = None
         if need_h:
             dh = torch.empty((T, D), dtype=h_dtype, device=dev)
-            ext().head_scatter(dh_rows, inverse, dh)
-        return (dh, dw) + (None,) * 6
+            ext().head_scatter(dh_rows, factor, w, labels, inverse, dh)
+        return (dh, dw) + (None,) * 7
 
 
 def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                           ignore_index: int = -100, *, weight_lowp: torch.Tensor | None = None,
-                          softcap: float | None = None, temperature: float = 1.0) -> torch.Tensor:
+                          softcap: float | None = None, temperature: float = 1.0,
+                          workspace_bytes: int | None = None) -> torch.Tensor:
     """fp32 log-probability of every label under ``softmax(softcap(hidden weight^T) / temperature)``.
 
     ``hidden`` [..., D] and ``weight`` [V, D] are bf16 or fp32, ``labels`` [...] int64 (already
@@ -128,7 +149,9 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: to
     0 where the label is ``ignore_index``; a label outside [0, V) gives NaN and no gradient.
     On CUDA the products are bf16 with fp32 accumulation, as everywhere in this package (an
     fp32 ``weight`` is cast, or ``weight_lowp``, its cached bf16 copy, is read instead), and D
-    must be a multiple of 8. The gradients have the inputs' types."""
+    must be a multiple of 8. The gradients have the inputs' types. ``workspace_bytes`` (8 GiB
+    when None) bounds the bf16 matrix that a training call keeps for its backward: two bytes for
+    each token and vocabulary entry, recomputed in parts where that is more."""
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear_token_logprobs: hidden [..., D] and weight [V, D], got "
                          f"{tuple(hidden.shape)} and {tuple(weight.shape)}")
@@ -162,5 +185,6 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: to
     h, w = _rows_aligned(h), _rows_aligned(w)
     train = torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
     out = _TokenLogprobs.apply(h, weight, labels.reshape(-1).contiguous(), int(ignore_index), w,
-                               float(softcap or 0.0), float(temperature), train)
+                               float(softcap or 0.0), float(temperature),
+                               WORKSPACE if workspace_bytes is None else int(workspace_bytes), train)
     return out.view(labels.shape)
