@@ -36,19 +36,28 @@ const int* count_ptr(const c10::optional<at::Tensor>& c, const at::Tensor& like)
   return c->data_ptr<int>();
 }
 
+int* int_ptr(const at::Tensor& t, int64_t n, const char* name) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() >= n, name,
+              " must be contiguous int32 with at least ", n, " elements");
+  return t.data_ptr<int>();
+}
+
 // C = alpha * op(A) op(B)^T (+ beta * D).
 // a: [M,K] (a_mn_major=false) or [K,M] (true); b: [N,K] or [K,N]; c: [M,N]
 // m_limit / k_limit: device counts of the rows of C / of the summed rows in use (splits 1)
 void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_major, at::Tensor& c,
           const c10::optional<at::Tensor>& d, double alpha, double beta, int64_t splits, int64_t bn,
           const c10::optional<at::Tensor>& status, const c10::optional<at::Tensor>& m_limit,
-          const c10::optional<at::Tensor>& k_limit) {
+          const c10::optional<at::Tensor>& k_limit, const c10::optional<at::Tensor>& split_out) {
   check_cuda(a, "a");
   check_cuda(b, "b");
   check_cuda(c, "c");
   TORCH_CHECK(is_bf16(a) && is_bf16(b), "gemm operands must be bf16");
-  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && c.dim() == 2, "gemm takes 2-D tensors");
-  TORCH_CHECK(a.stride(1) == 1 && b.stride(1) == 1 && c.stride(1) == 1, "gemm needs unit inner stride");
+  // with split_out, c [S, M, N] has room for S k splits stored apart
+  const int cd = split_out.has_value() ? 1 : 0;
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && c.dim() == 2 + cd, "gemm takes 2-D tensors");
+  TORCH_CHECK(a.stride(1) == 1 && b.stride(1) == 1 && c.stride(cd + 1) == 1, "gemm needs unit inner stride");
   TORCH_CHECK(is_bf16(c) || is_f32(c), "gemm output must be bf16 or fp32");
   const c10::cuda::CUDAGuard guard(a.device());
   plg::GemmProblem p;
@@ -57,7 +66,7 @@ void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_m
   p.N = static_cast<int>(b_mn_major ? b.size(1) : b.size(0));
   const int kb = static_cast<int>(b_mn_major ? b.size(0) : b.size(1));
   TORCH_CHECK(kb == p.K, "gemm: K mismatch (", p.K, " vs ", kb, ")");
-  TORCH_CHECK(c.size(0) == p.M && c.size(1) == p.N, "gemm: C must be [M, N]");
+  TORCH_CHECK(c.size(cd) == p.M && c.size(cd + 1) == p.N, "gemm: C must be [M, N]");
   p.A = a.data_ptr();
   p.lda = a.stride(0);
   p.a_mn_major = a_mn_major;
@@ -65,8 +74,14 @@ void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_m
   p.ldb = b.stride(0);
   p.b_mn_major = b_mn_major;
   p.C = c.data_ptr();
-  p.ldc = c.stride(0);
+  p.ldc = c.stride(cd);
   p.c_fp32 = is_f32(c);
+  if (split_out.has_value()) {
+    TORCH_CHECK(c.is_contiguous() && c.size(0) >= 1 && c.size(0) <= 64, "gemm: 1..64 contiguous splits");
+    p.max_split = static_cast<int>(c.size(0));
+    p.split_stride = c.stride(0);
+    p.split_out = int_ptr(*split_out, 1, "split_out");
+  }
   if (d.has_value() && beta != 0.0) {
     check_cuda(*d, "d");
     TORCH_CHECK(d->dim() == 2 && d->size(0) == p.M && d->size(1) == p.N && d->stride(1) == 1,
@@ -402,13 +417,6 @@ const int64_t* labels_ptr(const at::Tensor& labels) {
   return labels.data_ptr<int64_t>();
 }
 
-int* int_ptr(const at::Tensor& t, int64_t n, const char* name) {
-  check_cuda(t, name);
-  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() >= n, name,
-              " must be contiguous int32 with at least ", n, " elements");
-  return t.data_ptr<int>();
-}
-
 float* float_ptr(const at::Tensor& t, int64_t n, const char* name) {
   check_cuda(t, name);
   TORCH_CHECK(is_f32(t) && t.is_contiguous() && t.numel() >= n, name,
@@ -422,7 +430,7 @@ void head_compact_b(const at::Tensor& labels, int64_t V, int64_t ignore_index, a
   TORCH_CHECK(T <= INT32_MAX - 256, "linear_token_logprobs: too many tokens in one call");
   const c10::cuda::CUDAGuard guard(labels.device());
   plg::head_compact(labels_ptr(labels), T, V, ignore_index, int_ptr(row_map, T, "row_map"),
-                    int_ptr(inverse, T, "inverse"), int_ptr(count, 2, "count"), float_ptr(out, T, "out"),
+                    int_ptr(inverse, T, "inverse"), int_ptr(count, 3, "count"), float_ptr(out, T, "out"),
                     cur_stream());
 }
 
@@ -450,7 +458,7 @@ plg::HeadProblem head_problem(const at::Tensor& h, const at::Tensor& w, const at
   p.labels = labels_ptr(labels);
   if (row_map.has_value()) {
     p.row_map = int_ptr(*row_map, labels.numel(), "row_map");
-    p.n_rows = int_ptr(*count, 2, "count");
+    p.n_rows = int_ptr(*count, 3, "count");
   } else {
     TORCH_CHECK(labels.numel() == p.rows, "linear_token_logprobs: one label per row");
   }
@@ -537,11 +545,13 @@ void head_scale_rows_b(const at::Tensor& h, const at::Tensor& w, const at::Tenso
                        hs.data_ptr(), cur_stream());
 }
 
-void head_scatter_b(const at::Tensor& src, const c10::optional<at::Tensor>& factor, const at::Tensor& w,
+// src [S, rows, D] fp32, of which the first count[2] parts are summed
+void head_scatter_b(const at::Tensor& src, const at::Tensor& count, const c10::optional<at::Tensor>& factor,
+                    const at::Tensor& w,
                     const at::Tensor& labels, const at::Tensor& inverse, at::Tensor& dh) {
   check_cuda(dh, "dh");
-  TORCH_CHECK(dh.dim() == 2 && dh.is_contiguous() && (is_bf16(dh) || is_f32(dh)) && src.dim() == 2 &&
-                  src.size(1) == dh.size(1) && dh.size(1) % 8 == 0 && labels.numel() == dh.size(0) &&
+  TORCH_CHECK(dh.dim() == 2 && dh.is_contiguous() && (is_bf16(dh) || is_f32(dh)) && src.dim() == 3 &&
+                  src.size(2) == dh.size(1) && dh.size(1) % 8 == 0 && labels.numel() == dh.size(0) &&
                   is_bf16(w) && w.dim() == 2 && w.size(1) == dh.size(1),
               "head_scatter: dh contiguous [T, D] bf16 or fp32, src [rows, D], w bf16 [V, D]");
   const c10::cuda::CUDAGuard guard(dh.device());
@@ -550,8 +560,8 @@ void head_scatter_b(const at::Tensor& src, const c10::optional<at::Tensor>& fact
   p.w = w.data_ptr();
   p.ldw = w.stride(0);
   p.labels = labels_ptr(labels);
-  plg::head_scatter(p, float_ptr(src, src.numel(), "src"),
-                    factor.has_value() ? float_ptr(*factor, 2 * src.size(0), "factor") : nullptr,
+  plg::head_scatter(p, float_ptr(src, src.numel(), "src"), src.stride(0), int_ptr(count, 3, "count") + 2,
+                    factor.has_value() ? float_ptr(*factor, 2 * src.size(1), "factor") : nullptr,
                     int_ptr(inverse, dh.size(0), "inverse"), dh.data_ptr(), is_f32(dh), dh.size(0),
                     cur_stream());
 }
@@ -1210,7 +1220,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "pluggy_b200 sm_100a kernels";
   m.def("gemm", &gemm, py::arg("a"), py::arg("a_mn_major"), py::arg("b"), py::arg("b_mn_major"),
         py::arg("c"), py::arg("d"), py::arg("alpha"), py::arg("beta"), py::arg("splits"), py::arg("bn"),
-        py::arg("status"), py::arg("m_limit") = py::none(), py::arg("k_limit") = py::none());
+        py::arg("status"), py::arg("m_limit") = py::none(), py::arg("k_limit") = py::none(),
+        py::arg("split_out") = py::none());
   m.def("preference_fwd", &preference_fwd);
   m.def("preference_bwd", &preference_bwd);
   m.def("policy_fwd", &policy_fwd);

@@ -67,7 +67,28 @@ struct Args {
   int grp_count;         // mode 2: number of groups
   const int* m_limit;    // device row count of C (null: M)
   const int* k_limit;    // device length of the sum (null: K)
+  int max_split;         // > 1: k splits chosen here and stored apart
+  long long split_stride;
+  int* split_out;
 };
+
+// K splits of `tiles` output tiles over `slots` CTA pairs: the smallest modelled time
+// waves / s, where each further split adds 8 bytes per output to 2 K operations (about
+// 1100 / K of the time) and keeps at least 8 k blocks.
+__device__ __forceinline__ int pick_splits(int tiles, int slots, int k_blocks, int max_split) {
+  int best = 1;
+  float best_cost = 3.4e38f;
+  const float extra = 1100.f / (64.f * k_blocks);
+  for (int s = 1; s <= max_split && (s == 1 || k_blocks / s >= 8); ++s) {
+    const float cost = static_cast<float>((tiles * s + slots - 1) / slots) / s * (1.f + extra * (s - 1));
+    // every split must own at least one k block
+    if (cost < best_cost && (s - 1) * ((k_blocks + s - 1) / s) < k_blocks) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
 
 // m tiles and k blocks in use under the device limits
 __device__ __forceinline__ void limited_extent(const Args& args, int tile_m, int& m_tiles,
@@ -580,11 +601,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   int m_tiles, k_blocks;
   limited_extent(args, 2 * BM, m_tiles, k_blocks);
   const int total_tiles = m_tiles * args.n_tiles;  // 256 x 256 tiles
-  const int total_work = total_tiles * args.splits;
-  const int kb_per_split = (k_blocks + args.splits - 1) / args.splits;
+  const int splits = args.max_split > 1 ? pick_splits(total_tiles, npairs, k_blocks, args.max_split)
+                                        : args.splits;
+  if (args.max_split > 1 && blockIdx.x == 0 && threadIdx.x == 0) *args.split_out = splits;
+  const int total_work = total_tiles * splits;
+  const int kb_per_split = (k_blocks + splits - 1) / splits;
   auto decode = [&](int w, int& mt, int& nt, int& kb0, int& kb1) {
-    const int tile = w / args.splits;
-    const int sp = w - tile * args.splits;
+    const int tile = w / splits;
+    const int sp = w - tile * splits;
     if (args.raster_m) {
       mt = tile % m_tiles;
       nt = tile / m_tiles;
@@ -732,7 +756,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const long long row = (long long)mt * 2 * BM + rank * BM + row_in_tile;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
-      store_acc_row<BN>(args, t_row, row, row < args.M, nt * BN, kb0, epi_stage + q * 32 * 128,
+      // splits stored apart: split i's rows follow at i * split_stride (whole rows of C)
+      const long long crow =
+          args.max_split > 1 ? row + kb0 / max(kb_per_split, 1) * (args.split_stride / args.ldc) : row;
+      store_acc_row<BN>(args, t_row, crow, row < args.M, nt * BN, kb0, epi_stage + q * 32 * 128,
                         kb1 <= kb0);
       tc_fence_before();
       __syncwarp();
@@ -911,6 +938,9 @@ static void launch_pair(const GemmProblem& p, cudaStream_t stream) {
   a.status = p.status;
   a.m_limit = p.m_limit;
   a.k_limit = p.k_limit;
+  a.max_split = p.max_split;
+  a.split_stride = p.split_stride;
+  a.split_out = p.split_out;
   set_rs_fields(p, a, 2 * BM);
   auto kern = gemm_pair_kernel<A_MN, B_MN>;
   set_max_smem_once(reinterpret_cast<const void*>(kern), C_::kSmemBytes);
@@ -953,8 +983,8 @@ static void launch_pair(const GemmProblem& p, cudaStream_t stream) {
     }
   }
   a.raster_m = (static_cast<long long>(p.N) > static_cast<long long>(p.M)) ? 1 : 0;
-  const int work = tiles * splits;
-  const int nclusters = work < pairs ? work : pairs;
+  const long long work = static_cast<long long>(tiles) * (p.max_split > 1 ? p.max_split : splits);
+  const int nclusters = work < pairs ? static_cast<int>(work) : pairs;
   cfg.gridDim = dim3(2 * nclusters, 1, 1);
   PLG_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, a));
 }
@@ -985,6 +1015,9 @@ void gemm_bf16(const GemmProblem& p, cudaStream_t stream) {
   }
   if ((p.m_limit != nullptr || p.k_limit != nullptr) && (p.grp_mode || p.rs_n || p.allow_split))
     throw std::invalid_argument("gemm: device row counts need an ungrouped product without split-K");
+  if (p.max_split > 1 && (!p.c_fp32 || p.D != nullptr || p.allow_split || p.split_out == nullptr ||
+                          p.split_stride < (long long)p.M * p.ldc || p.split_stride % p.ldc || p.grp_mode || p.rs_n))
+    throw std::invalid_argument("gemm: k splits stored apart need a plain fp32 output with room for each");
   const bool wide = p.N >= 256 && p.bn != 128;
   // large problems: 256 x 256 tiles on SM pairs (bn == 256 keeps the one-SM kernel)
   const bool pair = wide && p.bn == 0 && p.M >= 256 && num_sms() >= 2 && !p.grp_mode;

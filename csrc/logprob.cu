@@ -55,9 +55,9 @@ constexpr float kRefOffset = 40.f;   // r_t - z_y log2e
 constexpr float kRefLimit = 100.f;   // lse2 - r_t beyond which X is recomputed
 // Reduction length of one accumulator of the statistics: the tensor cores truncate each
 // addition, a bias of about 1e-9 of the sum per column of D (measured: 2.5e-6 of a logit at
-// D = 2560, 5e-7 at 512, where an fp32 chain's own rounding is as large), so longer sums
-// are cut into pieces that the epilogue adds in fp32.
-constexpr int kSegBlocks = 512 / kBK;
+// D = 2560, 1e-6 at 1024; an fp32 chain's rounding is about 5e-7), so longer sums are cut
+// into pieces that the epilogue adds in fp32. Pieces of 512 cost 17% of the time at D = 1024.
+constexpr int kSegBlocks = 1024 / kBK;
 
 struct HeadArgs {
   int rows, N, k_blocks, segs;
@@ -473,7 +473,10 @@ __global__ void __launch_bounds__(kScan) compact_kernel(const int64_t* __restric
                                                         float* __restrict__ out) {
   __shared__ int s_warp[32];
   __shared__ int s_base;
-  if (blockIdx.x == 0 && threadIdx.x == 0) count[1] = 0;  // the flag that join_kernel may set
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    count[1] = 0;  // the flag that join_kernel may set
+    count[2] = 1;  // k splits of dh's product, which may choose more
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long b0 = static_cast<long long>(blockIdx.x) * kScan;
   int before = 0;
@@ -695,15 +698,17 @@ __global__ void __launch_bounds__(128) scale_rows_kernel(const __nv_bfloat16* __
   }
 }
 
-// dh[token] in dh's type from the compact fp32 rows, zeros for the tokens left out; with a
-// kept X, c_t times the row plus the left-out part of the label's entry times its weight row
+// dh[token] in dh's type from the compact fp32 rows (the sum of the product's k splits, in
+// their order), zeros for the tokens left out; with a kept X, c_t times the row plus the left-out part of the label's entry times its weight row
 template <typename T>
-__global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ src,
+__global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ src, long long split_stride,
+                                                      const int* __restrict__ splits,
                                                       const float2* __restrict__ factor,
                                                       const __nv_bfloat16* __restrict__ w, long long ldw,
                                                       const int64_t* __restrict__ labels,
                                                       const int* __restrict__ inverse,
                                                       T* __restrict__ dh, long long tokens, int D) {
+  const int ns = *splits;
   for (long long t = blockIdx.x; t < tokens; t += gridDim.x) {
     const int r = inverse[t];
     const float4* s = reinterpret_cast<const float4*>(src + static_cast<long long>(r < 0 ? 0 : r) * D);
@@ -713,6 +718,10 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ 
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r >= 0) {
         v = s[i];
+        for (int k = 1; k < ns; ++k) {
+          const float4 a = s[i + k * (split_stride / 4)];
+          v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+        }
         v.x *= c.x; v.y *= c.x; v.z *= c.x; v.w *= c.x;
         if (wr != nullptr) {
           const float2 a = unpack_bf16x2(wr[i].x), b = unpack_bf16x2(wr[i].y);
@@ -946,18 +955,20 @@ void head_gather(const HeadProblem& p, const void* h, bool fp32, long long ldh, 
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
-void head_scatter(const HeadProblem& p, const float* src, const float* factor, const int* inverse, void* dh,
-                  bool fp32, long long tokens, cudaStream_t st) {
+void head_scatter(const HeadProblem& p, const float* src, long long split_stride, const int* splits,
+                  const float* factor, const int* inverse, void* dh, bool fp32, long long tokens,
+                  cudaStream_t st) {
   if (tokens <= 0) return;
   const int blocks = static_cast<int>(std::min<long long>(tokens, 148 * 16));
   const float2* f = reinterpret_cast<const float2*>(factor);
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(p.w);
   if (fp32)
-    scatter_kernel<float><<<blocks, 256, 0, st>>>(src, f, w, p.ldw, p.labels, inverse, static_cast<float*>(dh),
-                                                  tokens, p.D);
+    scatter_kernel<float><<<blocks, 256, 0, st>>>(src, split_stride, splits, f, w, p.ldw, p.labels, inverse,
+                                                  static_cast<float*>(dh), tokens, p.D);
   else
-    scatter_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(src, f, w, p.ldw, p.labels, inverse,
-                                                          static_cast<__nv_bfloat16*>(dh), tokens, p.D);
+    scatter_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(src, split_stride, splits, f, w, p.ldw, p.labels,
+                                                          inverse, static_cast<__nv_bfloat16*>(dh), tokens,
+                                                          p.D);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 

@@ -55,6 +55,12 @@ struct GemmProblem {
   // count of 0 writes zeros).
   const int* m_limit = nullptr;
   const int* k_limit = nullptr;
+  // K splits stored apart: the kernel picks s <= max_split from the rows in use, split i's
+  // fp32 sums go to C + i * split_stride and s to *split_out (256 x 256 tiles only; other
+  // problems leave *split_out alone and write C)
+  int max_split = 1;
+  long long split_stride = 0;
+  int* split_out = nullptr;
 };
 void gemm_bf16(const GemmProblem& p, cudaStream_t stream);
 
@@ -183,7 +189,7 @@ void head_recompute(const HeadProblem& p, const float* lse2, const float* label_
 // tile's end) and factor [rows][2] = c and the part of the label's entry that X lacks
 void head_scale_rows(const HeadProblem& p, const float* lse2, const float* label_grad, const float* ref,
                      const float* gout, void* X, long long ldx, float* factor, void* hs, cudaStream_t stream);
-// row_map [T], inverse [T] (token -> row or -1), count [2] = {rows, 0}, and out = 0 / NaN of
+// row_map [T], inverse [T] (token -> row or -1), count [3] = {rows, 0, 1}, and out = 0 / NaN of
 // the tokens left out
 void head_compact(const int64_t* labels, long long T, long long V, long long ignore_index, int* row_map,
                   int* inverse, int* count, float* out, cudaStream_t stream);
@@ -191,10 +197,11 @@ void head_compact(const int64_t* labels, long long T, long long V, long long ign
 // ref [rows] (optional): the reference of X
 void head_gather(const HeadProblem& p, const void* h, bool fp32, long long ldh, void* out, int cap_rows,
                  float* ref, cudaStream_t stream);
-// dh[token] = src row (with factor: times c, plus the missing part times the label's weight
+// dh[token] = src row, summed over *splits parts (with factor: times c, plus the missing part times the label's weight
 // row), 0 for the tokens left out
-void head_scatter(const HeadProblem& p, const float* src, const float* factor, const int* inverse, void* dh,
-                  bool fp32, long long tokens, cudaStream_t stream);
+void head_scatter(const HeadProblem& p, const float* src, long long split_stride, const int* splits,
+                  const float* factor, const int* inverse, void* dh, bool fp32, long long tokens,
+                  cudaStream_t stream);
 
 // ---------------------------------------------------------------- objectives
 // Paired preference loss over [2, P, S] token log-probabilities (side 0 chosen, 1 rejected;

@@ -33,6 +33,8 @@ WORKSPACE = 8 << 30
 # tokens * vocabulary * D from which the matrix is kept: below it the product that this saves
 # takes less than 0.1 ms, and recomputing rounds the weight's gradient once less
 KEEP_PRODUCT = 1 << 36
+# bytes of the k splits' fp32 sums of the hidden rows' gradient
+SPLIT_WORKSPACE = 512 << 20
 # Scoring at most this many tokens skips the packing of the kept ones: up to 256 tokens
 # are one row of tiles, whose time is the head's one pass through memory.
 UNPACKED_ROWS = 256
@@ -72,7 +74,7 @@ class _TokenLogprobs(torch.autograd.Function):
         if train or T > UNPACKED_ROWS:
             rows = _round_up(T, 256)
             row_map, inverse = torch.empty((2, T), dtype=torch.int32, device=dev)
-            count = torch.empty(2, dtype=torch.int32, device=dev)
+            count = torch.empty(3, dtype=torch.int32, device=dev)  # rows, flag, splits
             ext().head_compact(labels, V, ignore_index, row_map, inverse, count, out)
             h = torch.empty((rows, D), dtype=torch.bfloat16, device=dev)
             if train:
@@ -118,15 +120,20 @@ class _TokenLogprobs(torch.autograd.Function):
             if 2 * rows * V > workspace:  # ranges of whole 256-column tiles within the workspace
                 width = max(1, workspace // (2 * rows * 256)) * 256
             x = torch.empty((rows, _round_up(min(width, V), 8)), dtype=torch.bfloat16, device=dev)
-        dh_rows = torch.empty((rows, D), dtype=torch.float32, device=dev) if need_h else None
+        # dh's product has few tiles and a long sum: one range's k splits are summed by scatter
+        splits = max(1, min(16, SPLIT_WORKSPACE // (4 * rows * D))) if width >= V else 1
+        dh_rows = torch.empty((splits, rows, D), dtype=torch.float32, device=dev) if need_h else None
         dw = torch.empty((V, D), dtype=w_dtype, device=dev) if need_w else None
         for v0 in range(0, V, width):
             wv = w[v0:v0 + width]
             xv = x[:, :wv.shape[0]]
             if factor is None:
                 recompute(v0, wv, xv, False)
-            if need_h:
-                ext().gemm(xv, False, wv, True, dh_rows, dh_rows if v0 else None, 1.0,
+            if need_h and splits > 1:
+                ext().gemm(xv, False, wv, True, dh_rows, None, 1.0, 0.0, 1, 0, status, count, None,
+                           count[2:])
+            elif need_h:
+                ext().gemm(xv, False, wv, True, dh_rows[0], dh_rows[0] if v0 else None, 1.0,
                            1.0 if v0 else 0.0, 1, 0, status, count, None)
             if need_w:
                 ext().gemm(xv, True, hs, True, dw[v0:v0 + width], None, 1.0, 0.0, 1, 0, status, None,
@@ -134,7 +141,7 @@ class _TokenLogprobs(torch.autograd.Function):
         dh = None
         if need_h:
             dh = torch.empty((T, D), dtype=h_dtype, device=dev)
-            ext().head_scatter(dh_rows, factor, w, labels, inverse, dh)
+            ext().head_scatter(dh_rows, count, factor, w, labels, inverse, dh)
         return (dh, dw) + (None,) * 7
 
 
