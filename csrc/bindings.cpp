@@ -504,7 +504,7 @@ void head_logprobs_b(const at::Tensor& h, const at::Tensor& w, const at::Tensor&
   TORCH_CHECK(ref.has_value() == x.has_value() && lse2.has_value() == label_grad.has_value() &&
                   (!x.has_value() || (lse2.has_value() && count.has_value())),
               "head_logprobs: x goes with ref, both with the gradient's row statistics and packed rows");
-  const int64_t parts = 2 * ((p.N + p.bn - 1) / p.bn);
+  const int64_t parts = plg::head_parts(p);
   // workspace: the rows' (reference, sum) pairs and their labels' logits
   at::Tensor part = at::empty({static_cast<int64_t>(p.rows) * (2 * parts + 1)}, out.options());
   float* target = part.data_ptr<float>() + 2 * parts * p.rows;

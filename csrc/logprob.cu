@@ -458,6 +458,261 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// Scoring at most 128 rows is one pass through the head, bound by its bytes. Here the roles
+// are swapped: 128 vocabulary entries are the tensor core's rows and the NT (32, 64 or 128)
+// hidden rows its columns, so that an MMA costs in proportion to the rows in use. CTA c takes
+// the entries [V c / CTAs, V (c + 1) / CTAs), equal shares of the bytes for every SM, in
+// equal tiles of at most 128 entries (256-column tiles leave 11 waves of 8 for 594 tiles).
+// Accumulator lane = entry, column = hidden row: a warp reduces 32 entries x 32 rows by
+// exchanging halves (31 shuffles instead of 160), which leaves lane j with row j's result,
+// and keeps each row's running (reference, sum) there. One pair per row, CTA and quadrant.
+constexpr int kThinThreads = 192;
+constexpr int kThinEntries = 128;
+
+template <int NT>
+struct Thin {
+  static constexpr int kA = kThinEntries * kBK * 2;
+  static constexpr int kB = NT * kBK * 2;
+  static constexpr int kStages = NT == 128 ? 6 : (NT == 64 ? 8 : 10);
+  static constexpr int kSmem = kStages * (kA + kB) + 1024 + 256;
+};
+
+struct ThinArgs {
+  int T, V, tile, k_blocks, segs;
+  const int64_t* labels;
+  float k, cap, inv_cap;
+  float2* part;   // [T][4 * CTAs]
+  float* target;  // [T]
+  int* status;
+};
+
+// lane j of the result = op over the lanes of column j: each step keeps one half of the
+// columns and trades the other half with the lane whose index differs in that bit
+template <typename Op>
+__device__ __forceinline__ float transpose_reduce(const float (&v)[32], int lane, Op op) {
+  float t[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const bool hi = lane & 16;
+    const float send = hi ? v[i] : v[i + 16], keep = hi ? v[i + 16] : v[i];
+    t[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, 16));
+  }
+#pragma unroll
+  for (int w = 8; w >= 1; w >>= 1) {
+    const bool hi = lane & w;
+#pragma unroll
+    for (int i = 0; i < w; ++i) {
+      const float send = hi ? t[i] : t[i + w], keep = hi ? t[i + w] : t[i];
+      t[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, w));
+    }
+  }
+  return t[0];
+}
+
+template <int NT, bool CAP>
+__global__ void __launch_bounds__(kThinThreads, 1)
+    thin_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmH,
+                const ThinArgs args) {
+  using C_ = Thin<NT>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C_::kStages * (C_::kA + C_::kB));
+  uint64_t* full_bar = bar;
+  uint64_t* empty_bar = bar + C_::kStages;
+  uint64_t* accf_bar = bar + 2 * C_::kStages;      // [2]
+  uint64_t* acce_bar = bar + 2 * C_::kStages + 2;  // [2]
+  uint64_t* done_bar = bar + 2 * C_::kStages + 4;
+  uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(bar + 2 * C_::kStages + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_smem + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C_::kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accf_bar[b], 1);
+      mbar_init(&acce_bar[b], 4);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_base_smem, 2 * NT);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_smem;
+  const int v0 = static_cast<int>(static_cast<long long>(args.V) * blockIdx.x / gridDim.x);
+  const int v1 = static_cast<int>(static_cast<long long>(args.V) * (blockIdx.x + 1) / gridDim.x);
+  const int tiles = (v1 - v0 + args.tile - 1) / args.tile;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, parity = 0;
+      bool ok = true;
+      const uint32_t bytes = args.tile * kBK * 2 + C_::kB;
+      for (int i = 0; i < tiles && ok; ++i) {
+        for (int kb = 0; kb < args.k_blocks; ++kb) {
+          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+            record_status(args.status, kTimeoutSmemEmpty);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          uint8_t* sA = smem + stage * (C_::kA + C_::kB);
+          mbar_arrive_expect_tx(&full_bar[stage], bytes);
+          tma_load_2d(sA, &tmW, &full_bar[stage], kb * kBK, v0 + i * args.tile);
+          tma_load_2d(sA + C_::kA, &tmH, &full_bar[stage], kb * kBK, 0);
+          issued |= 1u << stage;
+          parity = (parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == C_::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        for (int s = 0; s < C_::kStages; ++s)
+          if (((issued >> s) & 1u) && !mbar_wait_bounded(&full_bar[s], (parity >> s) & 1u, nullptr))
+            record_status(args.status, kTimeoutDrain);
+      }
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_bf16_f32(kThinEntries, NT, false, false);
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        for (int seg = 0; seg < args.segs && ok; ++seg, ++local) {
+          const int kb0 = seg * args.k_blocks / args.segs, kb1 = (seg + 1) * args.k_blocks / args.segs;
+          const int buf = local & 1;
+          if (!mbar_wait_bounded(&acce_bar[buf], ((local >> 1) & 1) ^ 1u, abort_flag)) {
+            record_status(args.status, kTimeoutAccEmpty);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag)) {
+              record_status(args.status, kTimeoutTmaFull);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sA = smem_u32(smem + stage * (C_::kA + C_::kB));
+            const uint64_t da = make_smem_desc(sA, 16, 1024, kLayoutSW128);
+            const uint64_t db = make_smem_desc(sA + C_::kA, 16, 1024, kLayoutSW128);
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk)
+              tc_mma_ss(tmem_base + buf * NT, desc_advance(da, kk * 32), desc_advance(db, kk * 32), idesc,
+                        (kb > kb0 || kk > 0) ? 1u : 0u);
+            tc_commit(&empty_bar[stage]);
+            if (++stage == C_::kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          if (ok) tc_commit(&accf_bar[buf]);
+        }
+      }
+      tc_commit(done_bar);
+      if (!mbar_wait_bounded(done_bar, 0, nullptr)) record_status(args.status, kTimeoutDrain);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    constexpr int kCh = NT / 32;
+    const int q = warp & 3;
+    float ref[kCh], sum[kCh];
+    int lab[kCh];  // the label of hidden row 32 c + lane (never in a tile if there is none)
+#pragma unroll
+    for (int c = 0; c < kCh; ++c) {
+      ref[c] = -INFINITY;
+      sum[c] = 0.f;
+      lab[c] = -1;
+      if (c * 32 + lane < args.T) {
+        const int64_t y = args.labels[c * 32 + lane];
+        lab[c] = y >= 0 && y < args.V ? static_cast<int>(y) : -1;
+      }
+    }
+    int local = 0;
+    bool ok = true;
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int e0 = v0 + i * args.tile + q * 32;              // the warp's first entry
+      const int end = min(v1, v0 + (i + 1) * args.tile);       // of the tile
+      float acc[kCh][32];
+      for (int seg = 0; seg < args.segs; ++seg, ++local) {
+        const int buf = local & 1;
+        if (!mbar_wait_bounded(&accf_bar[buf], (local >> 1) & 1, abort_flag)) {
+          record_status(args.status, kTimeoutAccFull);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kCh; ++c) {
+          uint32_t r[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * NT + c * 32, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c][j] = __uint_as_float(r[j]) + (seg == 0 ? 0.f : acc[c][j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acce_bar[buf]);
+      }
+      if (!ok || e0 >= end) continue;
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) {
+        if (c * 32 >= args.T) continue;
+        float(&v)[32] = acc[c];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          if (CAP) v[j] = args.cap * tanhf(v[j] * args.inv_cap);
+          if (e0 + lane >= end) v[j] = -INFINITY;
+        }
+        if (__any_sync(0xffffffffu, lab[c] >= e0 && lab[c] < min(e0 + 32, end))) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (__shfl_sync(0xffffffffu, lab[c], j) == e0 + lane && e0 + lane < end)
+              args.target[c * 32 + j] = v[j];
+        }
+        const float m = transpose_reduce(v, lane, [](float a, float b) { return fmaxf(a, b); });
+        const float nref = fmaxf(ref[c], m * args.k);
+        const float sub = nref == -INFINITY ? 0.f : nref;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          v[j] = ex2(fmaf(v[j], args.k, -__shfl_sync(0xffffffffu, sub, j)));
+        const float s = transpose_reduce(v, lane, [](float a, float b) { return a + b; });
+        sum[c] = sum[c] * ex2(ref[c] - sub) + s;
+        ref[c] = nref;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kCh; ++c)
+      if (c * 32 + lane < args.T)
+        args.part[(c * 32 + lane) * (4LL * gridDim.x) + 4 * blockIdx.x + q] = make_float2(ref[c], sum[c]);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * NT);
+  }
+}
+
 // ---------------------------------------------------------------- small kernels
 constexpr int kScan = 1024;
 
@@ -807,6 +1062,22 @@ void dispatch_head(const HeadProblem& p, const HeadArgs& a, void* X, long long l
   }
 }
 
+template <int NT, bool CAP>
+void launch_thin(const HeadProblem& p, const ThinArgs& a, int ctas, cudaStream_t st) {
+  auto kern = thin_kernel<NT, CAP>;
+  set_max_smem_once(reinterpret_cast<const void*>(kern), Thin<NT>::kSmem);
+  const CUtensorMap tw = head_map(p.w, p.N, p.D, p.ldw, kBK, a.tile);
+  const CUtensorMap th = head_map(p.h, p.rows, p.D, p.ldh, kBK, NT);
+  kern<<<ctas, kThinThreads, Thin<NT>::kSmem, st>>>(tw, th, a);
+  PLG_CUDA_CHECK(cudaGetLastError());
+}
+
+template <int NT>
+void dispatch_thin(const HeadProblem& p, const ThinArgs& a, int ctas, cudaStream_t st) {
+  if (p.softcap > 0.f) launch_thin<NT, true>(p, a, ctas, st);
+  else launch_thin<NT, false>(p, a, ctas, st);
+}
+
 void check_x(const void* X, long long ldx) {
   if (ldx % 8 || (reinterpret_cast<uintptr_t>(X) & 15))
     throw std::invalid_argument("linear_token_logprobs: the gradient rows must be 16-byte aligned");
@@ -865,10 +1136,42 @@ int head_tile_n(int rows, int N) {
   return best;
 }
 
+// CTAs of the few-rows kernel: one per SM, each with at least 32 entries
+static int thin_ctas(int V) { return std::max(1, std::min(sm_count(), V / 32)); }
+
+bool head_is_thin(const HeadProblem& p) { return p.n_rows == nullptr && p.rows <= kThinRows; }
+
+int head_parts(const HeadProblem& p) {
+  return head_is_thin(p) ? 4 * thin_ctas(p.N) : 2 * ((p.N + p.bn - 1) / p.bn);
+}
+
+static void head_thin(const HeadProblem& p, void* part, float* target, cudaStream_t st) {
+  const int ctas = thin_ctas(p.N);
+  ThinArgs a{};
+  a.T = p.rows;
+  a.V = p.N;
+  const int share = (p.N + ctas - 1) / ctas;  // the largest share of a CTA, in equal tiles
+  const int tiles = (share + kThinEntries - 1) / kThinEntries;
+  a.tile = (share + tiles - 1) / tiles;
+  a.k_blocks = (p.D + kBK - 1) / kBK;
+  a.segs = (a.k_blocks + kSegBlocks - 1) / kSegBlocks;
+  a.labels = p.labels;
+  a.k = kLog2e / p.temperature;
+  a.cap = p.softcap;
+  a.inv_cap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
+  a.part = static_cast<float2*>(part);
+  a.target = target;
+  a.status = p.status;
+  if (p.rows <= 32) dispatch_thin<32>(p, a, ctas, st);
+  else if (p.rows <= 64) dispatch_thin<64>(p, a, ctas, st);
+  else dispatch_thin<128>(p, a, ctas, st);
+}
+
 void head_stats(const HeadProblem& p, void* part, float* target, const float* ref, void* X, long long ldx,
                 cudaStream_t st) {
   if (p.rows <= 0) return;
   check_head(p);
+  if (head_is_thin(p) && X == nullptr) return head_thin(p, part, target, st);
   HeadArgs a = base_args(p);
   a.part = static_cast<float2*>(part);
   a.target = target;
@@ -885,7 +1188,7 @@ void head_join(const HeadProblem& p, const void* part, const float* target, long
                long long ignore_index, float* out, const float* ref, float* lse2, float* label_grad,
                int* flag, cudaStream_t st) {
   if (p.rows <= 0) return;
-  const int parts = 2 * ((p.N + p.bn - 1) / p.bn);
+  const int parts = head_parts(p);
   const float2* pp = static_cast<const float2*>(part);
   const float k = kLog2e / p.temperature;
   // a warp per row fills the machine from about 148 * 8 rows on

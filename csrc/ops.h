@@ -171,7 +171,9 @@ struct HeadProblem {
 };
 int head_pairs();                       // CTA pairs of the persistent grid
 int head_tile_n(int rows, int N);
-// per row and half tile (reference, sum) pairs: part is float2 [rows][2 * ceil(N / bn)];
+constexpr int kThinRows = 128;          // unpacked rows up to here take the few-rows kernel
+int head_parts(const HeadProblem& p);   // (reference, sum) pairs of a row
+// per row (reference, sum) pairs: part is float2 [rows][head_parts];
 // target [rows] receives the label's logit (after the softcap, before the temperature).
 // X (optional) bf16 [rows, ldx]: the gradient rows up to a factor, relative to ref [rows]
 void head_stats(const HeadProblem& p, void* part, float* target, const float* ref, void* X, long long ldx,
