@@ -6,7 +6,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
+#include <sstream>
+#include <string>
 #include <vector>
 
 #include "ops.h"
@@ -28,14 +31,6 @@ int* status_ptr(const c10::optional<at::Tensor>& s) {
   return s->data_ptr<int>();
 }
 
-// a device row count (int32, one element) or null
-const int* count_ptr(const c10::optional<at::Tensor>& c, const at::Tensor& like) {
-  if (!c.has_value()) return nullptr;
-  TORCH_CHECK(c->scalar_type() == at::kInt && c->numel() >= 1 && c->device() == like.device(),
-              "a device row count is an int32 (its tensor's first) on the operands' device");
-  return c->data_ptr<int>();
-}
-
 int* int_ptr(const at::Tensor& t, int64_t n, const char* name) {
   check_cuda(t, name);
   TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() >= n, name,
@@ -45,19 +40,15 @@ int* int_ptr(const at::Tensor& t, int64_t n, const char* name) {
 
 // C = alpha * op(A) op(B)^T (+ beta * D).
 // a: [M,K] (a_mn_major=false) or [K,M] (true); b: [N,K] or [K,N]; c: [M,N]
-// m_limit / k_limit: device counts of the rows of C / of the summed rows in use (splits 1)
 void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_major, at::Tensor& c,
           const c10::optional<at::Tensor>& d, double alpha, double beta, int64_t splits, int64_t bn,
-          const c10::optional<at::Tensor>& status, const c10::optional<at::Tensor>& m_limit,
-          const c10::optional<at::Tensor>& k_limit, const c10::optional<at::Tensor>& split_out) {
+          const c10::optional<at::Tensor>& status) {
   check_cuda(a, "a");
   check_cuda(b, "b");
   check_cuda(c, "c");
   TORCH_CHECK(is_bf16(a) && is_bf16(b), "gemm operands must be bf16");
-  // with split_out, c [S, M, N] has room for S k splits stored apart
-  const int cd = split_out.has_value() ? 1 : 0;
-  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && c.dim() == 2 + cd, "gemm takes 2-D tensors");
-  TORCH_CHECK(a.stride(1) == 1 && b.stride(1) == 1 && c.stride(cd + 1) == 1, "gemm needs unit inner stride");
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && c.dim() == 2, "gemm takes 2-D tensors");
+  TORCH_CHECK(a.stride(1) == 1 && b.stride(1) == 1 && c.stride(1) == 1, "gemm needs unit inner stride");
   TORCH_CHECK(is_bf16(c) || is_f32(c), "gemm output must be bf16 or fp32");
   const c10::cuda::CUDAGuard guard(a.device());
   plg::GemmProblem p;
@@ -66,7 +57,7 @@ void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_m
   p.N = static_cast<int>(b_mn_major ? b.size(1) : b.size(0));
   const int kb = static_cast<int>(b_mn_major ? b.size(0) : b.size(1));
   TORCH_CHECK(kb == p.K, "gemm: K mismatch (", p.K, " vs ", kb, ")");
-  TORCH_CHECK(c.size(cd) == p.M && c.size(cd + 1) == p.N, "gemm: C must be [M, N]");
+  TORCH_CHECK(c.size(0) == p.M && c.size(1) == p.N, "gemm: C must be [M, N]");
   p.A = a.data_ptr();
   p.lda = a.stride(0);
   p.a_mn_major = a_mn_major;
@@ -74,14 +65,8 @@ void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_m
   p.ldb = b.stride(0);
   p.b_mn_major = b_mn_major;
   p.C = c.data_ptr();
-  p.ldc = c.stride(cd);
+  p.ldc = c.stride(0);
   p.c_fp32 = is_f32(c);
-  if (split_out.has_value()) {
-    TORCH_CHECK(c.is_contiguous() && c.size(0) >= 1 && c.size(0) <= 64, "gemm: 1..64 contiguous splits");
-    p.max_split = static_cast<int>(c.size(0));
-    p.split_stride = c.stride(0);
-    p.split_out = int_ptr(*split_out, 1, "split_out");
-  }
   if (d.has_value() && beta != 0.0) {
     check_cuda(*d, "d");
     TORCH_CHECK(d->dim() == 2 && d->size(0) == p.M && d->size(1) == p.N && d->stride(1) == 1,
@@ -97,8 +82,6 @@ void gemm(const at::Tensor& a, bool a_mn_major, const at::Tensor& b, bool b_mn_m
   p.allow_split = splits != 1;
   p.bn = static_cast<int>(bn);
   p.status = status_ptr(status);
-  p.m_limit = count_ptr(m_limit, a);
-  p.k_limit = count_ptr(k_limit, a);
   plg::gemm_bf16(p, cur_stream());
 }
 
@@ -424,165 +407,219 @@ float* float_ptr(const at::Tensor& t, int64_t n, const char* name) {
   return t.data_ptr<float>();
 }
 
-void head_compact_b(const at::Tensor& labels, int64_t V, int64_t ignore_index, at::Tensor& row_map,
-                    at::Tensor& inverse, at::Tensor& count, at::Tensor& out) {
-  const int64_t T = labels.numel();
-  TORCH_CHECK(T <= INT32_MAX - 256, "linear_token_logprobs: too many tokens in one call");
-  const c10::cuda::CUDAGuard guard(labels.device());
-  plg::head_compact(labels_ptr(labels), T, V, ignore_index, int_ptr(row_map, T, "row_map"),
-                    int_ptr(inverse, T, "inverse"), int_ptr(count, 3, "count"), float_ptr(out, T, "out"),
-                    cur_stream());
-}
-
 plg::HeadProblem head_problem(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
-                              const c10::optional<at::Tensor>& row_map,
-                              const c10::optional<at::Tensor>& count, double softcap, double temperature,
-                              const c10::optional<at::Tensor>& status) {
-  check_cuda(h, "hidden");
-  check_cuda(w, "weight");
-  TORCH_CHECK(is_bf16(h) && is_bf16(w) && h.dim() == 2 && w.dim() == 2 && h.stride(1) == 1 &&
-                  w.stride(1) == 1 && h.size(1) == w.size(1),
-              "linear_token_logprobs: hidden [T, D] and weight [V, D] in bf16 with unit inner stride");
-  TORCH_CHECK(row_map.has_value() == count.has_value(), "linear_token_logprobs: row_map goes with count");
-  TORCH_CHECK(h.size(0) <= INT32_MAX - 256 && w.size(0) <= INT32_MAX - 256,
-              "linear_token_logprobs: too many rows in one call");
+                              double softcap, double temperature, int* status) {
   plg::HeadProblem p;
   p.rows = static_cast<int>(h.size(0));
   p.N = static_cast<int>(w.size(0));
-  p.D = static_cast<int>(h.size(1));
+  p.D = static_cast<int>(w.size(1));
   p.h = h.data_ptr();
   p.ldh = h.stride(0);
   p.w = w.data_ptr();
   p.ldw = w.stride(0);
   p.bn = plg::head_tile_n(p.rows, p.N);
-  p.labels = labels_ptr(labels);
-  if (row_map.has_value()) {
-    p.row_map = int_ptr(*row_map, labels.numel(), "row_map");
-    p.n_rows = int_ptr(*count, 3, "count");
-  } else {
-    TORCH_CHECK(labels.numel() == p.rows, "linear_token_logprobs: one label per row");
-  }
+  p.labels = labels.data_ptr<int64_t>();
   p.softcap = static_cast<float>(softcap);
   p.temperature = static_cast<float>(temperature);
-  p.status = status_ptr(status);
+  p.status = status;
   return p;
 }
 
-void* x_ptr(const at::Tensor& x, int64_t rows, int64_t cols) {
-  check_cuda(x, "x");
-  TORCH_CHECK(is_bf16(x) && x.dim() == 2 && x.size(0) == rows && x.size(1) == cols && x.stride(1) == 1,
-              "linear_token_logprobs: x must be bf16 [rows, N]");
-  return x.data_ptr();
-}
+int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-// packed rows of hidden; ref (optional) [rows]: the reference of a kept X
-void head_gather_b(const at::Tensor& hidden, const at::Tensor& w, const at::Tensor& labels,
-                   const at::Tensor& row_map, const at::Tensor& count, double softcap, double temperature,
-                   at::Tensor& out, const c10::optional<at::Tensor>& ref) {
+// Log-probabilities of labels [T] under hidden [T, D] (bf16 or fp32) and w [V, D] (bf16).
+// Returns {out}, or with train {out, h, ints, stats, x}: packed rows h [R, D], ints int32
+// [2 T + 3] (row_map, inverse, {rows, flag, splits}), stats fp32 [3, R] (lse2, label_grad,
+// ref) and, if keep, x bf16 [R, V] (else undefined).
+std::vector<c10::optional<at::Tensor>> token_logprobs_fwd(const at::Tensor& hidden, const at::Tensor& w,
+                                                          const at::Tensor& labels, int64_t ignore_index,
+                                                          double softcap, double temperature, bool pack,
+                                                          bool train, bool keep, const at::Tensor& status) {
   check_cuda(hidden, "hidden");
-  TORCH_CHECK(hidden.dim() == 2 && hidden.stride(1) == 1 && (is_bf16(hidden) || is_f32(hidden)),
-              "hidden must be [T, D] bf16 or fp32");
-  TORCH_CHECK(out.is_contiguous() && out.size(0) >= hidden.size(0), "head_gather: out must be [>= T, D]");
-  TORCH_CHECK(out.size(1) == hidden.size(1), "head_gather: out must be [>= T, D]");
+  check_cuda(w, "weight");
+  labels_ptr(labels);
+  TORCH_CHECK((is_bf16(hidden) || is_f32(hidden)) && is_bf16(w) && hidden.dim() == 2 && w.dim() == 2 &&
+                  hidden.stride(1) == 1 && w.stride(1) == 1 && hidden.size(1) == w.size(1),
+              "linear_token_logprobs: hidden [T, D] and weight [V, D] with unit inner stride, weight bf16");
+  const int64_t T = hidden.size(0), D = hidden.size(1), V = w.size(0);
+  TORCH_CHECK(T >= 1 && labels.numel() == T && T <= INT32_MAX / 2 && V <= INT32_MAX - 256,
+              "linear_token_logprobs: one label per row, fewer than 2^30 rows");
+  TORCH_CHECK((pack || !train) && (train || !keep), "linear_token_logprobs: training packs its rows");
   const c10::cuda::CUDAGuard guard(hidden.device());
-  const plg::HeadProblem p = head_problem(out, w, labels, row_map, count, softcap, temperature, c10::nullopt);
-  plg::head_gather(p, hidden.data_ptr(), is_f32(hidden), hidden.stride(0), out.data_ptr(),
-                   static_cast<int>(out.size(0)), ref.has_value() ? float_ptr(*ref, p.rows, "ref") : nullptr,
-                   cur_stream());
-}
-
-// out[token] = log-probability of its label; for the gradient, lse2 and label_grad [rows],
-// and with a kept x its reference ref [rows]
-void head_logprobs_b(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels, int64_t ignore_index,
-                     const c10::optional<at::Tensor>& row_map, const c10::optional<at::Tensor>& count,
-                     double softcap, double temperature, at::Tensor& out,
-                     const c10::optional<at::Tensor>& lse2, const c10::optional<at::Tensor>& label_grad,
-                     const c10::optional<at::Tensor>& ref, const c10::optional<at::Tensor>& x,
-                     const c10::optional<at::Tensor>& status) {
-  const c10::cuda::CUDAGuard guard(h.device());
-  const plg::HeadProblem p = head_problem(h, w, labels, row_map, count, softcap, temperature, status);
-  TORCH_CHECK(ref.has_value() == x.has_value() && lse2.has_value() == label_grad.has_value() &&
-                  (!x.has_value() || (lse2.has_value() && count.has_value())),
-              "head_logprobs: x goes with ref, both with the gradient's row statistics and packed rows");
-  const int64_t parts = plg::head_parts(p);
+  const auto f32 = hidden.options().dtype(at::kFloat), b16 = hidden.options().dtype(at::kBFloat16);
+  const auto st = cur_stream();
+  at::Tensor out = at::empty({T}, f32), h, ints, stats, x;
+  int* ip = nullptr;
+  float* sp = nullptr;
+  const int64_t R = pack ? round_up(T, 256) : T;
+  if (pack) {
+    ints = at::empty({2 * T + 3}, hidden.options().dtype(at::kInt));
+    ip = ints.data_ptr<int>();
+    plg::head_compact(labels.data_ptr<int64_t>(), T, V, ignore_index, ip, ip + T, ip + 2 * T,
+                      out.data_ptr<float>(), st);
+    h = at::empty({R, D}, b16);
+    if (train) {
+      stats = at::empty({3, R}, f32);
+      sp = stats.data_ptr<float>();
+    }
+    if (keep) x = at::empty({R, round_up(V, 8)}, b16).narrow(1, 0, V);
+  } else {
+    h = is_bf16(hidden) ? hidden : hidden.to(at::kBFloat16);
+  }
+  plg::HeadProblem p = head_problem(h, w, labels, softcap, temperature, status_ptr(status));
+  if (pack) {
+    p.row_map = ip;
+    p.n_rows = ip + 2 * T;
+    plg::head_gather(p, hidden.data_ptr(), is_f32(hidden), hidden.stride(0), h.data_ptr(), p.rows,
+                     keep ? sp + 2 * R : nullptr, st);
+  }
   // workspace: the rows' (reference, sum) pairs and their labels' logits
-  at::Tensor part = at::empty({static_cast<int64_t>(p.rows) * (2 * parts + 1)}, out.options());
-  float* target = part.data_ptr<float>() + 2 * parts * p.rows;
-  const float* rp = ref.has_value() ? float_ptr(*ref, p.rows, "ref") : nullptr;
-  plg::head_stats(p, part.data_ptr(), target, rp, x.has_value() ? x_ptr(*x, p.rows, p.N) : nullptr,
-                  x.has_value() ? x->stride(0) : 0, cur_stream());
-  plg::head_join(p, part.data_ptr(), target, p.N, ignore_index, float_ptr(out, labels.numel(), "out"), rp,
-                 lse2.has_value() ? float_ptr(*lse2, p.rows, "lse2") : nullptr,
-                 label_grad.has_value() ? float_ptr(*label_grad, p.rows, "label_grad") : nullptr,
-                 count.has_value() ? count->data_ptr<int>() + 1 : nullptr, cur_stream());
+  const int64_t parts = plg::head_parts(p);
+  at::Tensor part = at::empty({R * (2 * parts + 1)}, f32);
+  float* target = part.data_ptr<float>() + 2 * parts * R;
+  plg::head_stats(p, part.data_ptr(), target, keep ? sp + 2 * R : nullptr, keep ? x.data_ptr() : nullptr,
+                  keep ? x.stride(0) : 0, st);
+  plg::head_join(p, part.data_ptr(), target, V, ignore_index, out.data_ptr<float>(), keep ? sp + 2 * R : nullptr,
+                 sp, train ? sp + R : nullptr, pack ? ip + 2 * T + 1 : nullptr, st);
+  if (!train) return {out};
+  return {out, h, ints, stats, keep ? c10::optional<at::Tensor>(x) : c10::nullopt};
 }
 
-// x [rows, N] = gradient rows over the vocabulary range starting at v0; if_flagged: only when
-// count[1] is set
-void head_recompute_b(const at::Tensor& h, const at::Tensor& w, int64_t v0, const at::Tensor& labels,
-                      const at::Tensor& row_map, const at::Tensor& count, double softcap, double temperature,
-                      const at::Tensor& lse2, const at::Tensor& label_grad, const at::Tensor& gout,
-                      bool if_flagged, at::Tensor& x, const c10::optional<at::Tensor>& status) {
+// Gradients from what token_logprobs_fwd saved: {dh [T, D] of h_dtype, dw [V, D] of w_dtype}
+// (those asked for). Without a kept x the gradient matrix takes at most `workspace` bytes at a
+// time; split_workspace bounds the k splits' sums of dh.
+std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
+    const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels, const at::Tensor& ints,
+    const at::Tensor& stats, const c10::optional<at::Tensor>& kept, const at::Tensor& gout, double softcap,
+    double temperature, int64_t workspace, int64_t split_workspace, bool dh_f32, bool dw_f32, bool need_h,
+    bool need_w, const at::Tensor& status) {
+  check_cuda(h, "hidden");
+  const int64_t T = labels.numel(), R = h.size(0), D = h.size(1), V = w.size(0);
+  const float* g = float_ptr(gout, T, "gout");
   const c10::cuda::CUDAGuard guard(h.device());
-  plg::HeadProblem p = head_problem(h, w, labels, row_map, count, softcap, temperature, status);
-  p.label0 = v0;
-  plg::head_recompute(p, float_ptr(lse2, p.rows, "lse2"), float_ptr(label_grad, p.rows, "label_grad"),
-                      float_ptr(gout, labels.numel(), "gout"), if_flagged ? count.data_ptr<int>() + 1 : nullptr,
-                      x_ptr(x, p.rows, p.N), x.stride(0), cur_stream());
-}
-
-// completes a kept x; factor [rows, 2], hs [rows, D]
-void head_scale_rows_b(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
-                       const at::Tensor& row_map, const at::Tensor& count, double temperature,
-                       const at::Tensor& lse2, const at::Tensor& label_grad, const at::Tensor& ref,
-                       const at::Tensor& gout, at::Tensor& x, at::Tensor& factor, at::Tensor& hs) {
-  const c10::cuda::CUDAGuard guard(h.device());
-  const plg::HeadProblem p = head_problem(h, w, labels, row_map, count, 0.0, temperature, c10::nullopt);
-  TORCH_CHECK(is_bf16(hs) && hs.is_contiguous() && hs.sizes() == h.sizes(), "head_scale_rows: hs must be like h");
-  plg::head_scale_rows(p, float_ptr(lse2, p.rows, "lse2"), float_ptr(label_grad, p.rows, "label_grad"),
-                       float_ptr(ref, p.rows, "ref"), float_ptr(gout, labels.numel(), "gout"),
-                       x_ptr(x, p.rows, p.N), x.stride(0), float_ptr(factor, 2LL * p.rows, "factor"),
-                       hs.data_ptr(), cur_stream());
-}
-
-// src [S, rows, D] fp32, of which the first count[2] parts are summed
-void head_scatter_b(const at::Tensor& src, const at::Tensor& count, const c10::optional<at::Tensor>& factor,
-                    const at::Tensor& w,
-                    const at::Tensor& labels, const at::Tensor& inverse, at::Tensor& dh) {
-  check_cuda(dh, "dh");
-  TORCH_CHECK(dh.dim() == 2 && dh.is_contiguous() && (is_bf16(dh) || is_f32(dh)) && src.dim() == 3 &&
-                  src.size(2) == dh.size(1) && dh.size(1) % 8 == 0 && labels.numel() == dh.size(0) &&
-                  is_bf16(w) && w.dim() == 2 && w.size(1) == dh.size(1),
-              "head_scatter: dh contiguous [T, D] bf16 or fp32, src [rows, D], w bf16 [V, D]");
-  const c10::cuda::CUDAGuard guard(dh.device());
-  plg::HeadProblem p;
-  p.D = static_cast<int>(dh.size(1));
-  p.w = w.data_ptr();
-  p.ldw = w.stride(0);
-  p.labels = labels_ptr(labels);
-  plg::head_scatter(p, float_ptr(src, src.numel(), "src"), src.stride(0), int_ptr(count, 3, "count") + 2,
-                    factor.has_value() ? float_ptr(*factor, 2 * src.size(1), "factor") : nullptr,
-                    int_ptr(inverse, dh.size(0), "inverse"), dh.data_ptr(), is_f32(dh), dh.size(0),
-                    cur_stream());
+  const auto f32 = h.options().dtype(at::kFloat);
+  const auto st = cur_stream();
+  int* ip = int_ptr(ints, 2 * T + 3, "ints");
+  int* count = ip + 2 * T;
+  const float* sp = float_ptr(stats, 3 * R, "stats");
+  plg::HeadProblem p = head_problem(h, w, labels, softcap, temperature, status_ptr(status));
+  p.row_map = ip;
+  p.n_rows = count;
+  int64_t width = V;
+  at::Tensor x, hs = h, factor;
+  if (kept.has_value()) {
+    x = *kept;
+    plg::head_recompute(p, sp, sp + R, g, count + 1, x.data_ptr(), x.stride(0), st);  // only if flagged
+    hs = at::empty_like(h);
+    factor = at::empty({R, 2}, f32);
+    plg::head_scale_rows(p, sp, sp + R, sp + 2 * R, g, x.data_ptr(), x.stride(0), factor.data_ptr<float>(),
+                         hs.data_ptr(), st);
+  } else {
+    if (2 * R * V > workspace)  // ranges of whole 256-column tiles within the workspace
+      width = std::min(V, std::max<int64_t>(1, workspace / (2 * R * 256)) * 256);
+    x = at::empty({R, round_up(width, 8)}, h.options());
+  }
+  // dh's product has few tiles and a long sum: one range's k splits are summed by head_scatter
+  const int64_t splits =
+      width >= V ? std::max<int64_t>(1, std::min<int64_t>(16, split_workspace / (4 * R * D))) : 1;
+  at::Tensor dh_rows, dh, dw;
+  if (need_h) dh_rows = at::empty({splits, R, D}, f32);
+  if (need_w) dw = at::empty({V, D}, dw_f32 ? f32 : h.options());
+  for (int64_t v0 = 0; v0 < V; v0 += width) {
+    const int64_t n = std::min(width, V - v0);
+    if (!kept.has_value()) {
+      plg::HeadProblem r = p;
+      r.w = static_cast<const char*>(p.w) + 2 * v0 * p.ldw;
+      r.N = static_cast<int>(n);
+      r.bn = plg::head_tile_n(r.rows, r.N);
+      r.label0 = v0;
+      plg::head_recompute(r, sp, sp + R, g, nullptr, x.data_ptr(), x.stride(0), st);
+    }
+    plg::GemmProblem q;
+    q.A = x.data_ptr();
+    q.lda = x.stride(0);
+    q.b_mn_major = true;
+    q.ldc = D;
+    q.N = static_cast<int>(D);
+    q.splits = 1;
+    q.allow_split = false;
+    q.status = p.status;
+    if (need_h) {  // dh += x W over this range
+      plg::GemmProblem a = q;
+      a.M = static_cast<int>(R);
+      a.K = static_cast<int>(n);
+      a.B = static_cast<const char*>(p.w) + 2 * v0 * p.ldw;
+      a.ldb = p.ldw;
+      a.C = dh_rows.data_ptr();
+      a.c_fp32 = true;
+      a.m_limit = count;
+      if (splits > 1) {
+        a.max_split = static_cast<int>(splits);
+        a.split_stride = R * D;
+        a.split_out = count + 2;
+      } else if (v0 > 0) {
+        a.D = a.C;
+        a.ldd = D;
+        a.d_fp32 = true;
+        a.beta = 1.f;
+      }
+      plg::gemm_bf16(a, st);
+    }
+    if (need_w) {  // dW's rows of this range = x^T h
+      plg::GemmProblem b = q;
+      b.M = static_cast<int>(n);
+      b.K = static_cast<int>(R);
+      b.a_mn_major = true;
+      b.B = hs.data_ptr();
+      b.ldb = D;
+      b.C = static_cast<char*>(dw.data_ptr()) + v0 * D * (dw_f32 ? 4 : 2);
+      b.c_fp32 = dw_f32;
+      b.k_limit = count;
+      plg::gemm_bf16(b, st);
+    }
+  }
+  if (need_h) {
+    dh = at::empty({T, D}, dh_f32 ? f32 : h.options());
+    plg::head_scatter(p, dh_rows.data_ptr<float>(), R * D, count + 2,
+                      kept.has_value() ? factor.data_ptr<float>() : nullptr, ip + T, dh.data_ptr(), dh_f32, T, st);
+  }
+  return {need_h ? c10::optional<at::Tensor>(dh) : c10::nullopt,
+          need_w ? c10::optional<at::Tensor>(dw) : c10::nullopt};
 }
 
 // ---- objectives over token log-probabilities and router logits
-// a [..., S] tensor whose last dimension is contiguous (any stride when S < 2)
-void check_tokens(const at::Tensor& t, at::IntArrayRef shape, const char* name) {
-  check_cuda(t, name);
-  TORCH_CHECK(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
-  TORCH_CHECK(t.size(-1) < 2 || t.stride(-1) == 1, name, " must have contiguous tokens");
+// Their arguments come from users as they are, so that refusals raise ValueError and TypeError.
+std::string str(at::IntArrayRef v) {
+  std::ostringstream o;
+  o << v;
+  return o.str();
 }
 
-const uint8_t* mask_ptr(const at::Tensor& m) {
-  TORCH_CHECK(m.scalar_type() == at::kBool, "mask must be bool");
-  return reinterpret_cast<const uint8_t*>(m.data_ptr<bool>());
+// `t` has `shape` and the device of `like`; its last dimension is made contiguous if need be
+at::Tensor user_tokens(const at::Tensor& t, at::IntArrayRef shape, const at::Tensor& like, const char* op,
+                       const char* name, bool bf16_too) {
+  if (t.sizes() != shape || t.device() != like.device())
+    throw py::value_error(std::string(op) + ": " + name + " must have shape " + str(shape) +
+                          " on the mask's device, got " + str(t.sizes()));
+  if (!is_f32(t) && !(bf16_too && is_bf16(t)))
+    throw py::type_error(std::string(op) + ": " + name + (bf16_too ? " must be fp32 or bf16" : " must be fp32"));
+  return t.size(-1) < 2 || t.stride(-1) == 1 ? t : t.contiguous();
 }
+
+void check_mask(const at::Tensor& m, int64_t dims, const char* op) {
+  check_cuda(m, "mask");
+  if (m.dim() != dims || m.scalar_type() != at::kBool)
+    throw py::value_error(std::string(op) + ": mask must be bool with " + std::to_string(dims) + " dimensions");
+  for (int64_t d = 0; d < dims; ++d)
+    TORCH_CHECK(m.size(d) <= INT32_MAX / 2, op, ": too large");
+  TORCH_CHECK(m.size(-1) < 2 || m.stride(-1) == 1, op, ": mask must have contiguous tokens");
+}
+
+const uint8_t* mask_ptr(const at::Tensor& m) { return reinterpret_cast<const uint8_t*>(m.data_ptr<bool>()); }
 
 plg::PrefArgs pref_args(const at::Tensor& mask) {
-  TORCH_CHECK(mask.dim() == 3 && mask.size(0) == 2, "preference_loss: mask must be [2, P, S]");
-  check_tokens(mask, mask.sizes(), "mask");
-  TORCH_CHECK(mask.size(1) <= INT32_MAX / 2 && mask.size(2) <= INT32_MAX / 2, "preference_loss: too large");
+  check_mask(mask, 3, "preference_loss");
+  if (mask.size(0) != 2) throw py::value_error("preference_loss: mask must be [2, P, S]");
   plg::PrefArgs a;
   a.mask = mask_ptr(mask);
   a.mk_side = mask.stride(0);
@@ -592,84 +629,84 @@ plg::PrefArgs pref_args(const at::Tensor& mask) {
   return a;
 }
 
-// out: fp32 [4 P + 1]: row_scale [2, P], rewards [2, P], loss
-void preference_fwd(const at::Tensor& logps, const c10::optional<at::Tensor>& ref, const at::Tensor& mask,
-                    int64_t kind, double beta, double smoothing, bool normalized, at::Tensor& out) {
+// {loss, chosen rewards [P], rejected rewards [P], row_scale [2, P] for the backward}
+std::vector<at::Tensor> preference_fwd(const at::Tensor& logps, const c10::optional<at::Tensor>& ref,
+                                       const at::Tensor& mask, int64_t kind, double beta, double smoothing,
+                                       bool normalized) {
   const c10::cuda::CUDAGuard guard(mask.device());
   plg::PrefArgs a = pref_args(mask);
-  check_tokens(logps, mask.sizes(), "logps");
-  TORCH_CHECK(is_f32(logps), "preference_loss: logps must be fp32");
-  a.logps = logps.data_ptr<float>();
-  a.lp_side = logps.stride(0);
-  a.lp_pair = logps.stride(1);
+  const at::Tensor lp = user_tokens(logps, mask.sizes(), mask, "preference_loss", "logps", false);
+  a.logps = lp.data_ptr<float>();
+  a.lp_side = lp.stride(0);
+  a.lp_pair = lp.stride(1);
+  at::Tensor rf;
   if (ref.has_value()) {
-    check_tokens(*ref, mask.sizes(), "ref_logps");
-    TORCH_CHECK(is_f32(*ref) || is_bf16(*ref), "preference_loss: ref_logps must be fp32 or bf16");
-    a.ref = ref->data_ptr();
-    a.ref_bf16 = is_bf16(*ref);
-    a.ref_side = ref->stride(0);
-    a.ref_pair = ref->stride(1);
+    rf = user_tokens(*ref, mask.sizes(), mask, "preference_loss", "ref_logps", true);
+    a.ref = rf.data_ptr();
+    a.ref_bf16 = is_bf16(rf);
+    a.ref_side = rf.stride(0);
+    a.ref_pair = rf.stride(1);
   }
   a.kind = static_cast<int>(kind);
   a.beta = static_cast<float>(beta);
   a.smoothing = static_cast<float>(smoothing);
   a.normalized = normalized;
-  float* o = float_ptr(out, 4LL * a.P + 1, "out");
+  at::Tensor out = at::empty({1}, logps.options()), rewards = at::empty({2, a.P}, logps.options()),
+             row_scale = at::empty({2, a.P}, logps.options());
   // workspace: partial sums, block losses, ticket
-  const int64_t nb = plg::pref_blocks(a.P), np = 2LL * a.P * plg::pref_chunks(a.S);
+  const int64_t nb = plg::pref_blocks(a.P), np = 2LL * a.P * plg::pref_chunks(a.P, a.S);
   at::Tensor ws = at::empty({8 * (np + nb + 1)}, mask.options().dtype(at::kByte));
   char* w = static_cast<char*>(ws.data_ptr());
   plg::pref_forward(a, w, reinterpret_cast<double*>(w + 8 * np), reinterpret_cast<unsigned*>(w + 8 * (np + nb)),
-                    o, o + 4LL * a.P, o + 2LL * a.P, cur_stream());
+                    row_scale.data_ptr<float>(), out.data_ptr<float>(), rewards.data_ptr<float>(), cur_stream());
+  return {out.select(0, 0), rewards.select(0, 0), rewards.select(0, 1), row_scale};
 }
 
-void preference_bwd(const at::Tensor& mask, const at::Tensor& row_scale, const at::Tensor& gout, at::Tensor& grad) {
+at::Tensor preference_bwd(const at::Tensor& mask, const at::Tensor& row_scale, const at::Tensor& gout) {
   const c10::cuda::CUDAGuard guard(mask.device());
   const plg::PrefArgs a = pref_args(mask);
+  at::Tensor grad = at::empty(mask.sizes(), row_scale.options());
   plg::pref_backward(a, float_ptr(row_scale, 2LL * a.P, "row_scale"), float_ptr(gout, 1, "gout"),
-                     float_ptr(grad, mask.numel(), "grad"), cur_stream());
+                     grad.data_ptr<float>(), cur_stream());
+  return grad;
 }
 
-// out: fp32 [3]: loss, mean KL, clipped share; grad [R, S] (optional)
-void policy_fwd(const at::Tensor& logps, const c10::optional<at::Tensor>& old, const at::Tensor& adv,
-                const at::Tensor& mask, const c10::optional<at::Tensor>& ref, double clip_low, double clip_high,
-                double kl_coef, bool by_sequence, const c10::optional<at::Tensor>& grad, at::Tensor& out) {
-  TORCH_CHECK(mask.dim() == 2, "policy_loss: mask must be [R, S]");
+// {loss, mean KL, clipped share} and, with train, the gradient [R, S]
+std::vector<at::Tensor> policy_fwd(const at::Tensor& logps, const c10::optional<at::Tensor>& old,
+                                   const at::Tensor& adv, const at::Tensor& mask,
+                                   const c10::optional<at::Tensor>& ref, double clip_low, double clip_high,
+                                   double kl_coef, bool by_sequence, bool train) {
   const c10::cuda::CUDAGuard guard(mask.device());
-  check_tokens(mask, mask.sizes(), "mask");
-  check_tokens(logps, mask.sizes(), "logps");
-  TORCH_CHECK(mask.size(0) <= INT32_MAX / 2 && mask.size(1) <= INT32_MAX / 2, "policy_loss: too large");
-  TORCH_CHECK(is_f32(logps), "policy_loss: logps must be fp32");
+  const char* op = "policy_loss";
+  check_mask(mask, 2, op);
   plg::PolicyArgs a;
   a.R = static_cast<int>(mask.size(0));
   a.S = static_cast<int>(mask.size(1));
   a.mask = mask_ptr(mask);
   a.mk_row = mask.stride(0);
-  a.logps = logps.data_ptr<float>();
-  a.lp_row = logps.stride(0);
+  const at::Tensor lp = user_tokens(logps, mask.sizes(), mask, op, "logps", false);
+  a.logps = lp.data_ptr<float>();
+  a.lp_row = lp.stride(0);
+  at::Tensor ol, rf;
   if (old.has_value()) {
-    check_tokens(*old, mask.sizes(), "old_logps");
-    TORCH_CHECK(is_f32(*old) || is_bf16(*old), "policy_loss: old_logps must be fp32 or bf16");
-    a.old = old->data_ptr();
-    a.old_bf16 = is_bf16(*old);
-    a.old_row = old->stride(0);
+    ol = user_tokens(*old, mask.sizes(), mask, op, "old_logps", true);
+    a.old = ol.data_ptr();
+    a.old_bf16 = is_bf16(ol);
+    a.old_row = ol.stride(0);
   }
   if (ref.has_value()) {
-    check_tokens(*ref, mask.sizes(), "ref_logps");
-    TORCH_CHECK(is_f32(*ref) || is_bf16(*ref), "policy_loss: ref_logps must be fp32 or bf16");
-    a.ref = ref->data_ptr();
-    a.ref_bf16 = is_bf16(*ref);
-    a.ref_row = ref->stride(0);
+    rf = user_tokens(*ref, mask.sizes(), mask, op, "ref_logps", true);
+    a.ref = rf.data_ptr();
+    a.ref_bf16 = is_bf16(rf);
+    a.ref_row = rf.stride(0);
   }
-  check_cuda(adv, "advantages");
-  TORCH_CHECK(is_f32(adv) && (adv.dim() == 1 || adv.dim() == 2) && adv.size(0) == a.R,
-              "policy_loss: advantages must be fp32 [R] or [R, S]");
-  if (adv.dim() == 2) {
-    check_tokens(adv, mask.sizes(), "advantages");
-    a.adv_tok = 1;
-  }
-  a.adv = adv.data_ptr<float>();
-  a.adv_row = adv.stride(0);
+  a.adv_tok = adv.dim() == 2;
+  if (adv.dim() != 1 && adv.dim() != 2) throw py::value_error("policy_loss: advantages must be [R] or [R, S]");
+  const at::Tensor av =
+      a.adv_tok ? user_tokens(adv, mask.sizes(), mask, op, "advantages", false)
+                : user_tokens(adv.unsqueeze(1), {a.R, 1}, mask, op, "advantages", false);
+  a.adv = av.data_ptr<float>();
+  a.adv_row = av.stride(0);
   a.hi = static_cast<float>(1.0 + clip_high);
   a.lo = static_cast<float>(1.0 - clip_low);
   a.log_hi = static_cast<float>(std::log1p(clip_high));
@@ -681,10 +718,13 @@ void policy_fwd(const at::Tensor& logps, const c10::optional<at::Tensor>& old, c
   at::Tensor ws = at::empty({16 * cb + 24 * sb + 4LL * a.R + 4}, mask.options().dtype(at::kByte));
   char* w = static_cast<char*>(ws.data_ptr());
   int* counts = reinterpret_cast<int*>(w + 16 * cb + 24 * sb);
+  at::Tensor out = at::empty({3}, logps.options()), grad;
+  if (train) grad = at::empty(mask.sizes(), logps.options());
   plg::policy_forward(a, counts, w, reinterpret_cast<double*>(w + 16 * cb),
                       reinterpret_cast<unsigned*>(counts + a.R),
-                      grad.has_value() ? float_ptr(*grad, mask.numel(), "grad") : nullptr,
-                      float_ptr(out, 3, "out"), cur_stream());
+                      train ? grad.data_ptr<float>() : nullptr, out.data_ptr<float>(), cur_stream());
+  if (!train) return {out.select(0, 0), out.select(0, 1), out.select(0, 2)};
+  return {out.select(0, 0), out.select(0, 1), out.select(0, 2), grad};
 }
 
 void scale_unless_one_b(at::Tensor& x, const at::Tensor& s) {
@@ -692,68 +732,93 @@ void scale_unless_one_b(at::Tensor& x, const at::Tensor& s) {
   plg::scale_unless_one(float_ptr(x, x.numel(), "x"), x.numel(), float_ptr(s, 1, "s"), cur_stream());
 }
 
-plg::RouterArgs router_args(const std::vector<at::Tensor>& logits, const std::vector<at::Tensor>& idx,
-                            const c10::optional<at::Tensor>& mask) {
-  TORCH_CHECK(!logits.empty() && logits.size() <= plg::kRouterMaxLayers && idx.size() == logits.size(),
-              "router_balance_loss: 1..", plg::kRouterMaxLayers, " layers, one index tensor for each");
+// the layers' logits and, for the forward, their indices; tensors that had to be copied are kept
+// in `copies`
+plg::RouterArgs router_args(const std::vector<at::Tensor>& logits, const std::vector<at::Tensor>* idx,
+                            const c10::optional<at::Tensor>& mask, std::vector<at::Tensor>& copies) {
+  TORCH_CHECK(!logits.empty(), "router_balance_loss: no logits");
   plg::RouterArgs a{};
   const at::Tensor& x0 = logits[0];
   check_cuda(x0, "router_logits");
-  TORCH_CHECK(x0.dim() == 2 && idx[0].dim() == 2, "router_balance_loss: logits [T, E] and indices [T, k]");
-  a.L = static_cast<int>(logits.size());
+  if (x0.dim() != 2) throw py::value_error("router_balance_loss: the routers' logits must be [T, E], alike");
   a.T = x0.size(0);
   a.E = static_cast<int>(x0.size(1));
-  a.k = static_cast<int>(idx[0].size(1));
+  if (static_cast<int>(logits.size()) > plg::kRouterMaxLayers || a.E > plg::kRouterMaxExperts)
+    throw py::value_error("router_balance_loss: at most " + std::to_string(plg::kRouterMaxLayers) + " layers of " +
+                          std::to_string(plg::kRouterMaxExperts) + " experts on CUDA");
+  a.L = static_cast<int>(logits.size());
+  auto inner = [&](const at::Tensor& t) {
+    if (t.size(1) < 2 || t.stride(1) == 1) return t;
+    copies.push_back(t.contiguous());
+    return copies.back();
+  };
   for (int l = 0; l < a.L; ++l) {
-    const at::Tensor &x = logits[l], &i = idx[l];
-    TORCH_CHECK(x.device() == x0.device() && x.sizes() == x0.sizes() && x.scalar_type() == x0.scalar_type() &&
-                    (is_bf16(x) || is_f32(x)) && (x.stride(1) == 1 || a.E == 1),
-                "router_balance_loss: the layers' logits must be bf16 or fp32 [T, E], alike");
-    TORCH_CHECK(i.device() == x0.device() && i.scalar_type() == at::kLong && i.is_contiguous() && i.dim() == 2 &&
-                    i.size(0) == a.T && i.size(1) == a.k,
-                "router_balance_loss: indices must be contiguous int64 [T, k], alike");
+    if (logits[l].sizes() != x0.sizes() || logits[l].scalar_type() != x0.scalar_type() ||
+        logits[l].device() != x0.device())
+      throw py::value_error("router_balance_loss: the routers' logits must be [T, E], alike");
+    const at::Tensor x = inner(logits[l]);
     a.logits[l] = x.data_ptr();
     a.ld[l] = x.stride(0);
-    a.idx[l] = i.data_ptr<int64_t>();
+  }
+  if (idx != nullptr) {
+    const at::Tensor& i0 = (*idx)[0];
+    a.k = i0.dim() == 2 ? static_cast<int>(i0.size(1)) : 0;
+    for (int l = 0; l < a.L; ++l) {
+      const at::Tensor& i = (*idx)[l];
+      if (i.dim() != 2 || i.size(0) != a.T || i.size(1) != a.k || i.scalar_type() != at::kLong ||
+          i.device() != x0.device())
+        throw py::value_error("router_balance_loss: indices must be int64 [T, k], got " + str(i.sizes()));
+      if (!i.is_contiguous()) copies.push_back(i.contiguous());
+      a.idx[l] = i.is_contiguous() ? i.data_ptr<int64_t>() : copies.back().data_ptr<int64_t>();
+    }
   }
   if (mask.has_value()) {
-    check_tokens(*mask, {a.T}, "mask");
-    TORCH_CHECK(mask->is_contiguous(), "mask must be contiguous");
-    a.mask = mask_ptr(*mask);
+    if (mask->dim() != 1 || mask->size(0) != a.T || mask->scalar_type() != at::kBool || mask->device() != x0.device())
+      throw py::value_error("router_balance_loss: mask must be bool [T]");
+    copies.push_back(mask->contiguous());
+    a.mask = mask_ptr(copies.back());
   }
   return a;
 }
 
-// out: fp32 [E + 2]: slope [E + 1], loss; lse [L, T]; counts int64 [E]
-void router_balance_fwd(const std::vector<at::Tensor>& logits, const std::vector<at::Tensor>& idx,
-                        const c10::optional<at::Tensor>& mask, double balance, double zcoef, at::Tensor& lse,
-                        at::Tensor& counts, at::Tensor& out) {
-  const c10::cuda::CUDAGuard guard(lse.device());
-  const plg::RouterArgs a = router_args(logits, idx, mask);
-  TORCH_CHECK(counts.is_cuda() && counts.scalar_type() == at::kLong && counts.is_contiguous() &&
-                  counts.numel() == a.E, "router_balance_loss: counts must be int64 [E]");
-  float* o = float_ptr(out, a.E + 2, "out");
+// {loss, counts int64 [E], lse [L, T], slope [E + 1] for the backward}
+std::vector<at::Tensor> router_balance_fwd(const std::vector<at::Tensor>& logits,
+                                           const std::vector<at::Tensor>& idx,
+                                           const c10::optional<at::Tensor>& mask, double balance, double zcoef) {
+  std::vector<at::Tensor> copies;
+  copies.reserve(2 * logits.size() + 1);
+  const plg::RouterArgs a = router_args(logits, &idx, mask, copies);
+  const c10::cuda::CUDAGuard guard(logits[0].device());
+  const auto f32 = logits[0].options().dtype(at::kFloat);
+  at::Tensor lse = at::empty({a.L, a.T}, f32), counts = at::empty({a.E}, f32.dtype(at::kLong)),
+             loss = at::empty({}, f32), slope = at::empty({a.E + 1}, f32);
   const int64_t blocks = plg::router_blocks(a.L * a.T);
-  at::Tensor ws = at::empty({blocks * (16 + 8LL * a.E)}, lse.options().dtype(at::kByte));
+  const int64_t dots = (a.E + 31) / 32;
+  at::Tensor ws = at::empty({blocks * (16 + 8LL * a.E) + 8 * (dots + 1)}, lse.options().dtype(at::kByte));
   char* w = static_cast<char*>(ws.data_ptr());
-  float* pp = reinterpret_cast<float*>(w + 16 * blocks);
+  double* dp = reinterpret_cast<double*>(w + 16 * blocks);
+  float* pp = reinterpret_cast<float*>(w + 16 * blocks + 8 * (dots + 1));
   plg::router_balance_forward(a, is_bf16(logits[0]), static_cast<float>(balance), static_cast<float>(zcoef),
-                              float_ptr(lse, a.L * a.T, "lse"), pp, reinterpret_cast<int*>(pp + blocks * a.E),
-                              reinterpret_cast<double*>(w), o + a.E + 1, counts.data_ptr<int64_t>(), o,
-                              cur_stream());
+                              lse.data_ptr<float>(), pp, reinterpret_cast<int*>(pp + blocks * a.E),
+                              reinterpret_cast<double*>(w), dp, reinterpret_cast<unsigned*>(dp + dots),
+                              loss.data_ptr<float>(), counts.data_ptr<int64_t>(),
+                              slope.data_ptr<float>(), cur_stream());
+  return {loss, counts, lse, slope};
 }
 
-void router_balance_bwd(const std::vector<at::Tensor>& logits, const std::vector<at::Tensor>& idx,
-                        const c10::optional<at::Tensor>& mask, const at::Tensor& lse, const at::Tensor& slope,
-                        const at::Tensor& gout, at::Tensor& grad) {
+// gradients of the layers' logits, in their type
+std::vector<at::Tensor> router_balance_bwd(const std::vector<at::Tensor>& logits,
+                                           const c10::optional<at::Tensor>& mask, const at::Tensor& lse,
+                                           const at::Tensor& slope, const at::Tensor& gout) {
   const c10::cuda::CUDAGuard guard(lse.device());
-  const plg::RouterArgs a = router_args(logits, idx, mask);
-  check_cuda(grad, "grad");
-  TORCH_CHECK(grad.is_contiguous() && grad.scalar_type() == logits[0].scalar_type() &&
-                  grad.numel() == a.L * a.T * a.E, "router_balance_loss: grad must be [L, T, E] in the logits' type");
+  std::vector<at::Tensor> copies;
+  copies.reserve(logits.size() + 1);
+  const plg::RouterArgs a = router_args(logits, nullptr, mask, copies);
+  at::Tensor grad = at::empty({a.L, a.T, a.E}, logits[0].options());
   plg::router_balance_backward(a, is_bf16(logits[0]), float_ptr(lse, a.L * a.T, "lse"),
                                float_ptr(slope, a.E + 1, "slope"), float_ptr(gout, 1, "gout"), grad.data_ptr(),
                                cur_stream());
+  return grad.unbind(0);
 }
 
 void exp2_poly_eval_b(const at::Tensor& x, at::Tensor& poly, at::Tensor& ref) {
@@ -1218,22 +1283,15 @@ void set_peer_wait_deadline(int64_t ns) {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "pluggy_b200 sm_100a kernels";
-  m.def("gemm", &gemm, py::arg("a"), py::arg("a_mn_major"), py::arg("b"), py::arg("b_mn_major"),
-        py::arg("c"), py::arg("d"), py::arg("alpha"), py::arg("beta"), py::arg("splits"), py::arg("bn"),
-        py::arg("status"), py::arg("m_limit") = py::none(), py::arg("k_limit") = py::none(),
-        py::arg("split_out") = py::none());
+  m.def("gemm", &gemm);
   m.def("preference_fwd", &preference_fwd);
   m.def("preference_bwd", &preference_bwd);
   m.def("policy_fwd", &policy_fwd);
   m.def("scale_unless_one", &scale_unless_one_b);
   m.def("router_balance_fwd", &router_balance_fwd);
   m.def("router_balance_bwd", &router_balance_bwd);
-  m.def("head_compact", &head_compact_b);
-  m.def("head_gather", &head_gather_b);
-  m.def("head_logprobs", &head_logprobs_b);
-  m.def("head_recompute", &head_recompute_b);
-  m.def("head_scale_rows", &head_scale_rows_b);
-  m.def("head_scatter", &head_scatter_b);
+  m.def("token_logprobs_fwd", &token_logprobs_fwd);
+  m.def("token_logprobs_bwd", &token_logprobs_bwd);
   m.def("gemm_grouped", &gemm_grouped, py::arg("a"), py::arg("b"), py::arg("b_mn_major"), py::arg("c"),
         py::arg("mode"), py::arg("table"), py::arg("groups"), py::arg("b_rows"), py::arg("alpha"),
         py::arg("beta"), py::arg("status") = py::none());

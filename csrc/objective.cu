@@ -18,7 +18,10 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kWarpTokens = 1024;  // tokens of one row that a warp takes at a time
+// Tokens of one row that a warp takes at a time: 1024 once that gives every warp of the
+// machine (148 SMs x 16) a unit, fewer, down to 128, where there would be too few of them
+// (8 rows of 1023 tokens: 17.9 us at 1024, 6.4 us at 128).
+constexpr int kMaxWarpTokens = 1024, kMinWarpTokens = 128;
 
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
@@ -65,15 +68,15 @@ __device__ __forceinline__ void load_mask(const uint8_t* p, bool (&m)[VEC]) {
 // Row r = side * P + pair of [2, P, S] tensors.
 template <int VEC>
 __global__ void __launch_bounds__(256) pref_sums_kernel(const PrefArgs a, float2* __restrict__ part,
-                                                        int chunks, unsigned* __restrict__ ticket) {
+                                                        int chunks, int len, unsigned* __restrict__ ticket) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
   const int lane = threadIdx.x & 31;
   const long long units = 2LL * a.P * chunks;
   const long long nw = static_cast<long long>(gridDim.x) * 8;
   for (long long u = blockIdx.x * 8LL + (threadIdx.x >> 5); u < units; u += nw) {
     const long long r = u / chunks;
-    const int t0 = static_cast<int>(u - r * chunks) * kWarpTokens;
-    const int t1 = min(a.S, t0 + kWarpTokens);
+    const int t0 = static_cast<int>(u - r * chunks) * len;
+    const int t1 = min(a.S, t0 + len);
     const int side = r >= a.P ? 1 : 0;
     const long long pair = r - static_cast<long long>(side) * a.P;
     const float* lp = a.logps + side * a.lp_side + pair * a.lp_pair;
@@ -188,15 +191,15 @@ __global__ void __launch_bounds__(256) pref_pairs_kernel(const PrefArgs a, const
 template <int VEC>
 __global__ void __launch_bounds__(256) pref_grad_kernel(const PrefArgs a, const float* __restrict__ row_scale,
                                                         const float* __restrict__ gout,
-                                                        float* __restrict__ grad, int chunks) {
+                                                        float* __restrict__ grad, int chunks, int len) {
   const int lane = threadIdx.x & 31;
   const long long units = 2LL * a.P * chunks;
   const long long nw = static_cast<long long>(gridDim.x) * 8;
   const float g = *gout;
   for (long long u = blockIdx.x * 8LL + (threadIdx.x >> 5); u < units; u += nw) {
     const long long r = u / chunks;
-    const int t0 = static_cast<int>(u - r * chunks) * kWarpTokens;
-    const int t1 = min(a.S, t0 + kWarpTokens);
+    const int t0 = static_cast<int>(u - r * chunks) * len;
+    const int t1 = min(a.S, t0 + len);
     const int side = r >= a.P ? 1 : 0;
     const uint8_t* mk = a.mask + side * a.mk_side + (r - static_cast<long long>(side) * a.P) * a.mk_pair;
     const float c = g * row_scale[r];
@@ -279,17 +282,20 @@ __global__ void __launch_bounds__(256) policy_counts_kernel(const PolicyArgs a, 
   }
 }
 
-// e^d - 1 - d: the KL term per token. For small d the difference cancels, so its Taylor
-// series is summed instead (|d| < 1/4: the first dropped term is below 1e-8 of the result).
-__device__ __forceinline__ float kl_term(float d, float em1) {
-  if (fabsf(d) >= 0.25f) return em1 - d;
+// em1 = e^d - 1 and k3 = e^d - 1 - d, the KL term per token and (its negative) its slope. For
+// small d both differences cancel, so the Taylor series is summed there instead (|d| < 1/4:
+// the first dropped term is below 2e-8 of the result).
+__device__ __forceinline__ void kl_terms(float d, float& em1, float& k3) {
   float p = 1.f / 5040.f;
   p = fmaf(p, d, 1.f / 720.f);
   p = fmaf(p, d, 1.f / 120.f);
   p = fmaf(p, d, 1.f / 24.f);
   p = fmaf(p, d, 1.f / 6.f);
   p = fmaf(p, d, 0.5f);
-  return d * d * p;
+  const float q = d * d * p, e = expf(d) - 1.f;
+  const bool small = fabsf(d) < 0.25f;
+  em1 = small ? d + q : e;
+  k3 = small ? q : e - d;
 }
 
 // Per token, with r = logps - old and d = ref - logps:
@@ -297,11 +303,11 @@ __device__ __forceinline__ float kl_term(float d, float em1) {
 //   grad = -A e^r (0 past the bound) - kl_coef (e^d - 1)
 // each times the token's weight in the mean, known from the counts.
 template <int VEC>
-__global__ void __launch_bounds__(256) policy_kernel(const PolicyArgs a, const int* __restrict__ counts,
+__global__ void __launch_bounds__(256, 3) policy_kernel(const PolicyArgs a, const int* __restrict__ counts,
                                                      const longlong2* __restrict__ block_counts, int nblocks,
                                                      double* __restrict__ block_sums,
                                                      unsigned* __restrict__ ticket, float* __restrict__ grad,
-                                                     float* __restrict__ out, int chunks) {
+                                                     float* __restrict__ out, int chunks, int len) {
   __shared__ long long s_cnt[2][8];
   __shared__ double s_sum[3][8];
   __shared__ bool s_last;
@@ -336,47 +342,61 @@ __global__ void __launch_bounds__(256) policy_kernel(const PolicyArgs a, const i
   const long long nw = static_cast<long long>(gridDim.x) * 8;
   for (long long u = blockIdx.x * 8LL + warp; u < units; u += nw) {
     const long long r = u / chunks;
-    const int t0 = static_cast<int>(u - r * chunks) * kWarpTokens;
-    const int t1 = min(a.S, t0 + kWarpTokens);
-    const float* lp = a.logps + r * a.lp_row;
-    const uint8_t* mk = a.mask + r * a.mk_row;
+    const int t0 = static_cast<int>(u - r * chunks) * len;
+    const int t1 = min(a.S, t0 + len);
+    const float* __restrict__ lp = a.logps + r * a.lp_row;
+    const uint8_t* __restrict__ mk = a.mask + r * a.mk_row;
     const float row_adv = a.adv_tok == 0 ? a.adv[r * a.adv_row] : 0.f;
     const float w = static_cast<float>(a.by_sequence ? inv_rows / max(counts[r], 1) : inv_tokens);
+    float* __restrict__ gp = grad + r * a.S;
     float sl = 0.f, sk = 0.f;
     int sc = 0;
-#pragma unroll 2
-    for (int t = t0 + lane * VEC; t < t1; t += 32 * VEC) {
-      float x[VEC], o[VEC], f[VEC], A[VEC], g[VEC];
-      bool m[VEC];
+    float x[VEC], o[VEC], f[VEC], A[VEC];
+    bool m[VEC];
+    auto fetch = [&](int t) {
       load_f<VEC>(lp + t, x);
       load_mask<VEC>(mk + t, m);
       if (a.old != nullptr) load_any<VEC>(a.old, a.old_bf16, r * a.old_row + t, o);
       if (a.ref != nullptr) load_any<VEC>(a.ref, a.ref_bf16, r * a.ref_row + t, f);
       if (a.adv_tok != 0) load_f<VEC>(a.adv + r * a.adv_row + t, A);
+    };
+    int t = t0 + lane * VEC;
+    if (t < t1) fetch(t);
+    for (; t < t1; t += 32 * VEC) {
+      // this step's values, then the next step's loads ahead of the arithmetic
+      float lr[VEC], df[VEC], adv[VEC], g[VEC];
+      bool mm[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float adv = a.adv_tok != 0 ? A[j] : row_adv;
-        const float lr = a.old != nullptr ? x[j] - o[j] : 0.f;
-        const float ratio = a.old != nullptr ? expf(lr) : 1.f;
-        const bool up = adv > 0.f && lr > a.log_hi, dn = adv < 0.f && lr < a.log_lo;
-        float l = -(up ? a.hi : dn ? a.lo : ratio) * adv;
-        float d = (up || dn) ? 0.f : -adv * ratio;
+        lr[j] = a.old != nullptr ? x[j] - o[j] : 0.f;
+        df[j] = a.ref != nullptr ? f[j] - x[j] : 0.f;
+        adv[j] = a.adv_tok != 0 ? A[j] : row_adv;
+        mm[j] = m[j];
+      }
+      if (t + 32 * VEC < t1) fetch(t + 32 * VEC);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float ratio = a.old != nullptr ? expf(lr[j]) : 1.f;
+        const bool up = adv[j] > 0.f && lr[j] > a.log_hi, dn = adv[j] < 0.f && lr[j] < a.log_lo;
+        const bool clip = up || dn;
+        float l = -(up ? a.hi : dn ? a.lo : ratio) * adv[j];
+        float d = clip ? 0.f : -adv[j] * ratio;
         if (a.ref != nullptr) {
-          const float df = f[j] - x[j], em1 = expm1f(df), k3 = kl_term(df, em1);
-          sk += m[j] ? k3 : 0.f;
+          float em1, k3;
+          kl_terms(df[j], em1, k3);
+          sk += mm[j] ? k3 : 0.f;
           l = fmaf(a.kl_coef, k3, l);
           d = fmaf(-a.kl_coef, em1, d);
         }
-        sl += m[j] ? l : 0.f;
-        sc += (m[j] && (up || dn)) ? 1 : 0;
-        g[j] = m[j] ? d * w : 0.f;
+        sl += mm[j] ? l : 0.f;
+        sc += (mm[j] && clip) ? 1 : 0;
+        g[j] = mm[j] ? d * w : 0.f;
       }
       if (grad != nullptr) {
-        float* gp = grad + r * a.S + t;
         if (VEC == 4)
-          *reinterpret_cast<float4*>(gp) = make_float4(g[0], g[1 % VEC], g[2 % VEC], g[3 % VEC]);
+          *reinterpret_cast<float4*>(gp + t) = make_float4(g[0], g[1 % VEC], g[2 % VEC], g[3 % VEC]);
         else
-          *gp = g[0];
+          gp[t] = g[0];
       }
     }
     loss += static_cast<double>(sl) * w;
@@ -436,21 +456,80 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-template <typename T, int VEC, int G, int NV>
-__device__ __forceinline__ void load_row(const T* p, int sub, int E, float (&x)[NV * VEC]) {
+template <typename T, int VEC, int NV>
+struct RowRaw {
+  Pack<T, VEC> v[NV];
+};
+
+// a lane's part of one row as stored; p points at the lane's first column. Columns past E (a
+// multiple of VEC) are not read: FULL rows have none.
+template <typename T, int VEC, int G, int NV, bool FULL>
+__device__ __forceinline__ void fetch_row(const T* p, int sub, int E, RowRaw<T, VEC, NV>& x) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+    if (FULL || (v * G + sub) * VEC < E) x.v[v] = *reinterpret_cast<const Pack<T, VEC>*>(p + v * G * VEC);
+}
+
+// bf16 values are the upper halves of fp32 ones: one shift or mask each
+__device__ __forceinline__ float pair_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float pair_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+template <typename T, int VEC, int G, int NV, bool FULL>
+__device__ __forceinline__ void unpack_row(const RowRaw<T, VEC, NV>& r, int sub, int E, float (&x)[NV * VEC]) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = (v * G + sub) * VEC;
-    if (c < E) {  // E is a multiple of VEC
-      const Pack<T, VEC> u = *reinterpret_cast<const Pack<T, VEC>*>(p + c);
+    const bool has = FULL || (v * G + sub) * VEC < E;
+    if (sizeof(T) == 2 && VEC == 8) {
+      const uint4 u = *reinterpret_cast<const uint4*>(&r.v[v]);
+      const uint32_t* w = &u.x;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) x[v * VEC + j] = static_cast<float>(u.v[j]);
+      for (int j = 0; j < VEC / 2; ++j) {
+        x[v * VEC + 2 * j] = has ? pair_lo(w[j]) : -INFINITY;
+        x[v * VEC + (2 * j + 1) % VEC] = has ? pair_hi(w[j]) : -INFINITY;
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) x[v * VEC + j] = -INFINITY;
+      for (int j = 0; j < VEC; ++j) x[v * VEC + j] = has ? static_cast<float>(r.v[v].v[j]) : -INFINITY;
     }
   }
 }
+
+// Walks a warp's rows through the layers' matrices: kGroups = 32 / G neighbouring rows a step,
+// a group of lanes per row, steps of all warps interleaved so that the machine reads one
+// window of memory at a time. `p` is the lane's place in its group's current row. Rows number
+// fewer than 2^30 (checked by the launcher).
+template <typename T, int VEC, int G>
+struct RowWalk {
+  static constexpr int kGroups = 32 / G;
+  const T* p;
+  int r, end, t, layer, stride;
+  __device__ __forceinline__ RowWalk(const RouterArgs& a, int warp, int warps, int sub, int grp)
+      : r(warp * kGroups + grp), end(a.L * static_cast<int>(a.T)), stride(warps * kGroups) {
+    layer = r / static_cast<int>(a.T);
+    t = r - layer * static_cast<int>(a.T);
+    place(a, sub);
+  }
+  __device__ __forceinline__ void place(const RouterArgs& a, int sub) {
+    if (r < end) p = static_cast<const T*>(a.logits[layer]) + t * a.ld[layer] + sub * VEC;
+  }
+  __device__ __forceinline__ bool in() const { return r < end; }
+  // the row's mask byte, fetched beside the row: a row that does not count is read all the
+  // same, so that its load does not wait for the byte
+  __device__ __forceinline__ uint8_t mask(const RouterArgs& a) const {
+    return a.mask == nullptr ? 1 : a.mask[t];
+  }
+  __device__ __forceinline__ void next(const RouterArgs& a, int sub) {
+    const int T_ = static_cast<int>(a.T);
+    r += stride;
+    if (r >= end) return;
+    t += stride;
+    while (t >= T_) {
+      t -= T_;
+      ++layer;
+    }
+    place(a, sub);
+  }
+};
 
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -465,17 +544,22 @@ __device__ __forceinline__ float group_max(float v) {
   return v;
 }
 
-constexpr int kRouterThreads = 512;
+// Blocks an SM: the sums keep 32 bf16 values a lane (fewer shuffles and scalar steps for a row:
+// 112 us instead of 131 for the rows alone of 24 x 32768 x 256), the gradient 16.
+constexpr int kRouterThreads = 256, kRouterSumsResident = 2, kRouterGradResident = 4;
 
 // Per block: column sums of the probabilities, the sum of lse^2, the kept tokens and the
 // histogram of the chosen experts over the block's rows; lse of every row for the backward.
-template <typename T, int VEC, int G, int NV>
-__global__ void __launch_bounds__(kRouterThreads) router_sums_kernel(const __grid_constant__ RouterArgs a,
+template <typename T, int VEC, int G, int NV, bool FULL>
+__global__ void __launch_bounds__(kRouterThreads, kRouterSumsResident) router_sums_kernel(const __grid_constant__ RouterArgs a,
                                                                      float* __restrict__ lse_out,
                                                                      float* __restrict__ part_p,
                                                                      int* __restrict__ part_n,
-                                                                     double* __restrict__ part_z) {
+                                                                     double* __restrict__ part_z,
+                                                                     unsigned* __restrict__ ticket) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
   constexpr int kEl = NV * VEC, kCover = G * kEl, kGroups = 32 / G, kWarps = kRouterThreads / 32;
+  static_assert(kEl % 2 == 0, "values are processed in pairs");
   __shared__ float s_p[kCover];
   __shared__ int s_hist[kCover];
   __shared__ double s_z[kWarps];
@@ -493,59 +577,63 @@ __global__ void __launch_bounds__(kRouterThreads) router_sums_kernel(const __gri
   for (int i = 0; i < kEl; ++i) acc[i] = 0.f;
   double z = 0.0;
   int kept = 0;
-  // contiguous rows per warp, kGroups at a time
-  const long long total = static_cast<long long>(a.L) * a.T;
-  const long long nw = static_cast<long long>(gridDim.x) * kWarps;
-  const long long wid = static_cast<long long>(blockIdx.x) * kWarps + warp;
-  const long long r_begin = total * wid / nw, r_end = total * (wid + 1) / nw;
-  int layer = static_cast<int>((r_begin + grp) / a.T);
-  long long t = (r_begin + grp) - static_cast<long long>(layer) * a.T;
-  for (long long r0 = r_begin; r0 < r_end; r0 += kGroups) {
-    const long long r = r0 + grp;
-    const bool in = r < r_end;
-    const bool keep = in && (a.mask == nullptr || a.mask[t] != 0);
+  // each row is fetched one step ahead
+  RowWalk<T, VEC, G> w(a, blockIdx.x * kWarps + warp, gridDim.x * kWarps, sub, grp);
+  RowRaw<T, VEC, NV> raw;
+  uint8_t keep = 0;
+  if (w.in()) {
+    keep = w.mask(a);
+    fetch_row<T, VEC, G, NV, FULL>(w.p, sub, a.E, raw);
+  }
+  float zf = 0.f;
+  while (__any_sync(0xffffffffu, w.in())) {
+    const int r = w.r;
+    const bool kept_row = w.in() && keep != 0;
+    // the row's chosen experts, spread over its lanes: read here, counted after the arithmetic
+    const int64_t* ip = w.in() ? a.idx[w.layer] + static_cast<long long>(w.t) * a.k : nullptr;
+    int64_t chosen[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) chosen[j] = w.in() && sub + j * G < a.k ? ip[sub + j * G] : -1;
     float x[kEl];
-#pragma unroll
-    for (int i = 0; i < kEl; ++i) x[i] = -INFINITY;
-    if (in) {
-      load_row<T, VEC, G, NV>(static_cast<const T*>(a.logits[layer]) + t * a.ld[layer], sub, a.E, x);
-      if (keep) {
-        const int64_t* ip = a.idx[layer] + t * a.k;
-        for (int j = sub; j < a.k; j += G) {
-          const int64_t e = ip[j];
-          if (e >= 0 && e < a.E) atomicAdd(&s_hist[e], 1);
-          else s_bad = 1;
-        }
-      }
+    unpack_row<T, VEC, G, NV, FULL>(raw, sub, a.E, x);
+    w.next(a, sub);
+    if (w.in()) {
+      keep = w.mask(a);
+      fetch_row<T, VEC, G, NV, FULL>(w.p, sub, a.E, raw);
     }
-    float m = x[0];
+    // exponentials relative to the lane's own maximum, so that they do not wait for the row's
+    float ml = fmax3(x[0], x[1], x[2 % kEl]);
 #pragma unroll
-    for (int i = 1; i < kEl; ++i) m = fmaxf(m, x[i]);
-    m = group_max<G>(m);
-    const float ml = m * kLog2e;
-    float s = 0.f;
+    for (int e = 3; e + 1 < kEl; e += 2) ml = fmax3(ml, x[e], x[e + 1]);
+    ml = fmaxf(ml, x[kEl - 1]) * kLog2e;
+    const float off = ml == -INFINITY ? 0.f : ml;  // a lane past the last column
+    float s = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < kEl; ++i) {
-      x[i] = fast_exp2(fmaf(x[i], kLog2e, -ml));
-      s += x[i];
+    for (int e = 0; e < kEl; e += 2) {
+      x[e] = fast_exp2(fmaf(x[e], kLog2e, -off));
+      x[e + 1] = fast_exp2(fmaf(x[e + 1], kLog2e, -off));
+      s += x[e];
+      s1 += x[e + 1];
     }
-    s = group_sum<G>(s);
-    const float inv = 1.f / s, lse = m + kLn2 * log2f(s);
-    if (keep) {
+    const float m = group_max<G>(ml), to_row = fast_exp2(ml - m);
+    s = group_sum<G>((s + s1) * to_row);
+    const float inv = __fdividef(to_row, s), lse = kLn2 * (m + log2f(s));
+    if (kept_row) {
 #pragma unroll
-      for (int i = 0; i < kEl; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
+      for (int e = 0; e < kEl; ++e) acc[e] = fmaf(x[e], inv, acc[e]);
       if (sub == 0) {
-        z += static_cast<double>(lse) * lse;
+        zf = fmaf(lse, lse, zf);
         ++kept;
+        lse_out[r] = lse;
       }
-    }
-    if (in && sub == 0) lse_out[r] = lse;
-    t += kGroups;
-    while (t >= a.T) {
-      t -= a.T;
-      ++layer;
+      for (int j = sub; j < a.k; j += G) {
+        const int64_t e = j < G ? chosen[0] : j < 2 * G ? chosen[1] : ip[j];
+        if (e >= 0 && e < a.E) atomicAdd(&s_hist[e], 1);
+        else s_bad = 1;
+      }
     }
   }
+  z = zf;
   // the warps add their column sums in turn: a fixed order
 #pragma unroll
   for (int i = 0; i < kEl; ++i) {
@@ -582,71 +670,85 @@ __global__ void __launch_bounds__(kRouterThreads) router_sums_kernel(const __gri
   }
 }
 
-// One block joins the partial sums: loss, counts, and the backward's constants
+// Joins the partial sums, 32 columns a block; the last block to finish adds the blocks' parts
+// of the loss in their order. counts, and the backward's constants
 //   slope[e] = c_b E / n * f_e  and  slope[E] = 2 c_z / n
 __global__ void __launch_bounds__(1024) router_join_kernel(const float* __restrict__ part_p,
                                                            const int* __restrict__ part_n,
                                                            const double* __restrict__ part_z, int blocks,
                                                            int E, float balance, float zcoef,
+                                                           double* __restrict__ dots,
+                                                           unsigned* __restrict__ ticket,
                                                            float* __restrict__ loss,
                                                            int64_t* __restrict__ counts,
                                                            float* __restrict__ slope) {
   __shared__ double s_p[32][33];
-  __shared__ long long s_n[32][33];
-  __shared__ double s_red[32], s_tot[2];
+  __shared__ int s_n[32][33];
+  __shared__ double s_tot[2];
+  __shared__ bool s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (warp == 0) {
-    double z = 0.0, n = 0.0;
+  const int c = blockIdx.x * 32 + lane;
+  double p = 0.0;
+  int n = 0;  // at most L T k < 2^31 choices, checked by the launcher
+  if (c < E) {
+    // every load in flight at once: this kernel is one trip to memory
+    constexpr int kTrips = (148 * kRouterSumsResident + 31) / 32;
+    float pv[kTrips];
+    int nv[kTrips];
+#pragma unroll
+    for (int i = 0; i < kTrips; ++i) {
+      const int b = warp + 32 * i;
+      pv[i] = b < blocks ? part_p[static_cast<long long>(b) * E + c] : 0.f;
+      nv[i] = b < blocks ? part_n[static_cast<long long>(b) * E + c] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kTrips; ++i) {
+      p += pv[i];
+      n += nv[i];
+    }
+  }
+  s_p[warp][lane] = p;
+  s_n[warp][lane] = n;
+  if (warp == 1) {
+    double z = 0.0, k = 0.0;
     for (int b = lane; b < blocks; b += 32) {
       z += part_z[2 * b];
-      n += part_z[2 * b + 1];
+      k += part_z[2 * b + 1];
     }
     z = warp_sum_d(z);
-    n = warp_sum_d(n);
+    k = warp_sum_d(k);
     if (lane == 0) {
       s_tot[0] = z;
-      s_tot[1] = n > 0.0 ? n : 1.0;
+      s_tot[1] = k > 0.0 ? k : 1.0;
     }
   }
-  // cols chunks of 32 columns at a time, 32 / cols warps striding over the blocks of each
-  const int all = (E + 31) / 32;
-  int cols = 1;
-  while (cols < 32 && cols < all) cols *= 2;
-  const int per = 32 / cols;
+  __syncthreads();
+  if (warp != 0) return;
+  const double tokens = s_tot[1];
   double dot = 0.0;
-  for (int c0 = 0; c0 < all; c0 += cols) {
-    const int c = (c0 + warp / per) * 32 + lane;
-    double p = 0.0;
-    long long n = 0;
-    if (c < E) {
-#pragma unroll 8
-      for (int b = warp % per; b < blocks; b += per) {
-        p += part_p[static_cast<long long>(b) * E + c];
-        n += part_n[static_cast<long long>(b) * E + c];
-      }
+  if (c < E) {
+    long long total = 0;
+    p = 0.0;
+    for (int w = 0; w < 32; ++w) {
+      p += s_p[w][lane];
+      total += s_n[w][lane];
     }
-    __syncthreads();
-    s_p[warp][lane] = p;
-    s_n[warp][lane] = n;
-    __syncthreads();
-    if (warp % per == 0 && c < E) {
-      for (int w = 1; w < per; ++w) {
-        p += s_p[warp + w][lane];
-        n += s_n[warp + w][lane];
-      }
-      const double tokens = s_tot[1], f = static_cast<double>(n) / tokens;
-      counts[c] = n;
-      slope[c] = static_cast<float>(balance * E / tokens * f);
-      dot += f * (p / tokens);
-    }
+    const double f = static_cast<double>(total) / tokens;
+    counts[c] = total;
+    slope[c] = static_cast<float>(balance * E / tokens * f);
+    dot = f * (p / tokens);
   }
   dot = warp_sum_d(dot);
-  if (lane == 0) s_red[warp] = dot;
-  __syncthreads();
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
+    dots[blockIdx.x] = dot;
+    __threadfence();
+    s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  }
+  __syncwarp();
+  if (s_last && lane == 0) {
+    __threadfence();
     double t = 0.0;
-    for (int w = 0; w < 32; ++w) t += s_red[w];
-    const double tokens = s_tot[1];
+    for (int b = 0; b < gridDim.x; ++b) t += static_cast<volatile double*>(dots)[b];
     // NaN in s_tot[0] marks a chosen index outside [0, E)
     const bool bad = !(s_tot[0] == s_tot[0]);
     *loss = static_cast<float>(balance * E * t + (zcoef != 0.f || bad ? zcoef * s_tot[0] / tokens : 0.0));
@@ -655,8 +757,8 @@ __global__ void __launch_bounds__(1024) router_join_kernel(const float* __restri
 }
 
 // dlogit = gout p (slope_e - <p, slope> + slope_E lse), 0 in masked rows
-template <typename T, int VEC, int G, int NV>
-__global__ void __launch_bounds__(kRouterThreads) router_grad_kernel(const __grid_constant__ RouterArgs a,
+template <typename T, int VEC, int G, int NV, bool FULL>
+__global__ void __launch_bounds__(kRouterThreads, NV * VEC > 16 ? 2 : sizeof(T) == 2 ? kRouterGradResident : 3) router_grad_kernel(const __grid_constant__ RouterArgs a,
                                                                      const float* __restrict__ lse_in,
                                                                      const float* __restrict__ slope,
                                                                      const float* __restrict__ gout,
@@ -671,51 +773,47 @@ __global__ void __launch_bounds__(kRouterThreads) router_grad_kernel(const __gri
     const int c = ((i / VEC) * G + sub) * VEC + i % VEC;
     f[i] = c < a.E ? slope[c] * go : 0.f;
   }
-  const long long total = static_cast<long long>(a.L) * a.T;
-  const long long nw = static_cast<long long>(gridDim.x) * kWarps;
-  const long long wid = static_cast<long long>(blockIdx.x) * kWarps + warp;
-  const long long r_begin = total * wid / nw, r_end = total * (wid + 1) / nw;
-  int layer = static_cast<int>((r_begin + grp) / a.T);
-  long long t = (r_begin + grp) - static_cast<long long>(layer) * a.T;
-  for (long long r0 = r_begin; r0 < r_end; r0 += kGroups) {
-    const long long r = r0 + grp;
-    const bool in = r < r_end;
-    const bool keep = in && (a.mask == nullptr || a.mask[t] != 0);
+  RowWalk<T, VEC, G> w(a, blockIdx.x * kWarps + warp, gridDim.x * kWarps, sub, grp);
+  RowRaw<T, VEC, NV> raw;
+  float lse_next = 0.f;
+  uint8_t keep = 0;
+  auto fetch = [&] {
+    if (w.in()) {
+      keep = w.mask(a);
+      lse_next = lse_in[w.r];  // not written for rows that do not count, and not used there
+      fetch_row<T, VEC, G, NV, FULL>(w.p, sub, a.E, raw);
+    }
+  };
+  fetch();
+  while (__any_sync(0xffffffffu, w.in())) {
+    T* g = grad + static_cast<long long>(w.r) * a.E + sub * VEC;
+    const bool now = w.in(), kept = now && keep != 0;
     float x[kEl];
-    float lse = 0.f;
+    unpack_row<T, VEC, G, NV, FULL>(raw, sub, a.E, x);
+    const float lse = lse_next, l2 = lse * kLog2e;
+    w.next(a, sub);
+    fetch();
+    float d = 0.f, d1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < kEl; ++i) x[i] = -INFINITY;
-    if (keep) {
-      load_row<T, VEC, G, NV>(static_cast<const T*>(a.logits[layer]) + t * a.ld[layer], sub, a.E, x);
-      lse = lse_in[r];
+    for (int e = 0; e < kEl; e += 2) {
+      x[e] = fast_exp2(fmaf(x[e], kLog2e, -l2));
+      x[e + 1] = fast_exp2(fmaf(x[e + 1], kLog2e, -l2));
+      d = fmaf(x[e], f[e], d);
+      d1 = fmaf(x[e + 1], f[e + 1], d1);
     }
-    const float l2 = lse * kLog2e;
-    float d = 0.f;
-#pragma unroll
-    for (int i = 0; i < kEl; ++i) {
-      x[i] = fast_exp2(fmaf(x[i], kLog2e, -l2));
-      d = fmaf(x[i], f[i], d);
-    }
-    d = group_sum<G>(d);
+    d = group_sum<G>(d + d1);
     const float c = zs * lse - d;
-    if (in) {
-      T* g = grad + r * a.E;
+    if (now) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int col = (v * G + sub) * VEC;
-        if (col < a.E) {
+        if (FULL || (v * G + sub) * VEC < a.E) {
           Pack<T, VEC> u;
 #pragma unroll
           for (int j = 0; j < VEC; ++j)
-            u.v[j] = static_cast<T>(keep ? x[v * VEC + j] * (f[v * VEC + j] + c) : 0.f);
-          *reinterpret_cast<Pack<T, VEC>*>(g + col) = u;
+            u.v[j] = static_cast<T>(kept ? x[v * VEC + j] * (f[v * VEC + j] + c) : 0.f);
+          *reinterpret_cast<Pack<T, VEC>*>(g + v * G * VEC) = u;
         }
       }
-    }
-    t += kGroups;
-    while (t >= a.T) {
-      t -= a.T;
-      ++layer;
     }
   }
 }
@@ -724,7 +822,16 @@ int warp_grid(long long units) {
   return static_cast<int>(std::max<long long>(1, std::min<long long>((units + 7) / 8, 148 * 8)));
 }
 
-int chunks_of(int S) { return (S + kWarpTokens - 1) / kWarpTokens; }
+int warp_tokens(long long rows, int S) {
+  int len = kMaxWarpTokens;
+  while (len > kMinWarpTokens && rows * ((S + len - 1) / len) < 148LL * 16) len /= 2;
+  return len;
+}
+
+int chunks_of(long long rows, int S) {
+  const int len = warp_tokens(rows, S);
+  return std::max(1, (S + len - 1) / len);
+}
 
 // 4 tokens at a time need every row to start on a boundary of 4 elements
 bool aligned4(const void* p, int bytes, std::initializer_list<long long> strides) {
@@ -734,23 +841,32 @@ bool aligned4(const void* p, int bytes, std::initializer_list<long long> strides
   return true;
 }
 
-// the widest layout for E columns: 16-byte vectors when rows allow them, 16 values a lane
-template <typename T, typename F>
+// The layout for E columns: 16-byte vectors where every row allows them, PER_LANE values a lane
+// in the fewest lanes that hold a row (twice as many where 32 lanes do not); FULL where they
+// hold exactly it.
+template <typename T, int PER_LANE, typename F>
 void router_dispatch(int E, bool vec, F&& launch) {
-  constexpr int V = 16 / sizeof(T), N = 16 / V;
+  constexpr int V = 16 / sizeof(T), N = PER_LANE / V, K = PER_LANE;
+  auto pick = [&](auto VEC, auto G, auto NV) {
+    if (E == VEC.value * G.value * NV.value) launch(VEC, G, NV, std::true_type{});
+    else launch(VEC, G, NV, std::false_type{});
+  };
+  using std::integral_constant;
   if (vec) {
-    if (E <= 16) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, N>{});
-    else if (E <= 32) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, N>{});
-    else if (E <= 64) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, N>{});
-    else if (E <= 128) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 8>{}, std::integral_constant<int, N>{});
-    else if (E <= 256) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 16>{}, std::integral_constant<int, N>{});
-    else if (E <= 512) launch(std::integral_constant<int, V>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, N>{});
-    else launch(std::integral_constant<int, V>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 2 * N>{});
+    if (E <= K) pick(integral_constant<int, V>{}, integral_constant<int, 1>{}, integral_constant<int, N>{});
+    else if (E <= 2 * K) pick(integral_constant<int, V>{}, integral_constant<int, 2>{}, integral_constant<int, N>{});
+    else if (E <= 4 * K) pick(integral_constant<int, V>{}, integral_constant<int, 4>{}, integral_constant<int, N>{});
+    else if (E <= 8 * K) pick(integral_constant<int, V>{}, integral_constant<int, 8>{}, integral_constant<int, N>{});
+    else if (E <= 16 * K) pick(integral_constant<int, V>{}, integral_constant<int, 16>{}, integral_constant<int, N>{});
+    else if (E <= 32 * K) pick(integral_constant<int, V>{}, integral_constant<int, 32>{}, integral_constant<int, N>{});
+    else if constexpr (K < 32) pick(integral_constant<int, V>{}, integral_constant<int, 32>{}, integral_constant<int, 2 * N>{});
   } else {
-    if (E <= 128) launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
-    else if (E <= 256) launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
-    else if (E <= 512) launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
-    else launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 32>{});
+    using One = integral_constant<int, 1>;
+    using Warp = integral_constant<int, 32>;
+    if (E <= 128) launch(One{}, Warp{}, integral_constant<int, 4>{}, std::false_type{});
+    else if (E <= 256) launch(One{}, Warp{}, integral_constant<int, 8>{}, std::false_type{});
+    else if (E <= 512) launch(One{}, Warp{}, integral_constant<int, 16>{}, std::false_type{});
+    else launch(One{}, Warp{}, integral_constant<int, 32>{}, std::false_type{});
   }
 }
 
@@ -765,20 +881,20 @@ bool router_vec(const RouterArgs& a) {
 
 }  // namespace
 
-int pref_chunks(int S) { return std::max(1, chunks_of(S)); }
+int pref_chunks(int P, int S) { return chunks_of(2LL * P, S); }
 
 int pref_blocks(int P) { return std::max(1, std::min((P + 7) / 8, 148)); }
 
 void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* ticket, float* row_scale,
                   float* loss, float* rewards, cudaStream_t st) {
   if (a.P <= 0) return;
-  const int chunks = pref_chunks(a.S);
+  const int chunks = pref_chunks(a.P, a.S), len = warp_tokens(2LL * a.P, a.S);
   const bool vec = a.S % 4 == 0 && aligned4(a.logps, 4, {a.lp_side, a.lp_pair}) &&
                    aligned4(a.mask, 1, {a.mk_side, a.mk_pair}) &&
                    (a.ref == nullptr || aligned4(a.ref, a.ref_bf16 ? 2 : 4, {a.ref_side, a.ref_pair}));
   const int grid = warp_grid(2LL * a.P * chunks);
-  if (vec) pref_sums_kernel<4><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, ticket);
-  else pref_sums_kernel<1><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, ticket);
+  if (vec) pref_sums_kernel<4><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, len, ticket);
+  else pref_sums_kernel<1><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, len, ticket);
   PLG_CUDA_CHECK(cudaGetLastError());
   pref_pairs_kernel<<<pref_blocks(a.P), 256, 0, st>>>(a, static_cast<const float2*>(part), chunks, block_loss,
                                                       ticket, row_scale, loss, rewards);
@@ -787,11 +903,11 @@ void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* t
 
 void pref_backward(const PrefArgs& a, const float* row_scale, const float* gout, float* grad, cudaStream_t st) {
   if (a.P <= 0 || a.S <= 0) return;
-  const int chunks = pref_chunks(a.S);
+  const int chunks = pref_chunks(a.P, a.S), len = warp_tokens(2LL * a.P, a.S);
   const bool vec = a.S % 4 == 0 && aligned4(a.mask, 1, {a.mk_side, a.mk_pair}) && aligned4(grad, 4, {});
   const int grid = warp_grid(2LL * a.P * chunks);
-  if (vec) pref_grad_kernel<4><<<grid, 256, 0, st>>>(a, row_scale, gout, grad, chunks);
-  else pref_grad_kernel<1><<<grid, 256, 0, st>>>(a, row_scale, gout, grad, chunks);
+  if (vec) pref_grad_kernel<4><<<grid, 256, 0, st>>>(a, row_scale, gout, grad, chunks, len);
+  else pref_grad_kernel<1><<<grid, 256, 0, st>>>(a, row_scale, gout, grad, chunks, len);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
@@ -800,7 +916,7 @@ int policy_count_blocks(int R, int S) {
   return static_cast<int>(std::max<long long>(1, std::min<long long>(b, 148 * 4)));
 }
 
-int policy_blocks(int R, int S) { return warp_grid(static_cast<long long>(R) * std::max(1, chunks_of(S))); }
+int policy_blocks(int R, int S) { return warp_grid(static_cast<long long>(R) * chunks_of(R, S)); }
 
 void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double* block_sums,
                     unsigned* ticket, float* grad, float* out, cudaStream_t st) {
@@ -810,14 +926,14 @@ void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double
   if (a.S > 2048) policy_counts_kernel<true><<<cb, 256, 0, st>>>(a, counts, bc, ticket);
   else policy_counts_kernel<false><<<cb, 256, 0, st>>>(a, counts, bc, ticket);
   PLG_CUDA_CHECK(cudaGetLastError());
-  const int chunks = std::max(1, chunks_of(a.S));
+  const int chunks = chunks_of(a.R, a.S), len = warp_tokens(a.R, a.S);
   const bool vec = a.S % 4 == 0 && aligned4(a.logps, 4, {a.lp_row}) && aligned4(a.mask, 1, {a.mk_row}) &&
                    (a.old == nullptr || aligned4(a.old, a.old_bf16 ? 2 : 4, {a.old_row})) &&
                    (a.ref == nullptr || aligned4(a.ref, a.ref_bf16 ? 2 : 4, {a.ref_row})) &&
                    (a.adv_tok == 0 || aligned4(a.adv, 4, {a.adv_row})) && aligned4(grad, 4, {});
   const int grid = policy_blocks(a.R, a.S);
-  if (vec) policy_kernel<4><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket, grad, out, chunks);
-  else policy_kernel<1><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket, grad, out, chunks);
+  if (vec) policy_kernel<4><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket, grad, out, chunks, len);
+  else policy_kernel<1><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket, grad, out, chunks, len);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
@@ -830,31 +946,34 @@ void scale_unless_one(float* x, long long n, const float* s, cudaStream_t st) {
 }
 
 int router_blocks(long long rows) {
-  // at least 64 rows a block, at most two blocks an SM (their partial sums are joined by one)
-  return static_cast<int>(std::max<long long>(1, std::min<long long>((rows + 63) / 64, 296)));
+  // at least 64 rows a block
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((rows + 63) / 64, 148 * kRouterSumsResident)));
 }
 
 void router_balance_forward(const RouterArgs& a, bool bf16, float balance, float zcoef, float* lse,
-                            float* part_p, int* part_n, double* part_z, float* loss, int64_t* counts,
-                            float* slope, cudaStream_t st) {
+                            float* part_p, int* part_n, double* part_z, double* dots, unsigned* ticket,
+                            float* loss, int64_t* counts, float* slope, cudaStream_t st) {
   if (a.E < 1 || a.E > kRouterMaxExperts || a.L < 1 || a.L > kRouterMaxLayers || a.k < 0)
     throw std::invalid_argument("router_balance_loss: 1..1024 experts and 1..128 layers in one call");
   const long long rows = static_cast<long long>(a.L) * a.T;
+  if (rows >= 1 << 30 || rows * std::max(a.k, 1) > INT32_MAX)
+    throw std::invalid_argument("router_balance_loss: more than 2^30 rows or 2^31 choices in one call");
   const int blocks = router_blocks(rows);
+  if (rows == 0) PLG_CUDA_CHECK(cudaMemsetAsync(ticket, 0, sizeof(unsigned), st));
   if (rows > 0) {
     auto run = [&](auto* tag, bool vec) {
       using T = std::remove_pointer_t<decltype(tag)>;
-      router_dispatch<T>(a.E, vec, [&](auto V, auto G, auto N) {
-        router_sums_kernel<T, V.value, G.value, N.value><<<blocks, kRouterThreads, 0, st>>>(a, lse, part_p, part_n,
-                                                                                          part_z);
+      router_dispatch<T, sizeof(T) == 2 ? 32 : 16>(a.E, vec, [&](auto V, auto G, auto N, auto FULL) {
+        router_sums_kernel<T, V.value, G.value, N.value, FULL.value><<<blocks, kRouterThreads, 0, st>>>(a, lse, part_p, part_n,
+                                                                                          part_z, ticket);
       });
     };
     if (bf16) run(static_cast<__nv_bfloat16*>(nullptr), router_vec<__nv_bfloat16>(a));
     else run(static_cast<float*>(nullptr), router_vec<float>(a));
     PLG_CUDA_CHECK(cudaGetLastError());
   }
-  router_join_kernel<<<1, 1024, 0, st>>>(part_p, part_n, part_z, rows > 0 ? blocks : 0, a.E, balance, zcoef, loss,
-                                         counts, slope);
+  router_join_kernel<<<(a.E + 31) / 32, 1024, 0, st>>>(part_p, part_n, part_z, rows > 0 ? blocks : 0, a.E, balance,
+                                                       zcoef, dots, ticket, loss, counts, slope);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
@@ -862,12 +981,13 @@ void router_balance_backward(const RouterArgs& a, bool bf16, const float* lse, c
                              const float* gout, void* grad, cudaStream_t st) {
   const long long rows = static_cast<long long>(a.L) * a.T;
   if (rows <= 0) return;
-  const int blocks = router_blocks(rows);
+  const int blocks =
+      static_cast<int>(std::max<long long>(1, std::min<long long>((rows + 31) / 32, 148 * kRouterGradResident)));
   auto run = [&](auto* tag, bool vec) {
     using T = std::remove_pointer_t<decltype(tag)>;
     vec = vec && (reinterpret_cast<uintptr_t>(grad) & 15) == 0;
-    router_dispatch<T>(a.E, vec, [&](auto V, auto G, auto N) {
-      router_grad_kernel<T, V.value, G.value, N.value><<<blocks, kRouterThreads, 0, st>>>(a, lse, slope, gout,
+    router_dispatch<T, 16>(a.E, vec, [&](auto V, auto G, auto N, auto FULL) {
+      router_grad_kernel<T, V.value, G.value, N.value, FULL.value><<<blocks, kRouterThreads, 0, st>>>(a, lse, slope, gout,
                                                                                         static_cast<T*>(grad));
     });
   };

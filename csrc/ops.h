@@ -221,8 +221,8 @@ struct PrefArgs {
   float beta = 0.1f, smoothing = 0.f;
   bool normalized = false;    // mean over a sequence's tokens instead of the sum
 };
-int pref_chunks(int S);       // part holds float2 [2 * P * chunks]
-int pref_blocks(int P);       // block_loss holds that many doubles
+int pref_chunks(int P, int S);  // part holds float2 [2 * P * chunks]
+int pref_blocks(int P);         // block_loss holds that many doubles
 // row_scale [2, P] = d loss / d logps of each row's tokens; rewards [2, P] = beta * sums
 void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* ticket, float* row_scale,
                   float* loss, float* rewards, cudaStream_t stream);
@@ -268,10 +268,11 @@ struct RouterArgs {
   int L, E, k;
 };
 int router_blocks(long long rows);
-// lse [L, T]; workspaces part_p, part_n [blocks, E], part_z [blocks, 2]; slope [E + 1]
+// lse [L, T]; workspaces part_p, part_n [blocks, E], part_z [blocks, 2], dots [E / 32 rounded
+// up], ticket [1]; slope [E + 1]
 void router_balance_forward(const RouterArgs& a, bool bf16, float balance, float zcoef, float* lse,
-                            float* part_p, int* part_n, double* part_z, float* loss, int64_t* counts,
-                            float* slope, cudaStream_t stream);
+                            float* part_p, int* part_n, double* part_z, double* dots, unsigned* ticket,
+                            float* loss, int64_t* counts, float* slope, cudaStream_t stream);
 // grad [L, T, E] in the logits' type
 void router_balance_backward(const RouterArgs& a, bool bf16, const float* lse, const float* slope,
                              const float* gout, void* grad, cudaStream_t stream);

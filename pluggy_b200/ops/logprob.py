@@ -65,84 +65,26 @@ def _round_up(n: int, m: int) -> int:
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, labels, ignore_index, w, softcap, temperature, workspace, train):
+    def forward(ctx, hidden, weight, labels, ignore_index, w, softcap, temperature, workspace):
         T, D = hidden.shape
         V = w.shape[0]
-        dev = hidden.device
-        out = torch.empty(T, dtype=torch.float32, device=dev)
-        row_map = inverse = count = lse2 = label_grad = ref = x = None
-        if train or T > UNPACKED_ROWS:
-            rows = _round_up(T, 256)
-            row_map, inverse = torch.empty((2, T), dtype=torch.int32, device=dev)
-            count = torch.empty(3, dtype=torch.int32, device=dev)  # rows, flag, splits
-            ext().head_compact(labels, V, ignore_index, row_map, inverse, count, out)
-            h = torch.empty((rows, D), dtype=torch.bfloat16, device=dev)
-            if train:
-                lse2, label_grad, ref = torch.empty((3, rows), dtype=torch.float32, device=dev)
-                if 2 * rows * V <= workspace and T * V * D >= KEEP_PRODUCT:
-                    x = torch.empty((rows, _round_up(V, 8)), dtype=torch.bfloat16, device=dev)[:, :V]
-                else:
-                    ref = None
-            ext().head_gather(hidden, w, labels, row_map, count, softcap, temperature, h, ref)
-        else:
-            h = hidden.to(torch.bfloat16)
-        ext().head_logprobs(h, w, labels, ignore_index, row_map, count, softcap, temperature, out,
-                            lse2, label_grad, ref, x, status_word(dev))
-        if train:
-            ctx.save_for_backward(h, w, labels, row_map, inverse, count, lse2, label_grad, ref, x)
-            ctx.cfg = (softcap, temperature, workspace, hidden.dtype, weight.dtype, T)
+        keep = 2 * _round_up(T, 256) * V <= workspace and T * V * D >= KEEP_PRODUCT
+        out, *saved = ext().token_logprobs_fwd(hidden, w, labels, ignore_index, softcap, temperature,
+                                               True, True, keep, status_word(hidden.device))
+        ctx.save_for_backward(w, labels, *saved)
+        ctx.cfg = (softcap, temperature, workspace, hidden.dtype, weight.dtype)
         return out
 
     @staticmethod
     def backward(ctx, gout):
-        h, w, labels, row_map, inverse, count, lse2, label_grad, ref, x = ctx.saved_tensors
-        softcap, temperature, workspace, h_dtype, w_dtype, T = ctx.cfg
-        rows, D = h.shape
-        V = w.shape[0]
-        dev = h.device
+        w, labels, h, ints, stats, kept = ctx.saved_tensors
+        softcap, temperature, workspace, h_dtype, w_dtype = ctx.cfg
         need_h, need_w = ctx.needs_input_grad[:2]
-        status = status_word(dev)
-
-        gout = gout.contiguous()
-
-        def recompute(v0, wv, xv, if_flagged):
-            ext().head_recompute(h, wv, v0, labels, row_map, count, softcap, temperature, lse2,
-                                 label_grad, gout, if_flagged, xv, status)
-
-        width, factor, hs = V, None, h
-        if x is not None:
-            recompute(0, w, x, True)  # runs only if a row of x left bf16's range
-            factor = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-            hs = torch.empty_like(h)
-            ext().head_scale_rows(h, w, labels, row_map, count, temperature, lse2, label_grad, ref,
-                                  gout, x, factor, hs)
-        else:
-            if 2 * rows * V > workspace:  # ranges of whole 256-column tiles within the workspace
-                width = max(1, workspace // (2 * rows * 256)) * 256
-            x = torch.empty((rows, _round_up(min(width, V), 8)), dtype=torch.bfloat16, device=dev)
-        # dh's product has few tiles and a long sum: one range's k splits are summed by scatter
-        splits = max(1, min(16, SPLIT_WORKSPACE // (4 * rows * D))) if width >= V else 1
-        dh_rows = torch.empty((splits, rows, D), dtype=torch.float32, device=dev) if need_h else None
-        dw = torch.empty((V, D), dtype=w_dtype, device=dev) if need_w else None
-        for v0 in range(0, V, width):
-            wv = w[v0:v0 + width]
-            xv = x[:, :wv.shape[0]]
-            if factor is None:
-                recompute(v0, wv, xv, False)
-            if need_h and splits > 1:
-                ext().gemm(xv, False, wv, True, dh_rows, None, 1.0, 0.0, 1, 0, status, count, None,
-                           count[2:])
-            elif need_h:
-                ext().gemm(xv, False, wv, True, dh_rows[0], dh_rows[0] if v0 else None, 1.0,
-                           1.0 if v0 else 0.0, 1, 0, status, count, None)
-            if need_w:
-                ext().gemm(xv, True, hs, True, dw[v0:v0 + width], None, 1.0, 0.0, 1, 0, status, None,
-                           count)
-        dh = None
-        if need_h:
-            dh = torch.empty((T, D), dtype=h_dtype, device=dev)
-            ext().head_scatter(dh_rows, count, factor, w, labels, inverse, dh)
-        return (dh, dw) + (None,) * 7
+        dh, dw = ext().token_logprobs_bwd(h, w, labels, ints, stats, kept, gout.contiguous(), softcap,
+                                          temperature, workspace, SPLIT_WORKSPACE,
+                                          h_dtype == torch.float32, w_dtype == torch.float32, need_h,
+                                          need_w, status_word(h.device))
+        return (dh, dw) + (None,) * 6
 
 
 def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
@@ -190,8 +132,12 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: to
     w = weight_lowp if weight_lowp is not None else weight.detach().to(torch.bfloat16)
     h = hidden.reshape(-1, D)
     h, w = _rows_aligned(h), _rows_aligned(w)
-    train = torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
-    out = _TokenLogprobs.apply(h, weight, labels.reshape(-1).contiguous(), int(ignore_index), w,
-                               float(softcap or 0.0), float(temperature),
-                               WORKSPACE if workspace_bytes is None else int(workspace_bytes), train)
+    y = labels.reshape(-1).contiguous()
+    cap, tau = float(softcap or 0.0), float(temperature)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        out = _TokenLogprobs.apply(h, weight, y, int(ignore_index), w, cap, tau,
+                                   WORKSPACE if workspace_bytes is None else int(workspace_bytes))
+    else:
+        (out,) = ext().token_logprobs_fwd(h.detach(), w, y, int(ignore_index), cap, tau,
+                                          h.shape[0] > UNPACKED_ROWS, False, False, status_word(h.device))
     return out.view(labels.shape)

@@ -83,9 +83,6 @@ def moe_expert_ffn(hidden, top_indices, top_weights, gate_up_proj, down_proj, *,
 
 
 # ------------------------------------------------------------------ router losses
-MAX_ROUTER_LAYERS, MAX_ROUTER_EXPERTS = 128, 1024
-
-
 def router_balance_loss_reference(router_logits, top_indices, balance_coef=1.0, z_coef=0.0, mask=None):
     """fp32 math in eager torch on lists of [T, E] logits and [T, k] indices."""
     E = router_logits[0].shape[1]
@@ -109,25 +106,20 @@ class _RouterBalanceLoss(torch.autograd.Function):
     def forward(ctx, idx, mask, balance_coef, z_coef, *logits):
         from pluggy_b200.ops._ext import ext
 
-        T, E = logits[0].shape
-        dev = logits[0].device
-        lse = torch.empty((len(logits), T), dtype=torch.float32, device=dev)
-        counts = torch.empty(E, dtype=torch.int64, device=dev)
-        out = torch.empty(E + 2, dtype=torch.float32, device=dev)
-        ext().router_balance_fwd(logits, idx, mask, balance_coef, z_coef, lse, counts, out)
-        ctx.save_for_backward(lse, out, *logits)
-        ctx.idx, ctx.mask = idx, mask
+        loss, counts, lse, slope = ext().router_balance_fwd(logits, idx, mask, balance_coef, z_coef)
+        ctx.save_for_backward(lse, slope, mask, *logits)
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(counts)
-        return out[E + 1], counts
+        return loss, counts
 
     @staticmethod
     def backward(ctx, gout, _):
         from pluggy_b200.ops._ext import ext
 
-        lse, slope, *logits = ctx.saved_tensors
-        grad = torch.empty((len(logits), *logits[0].shape), dtype=logits[0].dtype, device=lse.device)
-        ext().router_balance_bwd(logits, ctx.idx, ctx.mask, lse, slope, gout, grad)
-        return (None, None, None, None, *grad.unbind())
+        lse, slope, mask, *logits = ctx.saved_tensors
+        if gout is None:
+            return (None,) * (4 + len(logits))
+        return (None, None, None, None, *ext().router_balance_bwd(logits, mask, lse, slope, gout))
 
 
 def router_balance_loss(router_logits, top_indices, *, balance_coef: float = 1.0, z_coef: float = 0.0,
@@ -142,7 +134,8 @@ def router_balance_loss(router_logits, top_indices, *, balance_coef: float = 1.0
         loss = balance_coef * E * sum_e (counts[e] / n) * mean(p[:, e]) + z_coef * mean(logsumexp^2)
 
     Returns ``(loss, counts int64 [E])``; the gradient goes to the logits (the counts are
-    constants, as in the models' auxiliary loss). An index outside [0, E) makes the loss NaN.
+    constants, as in the models' auxiliary loss). An index outside [0, E) makes the loss NaN. On
+    CUDA at most 128 layers of 1024 experts in one call.
 
     CUDA path (csrc/objective.cu): all layers in one launch that keeps a row's probabilities
     in registers and writes only its log-sum-exp, one small kernel for the loss, one launch
@@ -154,25 +147,19 @@ def router_balance_loss(router_logits, top_indices, *, balance_coef: float = 1.0
         raise ValueError(f"router_balance_loss: one index tensor for each router, got {len(logits)} and "
                          f"{len(idx)}")
     x0 = logits[0]
+    if x0.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"router_balance_loss: logits must be bf16 or fp32, got {x0.dtype}")
+    if x0.dim() != 2 or x0.shape[1] == 0:
+        raise ValueError(f"router_balance_loss: logits must be [T, E] with E > 0, got {tuple(x0.shape)}")
+    if x0.is_cuda:  # the extension checks every layer
+        return _RouterBalanceLoss.apply(idx, mask, float(balance_coef), float(z_coef), *logits)
     for x, i in zip(logits, idx):
-        if x.dim() != 2 or x.shape != x0.shape or x.dtype != x0.dtype or x.device != x0.device:
+        if x.shape != x0.shape or x.dtype != x0.dtype or x.device != x0.device:
             raise ValueError("router_balance_loss: the routers' logits must be [T, E], alike")
         if i.shape != (x.shape[0], idx[0].shape[-1]) or i.dtype != torch.int64 or i.device != x.device:
             raise ValueError(f"router_balance_loss: indices must be int64 [T, k], got {i.dtype} "
                              f"{tuple(i.shape)}")
-    if x0.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"router_balance_loss: logits must be bf16 or fp32, got {x0.dtype}")
-    if x0.shape[1] == 0:
-        raise ValueError("router_balance_loss: no experts")
     if mask is not None and (mask.shape != x0.shape[:1] or mask.dtype != torch.bool
                              or mask.device != x0.device):
         raise ValueError(f"router_balance_loss: mask must be bool [{x0.shape[0]}]")
-    if not x0.is_cuda:
-        return router_balance_loss_reference(logits, idx, balance_coef, z_coef, mask)
-    if len(logits) > MAX_ROUTER_LAYERS or x0.shape[1] > MAX_ROUTER_EXPERTS:
-        raise ValueError(f"router_balance_loss: at most {MAX_ROUTER_LAYERS} layers of "
-                         f"{MAX_ROUTER_EXPERTS} experts on CUDA")
-    logits = [x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous() for x in logits]
-    return _RouterBalanceLoss.apply([i.contiguous() for i in idx],
-                                    None if mask is None else mask.contiguous(), float(balance_coef),
-                                    float(z_coef), *logits)
+    return router_balance_loss_reference(logits, idx, balance_coef, z_coef, mask)

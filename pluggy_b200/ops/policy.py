@@ -24,7 +24,7 @@ import math
 import torch
 
 from pluggy_b200.ops._ext import ext
-from pluggy_b200.ops.preference import check_no_grad, tokens_contiguous
+from pluggy_b200.ops.preference import check_no_grad, check_tokens, tokens_contiguous
 
 
 class _KlTerm(torch.autograd.Function):
@@ -73,25 +73,24 @@ def policy_loss_reference(logps, old_logps, advantages, mask, ref_logps=None, cl
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logps, old_logps, advantages, mask, ref_logps, clip_low, clip_high, kl_coef,
-                by_sequence, train):
-        grad = torch.empty(mask.shape, dtype=torch.float32, device=mask.device) if train else None
-        out = torch.empty(3, dtype=torch.float32, device=mask.device)
-        ext().policy_fwd(logps, old_logps, advantages, mask, ref_logps, clip_low, clip_high, kl_coef,
-                         by_sequence, grad, out)
-        ctx.grad = grad
-        loss, kl, clipped = out.unbind()
+                by_sequence):
+        loss, kl, clipped, ctx.grad = ext().policy_fwd(logps, old_logps, advantages, mask, ref_logps,
+                                                       clip_low, clip_high, kl_coef, by_sequence, True)
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(kl, clipped)
         return loss, kl, clipped
 
     @staticmethod
     def backward(ctx, gout, *_):
+        if gout is None:
+            return (None,) * 9
         grad = ctx.grad
         if grad is None:
             raise RuntimeError("policy_loss: backward called twice; the stored gradient is handed out "
                                "by the first call, so retain_graph does not work through this op")
         ctx.grad = None
         ext().scale_unless_one(grad, gout)
-        return (grad,) + (None,) * 9
+        return (grad,) + (None,) * 8
 
 
 def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages: torch.Tensor,
@@ -105,17 +104,6 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
     term. Only ``logps`` has a gradient. Places outside the mask may hold anything."""
     if mask.dim() != 2 or mask.dtype != torch.bool:
         raise ValueError(f"policy_loss: mask must be bool [R, S], got {mask.dtype} {tuple(mask.shape)}")
-    stored = (torch.float32, torch.bfloat16)
-    for name, t, types in (("logps", logps, stored[:1]), ("old_logps", old_logps, stored),
-                           ("ref_logps", ref_logps, stored), ("advantages", advantages, stored[:1])):
-        if t is None:
-            continue
-        per_row = name == "advantages" and t.dim() == 1
-        if t.shape != (mask.shape[:1] if per_row else mask.shape) or t.device != mask.device:
-            raise ValueError(f"policy_loss: {name} must have mask's shape {tuple(mask.shape)} and device, "
-                             f"got {tuple(t.shape)} on {t.device}")
-        if t.dtype not in types:
-            raise TypeError(f"policy_loss: {name} is {t.dtype}, expected one of {types}")
     if not 0 <= clip_low < 1 or not clip_high >= 0:
         raise ValueError("policy_loss: clip_low in [0, 1) and clip_high >= 0")
     if reduction not in ("token", "sequence"):
@@ -124,10 +112,16 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
         raise ValueError("policy_loss: kl_coef needs ref_logps")
     check_no_grad("policy_loss", old_logps=old_logps, ref_logps=ref_logps, advantages=advantages)
     if not mask.is_cuda or mask.shape[0] == 0:
+        fp32 = (torch.float32,)
+        check_tokens("policy_loss", mask, logps=(logps, fp32),
+                     old_logps=(old_logps, (torch.float32, torch.bfloat16)),
+                     ref_logps=(ref_logps, (torch.float32, torch.bfloat16)))
+        check_tokens("policy_loss", mask.any(1) if advantages.dim() == 1 else mask,
+                     advantages=(advantages, fp32))
         return policy_loss_reference(logps, old_logps, advantages, mask, ref_logps, clip_low, clip_high,
                                      kl_coef, reduction)
-    old, ref, adv = (None if t is None else tokens_contiguous(t.detach()) if t.dim() == 2 else t.detach()
-                     for t in (old_logps, ref_logps, advantages))
-    return _PolicyLoss.apply(tokens_contiguous(logps), old, adv, tokens_contiguous(mask), ref,
-                             float(clip_low), float(clip_high), float(kl_coef), reduction == "sequence",
-                             torch.is_grad_enabled() and logps.requires_grad)
+    args = (logps, old_logps, advantages, tokens_contiguous(mask), ref_logps, float(clip_low),
+            float(clip_high), float(kl_coef), reduction == "sequence")
+    if torch.is_grad_enabled() and logps.requires_grad:
+        return _PolicyLoss.apply(*args)
+    return tuple(ext().policy_fwd(*args, False))

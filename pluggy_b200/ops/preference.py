@@ -49,21 +49,31 @@ def preference_loss_reference(logps, ref_logps, mask, beta=0.1, kind="sigmoid", 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logps, ref_logps, mask, beta, kind, label_smoothing, length_normalized):
-        P = mask.shape[1]
-        out = torch.empty(4 * P + 1, dtype=torch.float32, device=mask.device)
-        ext().preference_fwd(logps, ref_logps, mask, KINDS[kind], beta, label_smoothing,
-                             length_normalized, out)
-        ctx.save_for_backward(mask, out)
-        chosen, rejected = out[2 * P:3 * P], out[3 * P:4 * P]
+        loss, chosen, rejected, row_scale = ext().preference_fwd(
+            logps, ref_logps, mask, KINDS[kind], beta, label_smoothing, length_normalized)
+        ctx.save_for_backward(mask, row_scale)
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(chosen, rejected)
-        return out[4 * P], chosen, rejected
+        return loss, chosen, rejected
 
     @staticmethod
     def backward(ctx, gout, *_):
         mask, row_scale = ctx.saved_tensors
-        grad = torch.empty(mask.shape, dtype=torch.float32, device=mask.device)
-        ext().preference_bwd(mask, row_scale, gout, grad)
+        grad = None if gout is None else ext().preference_bwd(mask, row_scale, gout)
         return (grad,) + (None,) * 6
+
+
+def check_tokens(op: str, mask: torch.Tensor, **tensors) -> None:
+    """Shapes, devices and types of (tensor or None, allowed types) against the mask's, for CPU
+    tensors; the CUDA entry points check the same."""
+    for name, (t, types) in tensors.items():
+        if t is None:
+            continue
+        if t.shape != mask.shape or t.device != mask.device:
+            raise ValueError(f"{op}: {name} must have mask's shape {tuple(mask.shape)} and device, got "
+                             f"{tuple(t.shape)} on {t.device}")
+        if t.dtype not in types:
+            raise TypeError(f"{op}: {name} is {t.dtype}, expected one of {types}")
 
 
 def tokens_contiguous(t: torch.Tensor) -> torch.Tensor:
@@ -89,26 +99,18 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
     if mask.dim() != 3 or mask.shape[0] != 2 or mask.dtype != torch.bool:
         raise ValueError(f"preference_loss: mask must be bool [2, P, S], got {mask.dtype} "
                          f"{tuple(mask.shape)}")
-    for name, t, types in (("logps", logps, (torch.float32,)),
-                           ("ref_logps", ref_logps, (torch.float32, torch.bfloat16))):
-        if t is None:
-            continue
-        if t.shape != mask.shape or t.device != mask.device:
-            raise ValueError(f"preference_loss: {name} must have mask's shape {tuple(mask.shape)} and "
-                             f"device, got {tuple(t.shape)} on {t.device}")
-        if t.dtype not in types:
-            raise TypeError(f"preference_loss: {name} is {t.dtype}, expected one of {types}")
     if kind not in KINDS:
         raise ValueError(f"preference_loss: kind must be one of {sorted(KINDS)}, got {kind!r}")
     if not beta > 0:
         raise ValueError("preference_loss: beta must be positive")
     if not 0 <= label_smoothing < 0.5 or (label_smoothing and kind != "sigmoid"):
         raise ValueError("preference_loss: label_smoothing in [0, 0.5), for kind 'sigmoid' only")
-    check_no_grad("preference_loss", ref_logps=ref_logps)
+    if ref_logps is not None and ref_logps.requires_grad:
+        check_no_grad("preference_loss", ref_logps=ref_logps)
     if not mask.is_cuda or mask.shape[1] == 0:
+        check_tokens("preference_loss", mask, logps=(logps, (torch.float32,)),
+                     ref_logps=(ref_logps, (torch.float32, torch.bfloat16)))
         return preference_loss_reference(logps, ref_logps, mask, beta, kind, label_smoothing,
                                          length_normalized)
-    return _PreferenceLoss.apply(tokens_contiguous(logps),
-                                 None if ref_logps is None else tokens_contiguous(ref_logps.detach()),
-                                 tokens_contiguous(mask), float(beta), kind, float(label_smoothing),
-                                 bool(length_normalized))
+    return _PreferenceLoss.apply(logps, ref_logps, tokens_contiguous(mask), float(beta), kind,
+                                 float(label_smoothing), bool(length_normalized))
