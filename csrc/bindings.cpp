@@ -8,7 +8,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <sstream>
 #include <string>
 #include <vector>
 
@@ -589,18 +588,18 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
 
 // ---- objectives over token log-probabilities and router logits
 // Their arguments come from users as they are, so that refusals raise ValueError and TypeError.
-std::string str(at::IntArrayRef v) {
-  std::ostringstream o;
-  o << v;
-  return o.str();
+std::string shape_text(at::IntArrayRef v) {
+  std::string s = "[";
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  return s + "]";
 }
 
 // `t` has `shape` and the device of `like`; its last dimension is made contiguous if need be
 at::Tensor user_tokens(const at::Tensor& t, at::IntArrayRef shape, const at::Tensor& like, const char* op,
                        const char* name, bool bf16_too) {
   if (t.sizes() != shape || t.device() != like.device())
-    throw py::value_error(std::string(op) + ": " + name + " must have shape " + str(shape) +
-                          " on the mask's device, got " + str(t.sizes()));
+    throw py::value_error(std::string(op) + ": " + name + " must have shape " + shape_text(shape) +
+                          " on the mask's device, got " + shape_text(t.sizes()));
   if (!is_f32(t) && !(bf16_too && is_bf16(t)))
     throw py::type_error(std::string(op) + ": " + name + (bf16_too ? " must be fp32 or bf16" : " must be fp32"));
   return t.size(-1) < 2 || t.stride(-1) == 1 ? t : t.contiguous();
@@ -767,7 +766,7 @@ plg::RouterArgs router_args(const std::vector<at::Tensor>& logits, const std::ve
       const at::Tensor& i = (*idx)[l];
       if (i.dim() != 2 || i.size(0) != a.T || i.size(1) != a.k || i.scalar_type() != at::kLong ||
           i.device() != x0.device())
-        throw py::value_error("router_balance_loss: indices must be int64 [T, k], got " + str(i.sizes()));
+        throw py::value_error("router_balance_loss: indices must be int64 [T, k], got " + shape_text(i.sizes()));
       if (!i.is_contiguous()) copies.push_back(i.contiguous());
       a.idx[l] = i.is_contiguous() ? i.data_ptr<int64_t>() : copies.back().data_ptr<int64_t>();
     }
