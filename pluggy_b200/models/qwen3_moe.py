@@ -10,7 +10,11 @@ Parity: reference ``pluggy/models/qwen3_moe/qwen3_moe.py:140-444``:
 * dense blocks from ``decoder_sparse_step`` / ``mlp_only_layers``;
 * Switch load-balance loss and ST-MoE z-loss over the step's router logits,
   ``aux_loss()`` returns their weighted sum (None when no sparse layer ran);
-* ``last_tokens_per_expert`` per-expert token counts for logging.
+* ``last_tokens_per_expert`` per-expert token counts for logging;
+* ``fused_router_losses=True`` (off by default) computes ``aux_loss()`` and the counts by
+  :func:`pluggy_b200.ops.router_balance_loss`: the same formulas on the routers' own top-k
+  choices (the default recomputes the top-k, which differs only where probabilities tie),
+  without the concatenated logits, and with padded tokens left out.
 
 CUDA path: the attention sublayer is the fused ``_engine.AttnSublayer``; the
 sparse MLP composes this package's kernels (RMSNorm, router GEMM, one grouped
@@ -29,7 +33,7 @@ from pluggy_b200.models.common import (GQAttention, RotaryEmbedding, SwiGLU, def
                                        norm_eps, position_ids_for)
 from pluggy_b200.models.qwen3 import Qwen3TransformerBlock
 from pluggy_b200.ops.linear import WeightCache, linear
-from pluggy_b200.ops.moe import expert_histogram, moe_expert_ffn
+from pluggy_b200.ops.moe import expert_histogram, moe_expert_ffn, router_balance_loss
 
 
 class _RouterTopK(torch.autograd.Function):
@@ -172,8 +176,9 @@ class Qwen3Moe(nn.Module):
                  decoder_sparse_step: int = 1, mlp_only_layers: list[int] | None = None,
                  router_aux_loss_coef: float = 0.001, router_z_loss_coef: float = 0.001,
                  rope_base: float = 1_000_000.0, tie_embeddings: bool = False,
-                 router_init_std: float = 0.0):
+                 router_init_std: float = 0.0, fused_router_losses: bool = False):
         super().__init__()
+        self.fused_router_losses = fused_router_losses
         mlp_only = set(mlp_only_layers or [])
         # 0 keeps the routers at zeros through init_weights (the reference's init: every
         # token's top-k then ties on the same experts until training spreads them);
@@ -196,6 +201,7 @@ class Qwen3Moe(nn.Module):
         if tie_embeddings:
             self.lm_head.weight = self.token_emb.weight
         self._router_logits: list[torch.Tensor] = []
+        self._token_mask: torch.Tensor | None = None
         self.last_tokens_per_expert: torch.Tensor | None = None
         self.weight_cache = WeightCache()
         # the expert banks' bf16 copies come from the same cache (kept current by the
@@ -235,7 +241,7 @@ class Qwen3Moe(nn.Module):
     def _update_expert_counts(self, logits) -> None:
         """Tokens routed to each expert this forward, summed over the sparse layers
         (from the routers' own top-k choices)."""
-        if not logits:
+        if not logits or self.fused_router_losses:  # aux_loss() counts them, too
             self.last_tokens_per_expert = None
             return
         counts = torch.zeros(self.num_experts, device=logits[0].device)
@@ -251,6 +257,13 @@ class Qwen3Moe(nn.Module):
         logits = self._router_logits
         if not logits:
             return None
+        if self.fused_router_losses:
+            idx = [b.ffn.last_top_idx for b in self.blocks
+                   if isinstance(b.ffn, Qwen3MoeSparseMLP) and b.ffn.last_router_logits is not None]
+            loss, counts = router_balance_loss(logits, idx, balance_coef=self.router_aux_loss_coef,
+                                               z_coef=self.router_z_loss_coef, mask=self._token_mask)
+            self.last_tokens_per_expert = counts.float()
+            return loss
         loss = torch.zeros((), device=logits[0].device)
         if self.router_aux_loss_coef != 0.0:
             loss = loss + self.router_aux_loss_coef * load_balancing_loss(logits, self.num_experts,
@@ -266,6 +279,7 @@ class Qwen3Moe(nn.Module):
                 b.ffn.last_router_logits = None
                 b.ffn.last_top_idx = None
         self._router_logits = []
+        self._token_mask = None if attention_mask is None else attention_mask.bool().reshape(-1)
         B, S = x.shape
         fused = (x.is_cuda and attention_mask is None and not return_hidden_states
                  and position_ids is None and getattr(self, "tp", None) is None

@@ -1,0 +1,170 @@
+"""The post-training objectives on models, and the MoE model's fused router losses."""
+
+import importlib.util
+import os
+
+import pytest
+import torch
+
+from pluggy_b200.models.builder import build_model
+from pluggy_b200.objectives.builder import build_objective
+
+GPU = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=GPU)]
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+IGN = -100
+
+
+def small(name="qwen3_dense", dev="cpu", **kw):
+    cfg = dict(num_layers=2, num_heads=2, num_kv_heads=1, emb_dim=128, head_dim=64, vocab_size=200)
+    cfg.update({"qwen3_moe": dict(moe_ffn_dim=128, num_experts=32, top_k=4, router_init_std=0.02),
+                "gemma4": dict(ffn_dim=128, global_head_dim=64, sliding_window=16,
+                               final_logit_softcapping=3.0)}.get(name, dict(ffn_dim=256)))
+    cfg.update(kw)
+    torch.manual_seed(0)
+    m = build_model(name, cfg)
+    m.init_weights(0.2) if name == "gemma4" else m.init_weights()
+    return m.to(dev)
+
+
+def pairs(dev, P=3, S=128, V=200):
+    g = torch.Generator().manual_seed(1)
+    out = {}
+    for side in ("chosen", "rejected"):
+        ids = torch.randint(0, V, (P, S), generator=g)
+        labels = ids.clone()
+        labels[:, :4] = IGN
+        labels[1, 70:] = IGN
+        out[f"{side}_ids"], out[f"{side}_labels"] = ids.to(dev), labels.to(dev)
+    return out
+
+
+def logits_logps(model, ids, labels):
+    """[B, S] log-probabilities from the model's full logits, shifted like the objectives'."""
+    lp = torch.log_softmax(model(ids).float(), -1)
+    y = torch.cat((labels[:, 1:], torch.full_like(labels[:, :1], IGN)), 1)
+    return torch.where(y == IGN, 0.0, lp.gather(2, y.clamp_min(0)[..., None])[..., 0])
+
+
+@pytest.mark.parametrize("name", ["qwen3_dense", "gemma4", "qwen3_moe"])
+def test_scores_are_the_models_log_probabilities(name):
+    """On CPU in fp32: the same numbers as from the logits, the logit softcap included."""
+    m = small(name)
+    b = pairs("cpu")
+    got = build_objective("PREFERENCE", {}).score(m, b)
+    assert not got.requires_grad
+    with torch.no_grad():
+        for i, side in enumerate(("chosen", "rejected")):
+            want = logits_logps(m, b[f"{side}_ids"], b[f"{side}_labels"])
+            assert torch.allclose(got[i], want, atol=1e-5, rtol=1e-5)
+
+
+@GPU
+def test_scores_on_the_gpu_match_the_cpu():
+    """bf16 forward and head against fp32: log-probabilities of about -5 to 2^-6 of that."""
+    b = pairs("cpu")
+    cpu = build_objective("PREFERENCE", {}).score(small(), b)
+    gpu = build_objective("PREFERENCE", {}).score(small(dev="cuda"), {k: v.cuda() for k, v in b.items()})
+    assert ((gpu.cpu() - cpu).abs() <= 0.08).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_preference_objective_at_the_reference(dev):
+    """Policy = reference: loss log 2, no rewards, and a gradient that favours the chosen."""
+    m = small(dev=dev)
+    obj = build_objective("PREFERENCE", dict(beta=0.5))
+    b = pairs(dev)
+    b["ref_logps"] = obj.score(m, b)
+    loss = obj.compute_loss(m, b)
+    assert abs(loss.item() - 0.6931472) < 1e-5
+    assert obj.metrics["chosen_reward"] == 0 and obj.metrics["rejected_reward"] == 0
+    loss.backward()
+    with torch.no_grad():
+        for p in m.parameters():
+            if p.grad is not None:
+                p -= 0.05 * p.grad
+        assert obj.compute_loss(m, b) < loss
+        assert obj.metrics["chosen_reward"] > obj.metrics["rejected_reward"]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_policy_objective_first_update(dev):
+    """Without old log-probabilities the gradient is that of -sum A log p / n."""
+    m = small(dev=dev)
+    obj = build_objective("POLICY", {})
+    b = pairs(dev)
+    batch = {"input_ids": b["chosen_ids"], "labels": b["chosen_labels"],
+             "advantages": torch.tensor([1.0, -2.0, 0.5], device=dev)}
+    loss = obj.compute_loss(m, batch)
+    (g,) = torch.autograd.grad(loss, m.lm_head.weight)
+    from pluggy_b200.objectives.post_training import token_logprobs
+
+    lp, mask = token_logprobs(m, batch["input_ids"], batch["labels"])
+    want = -(lp * batch["advantages"][:, None] * mask).sum() / mask.sum()
+    (gw,) = torch.autograd.grad(want, m.lm_head.weight)
+    assert (g - gw).norm() <= 2.0 ** -7 * gw.norm()
+    assert obj.metrics["clipped"] == 0
+
+
+def test_objectives_refuse_what_they_cannot_use():
+    m = small()
+    b = pairs("cpu")
+    pref, pol = build_objective("PREFERENCE", {}), build_objective("POLICY", dict(kl_coef=0.1))
+    with pytest.raises(ValueError, match="ref_logps"):
+        pref.compute_loss(m, b)
+    with pytest.raises(ValueError, match="chosen_ids"):
+        build_objective("PREFERENCE", dict(reference_free=True)).compute_loss(m, {"input_ids": b["chosen_ids"]})
+    with pytest.raises(ValueError, match="advantages"):
+        pol.compute_loss(m, {"input_ids": b["chosen_ids"], "labels": b["chosen_labels"]})
+    build_objective("PREFERENCE", dict(reference_free=True)).compute_loss(m, b)
+
+    class Split:
+        dim = "tp"
+
+        class mesh:
+            size = staticmethod(lambda dim: 2)
+
+    m.tp = Split()
+    with pytest.raises(NotImplementedError, match="tp"):
+        build_objective("PREFERENCE", dict(reference_free=True)).compute_loss(m, b)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("padded", [False, True])
+def test_fused_router_losses_match_the_default(dev, padded):
+    """Same loss, gradients and counts; with a padding mask, those of the tokens that count."""
+    ids = torch.randint(0, 200, (2, 128), generator=torch.Generator().manual_seed(3)).to(dev)
+    mask = None
+    if padded:
+        mask = torch.ones(2, 128, dtype=torch.long, device=dev)
+        mask[0, 100:] = 0
+    got = []
+    for fused in (False, True):
+        m = small("qwen3_moe", dev, fused_router_losses=fused, router_aux_loss_coef=0.1)
+        m(ids, attention_mask=mask)
+        aux = m.aux_loss()
+        if padded and not fused:  # the default counts padded tokens: restate it without them
+            from pluggy_b200.models.qwen3_moe import load_balancing_loss, router_z_loss
+
+            keep = mask.bool().reshape(-1)
+            logits = [x[keep] for x in m._router_logits]
+            aux = 0.1 * load_balancing_loss(logits, 32, 4) + 0.001 * router_z_loss(logits)
+        grads = torch.autograd.grad(aux, [b.ffn.router.weight for b in m.blocks])
+        got.append((aux.detach(), grads, m.last_tokens_per_expert))
+    (a, ga, ca), (b, gb, cb) = got
+    assert abs(a - b) <= 2.0 ** -16 * a
+    for x, y in zip(ga, gb):
+        # on the GPU the routers' logits, and so their gradients, are bf16
+        assert (x - y).norm() <= (2.0 ** -7 if dev == "cuda" else 1e-4) * x.norm()
+    if not padded:
+        assert torch.equal(ca, cb)
+    assert cb.sum() == (228 if padded else 256) * 4 * 2
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_example_runs(dev):
+    spec = importlib.util.spec_from_file_location("post_training_example",
+                                                  os.path.join(ROOT, "examples", "post_training.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    assert ex.main(["--device", dev, "--steps", "3"]) == 0
