@@ -577,6 +577,12 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
       plg::gemm_bf16(b, st);
     }
   }
+  if (need_w && kept.has_value()) {
+    // labels as int32 (half the sort's passes); those outside the vocabulary are left out anyway
+    const auto order = at::sort(labels.clamp(-1, V).to(at::kInt), /*stable=*/true, 0, /*descending=*/false);
+    plg::head_label_rows(p, std::get<0>(order).data_ptr<int>(), std::get<1>(order).data_ptr<int64_t>(), ip + T,
+                         factor.data_ptr<float>(), dw.data_ptr(), dw_f32, static_cast<int>(T), st);
+  }
   if (need_h) {
     dh = at::empty({T, D}, dh_f32 ? f32 : h.options());
     plg::head_scatter(p, dh_rows.data_ptr<float>(), R * D, count + 2,

@@ -14,12 +14,13 @@
 // 8 T V D operations in all. Large problems need 6: dh = diag(c) X W and dW = X^T diag(c) h
 // hold for any X whose rows are G's up to factors c_t, so the forward pass already stores
 //   X[t, v] = bf16(2^(z log2e - r_t) * softcap'(a)),   r_t = z[t, y_t] log2e + 40
-// with a reference r_t that one dot product gives beforehand, and the backward pass writes
-// the label's entry and folds c_t = -(g_t / temperature) 2^(r_t - lse2_t) into the hidden rows
-// (for dW) and into the result (for dh). Since lse2 >= z_y log2e, the entries that matter
+// with a reference r_t that one dot product gives beforehand, and the backward pass folds
+// c_t = -(g_t / temperature) 2^(r_t - lse2_t) into the hidden rows (for dW) and into the result
+// (for dh). The labels' entries, most of a gradient's norm, are left out of X and added in
+// fp32: one weight row to each row of dh, one hidden row for each token to dW. Since lse2 >= z_y log2e, the entries that matter
 // lie above 2^-100 and below 2^(-out log2e - 40): bf16's range holds them unless out < -97 or
 // so. If any row is beyond that, a flag in device memory makes the backward pass recompute.
-// What it costs: c_t h_t is rounded to bf16 once more (2^-8 of a term of dW).
+// What it costs: c_t h_t is rounded to bf16 (2^-8 of a term of dW other than the labels').
 //
 // Rows whose label is ignore_index are left out of the products: compact_kernel lists
 // the others on the device, gather_kernel packs their hidden rows, and every later kernel reads
@@ -903,9 +904,9 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ pa
   }
 }
 
-// Completes a kept X. Per row: c_t, the bf16 row c_t h_t, the label's entry of X (rounded to
-// bf16) and, for dh, what that rounding left out. Under the flag X has been recomputed as the
-// gradient rows themselves: c_t = 1.
+// Completes a kept X. Per row: c_t, the bf16 row c_t h_t, and the label's own factor, whose
+// entry of X becomes 0. Under the flag X has been recomputed as the gradient rows themselves,
+// labels included: the factors are 1 and 0.
 __global__ void __launch_bounds__(128) scale_rows_kernel(const __nv_bfloat16* __restrict__ h, int D,
                                                          const int* __restrict__ row_map,
                                                          const int* __restrict__ count,
@@ -932,9 +933,8 @@ __global__ void __launch_bounds__(128) scale_rows_kernel(const __nv_bfloat16* __
       const float gap = lse2[r] - ref[r], g = gout[tok] * inv_temp;
       c = -g * exp2f(-gap);
       if (threadIdx.x == 0) {
-        const __nv_bfloat16 entry = __float2bfloat16(-label_grad[r] * exp2f(gap));
-        X[r * ldx + labels[tok]] = entry;
-        factor[r] = make_float2(c, g * label_grad[r] - c * __bfloat162float(entry));
+        X[r * ldx + labels[tok]] = __float2bfloat16(0.f);
+        factor[r] = make_float2(c, g * label_grad[r]);
       }
     } else if (threadIdx.x == 0) {
       factor[r] = make_float2(1.f, 0.f);
@@ -954,7 +954,8 @@ __global__ void __launch_bounds__(128) scale_rows_kernel(const __nv_bfloat16* __
 }
 
 // dh[token] in dh's type from the compact fp32 rows (the sum of the product's k splits, in
-// their order), zeros for the tokens left out; with a kept X, c_t times the row plus the left-out part of the label's entry times its weight row
+// their order), zeros for the tokens left out; with a kept X, c_t times the row plus the
+// label's factor times its weight row
 template <typename T>
 __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ src, long long split_stride,
                                                       const int* __restrict__ splits,
@@ -990,6 +991,62 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ 
         reinterpret_cast<uint2*>(dh + t * D)[i] = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
       else
         reinterpret_cast<float4*>(dh + t * D)[i] = v;
+    }
+  }
+}
+
+// The labels' part of dW with a kept X: dW[v] += sum of the label factors times the hidden
+// rows of the tokens with label v. Tokens come sorted by label (stable); the block at a run's
+// first token (and, in y, at 512 columns) adds up the run in token order: no atomics. A run's
+// rows and factors are listed 128 at a time, so that the row loads do not wait for them.
+template <typename T>
+__global__ void __launch_bounds__(128) label_rows_kernel(const int* __restrict__ sorted,
+                                                         const int64_t* __restrict__ token,
+                                                         const int* __restrict__ inverse,
+                                                         const float2* __restrict__ factor,
+                                                         const __nv_bfloat16* __restrict__ h, int D,
+                                                         T* __restrict__ dw, int tokens) {
+  __shared__ int s_row[128];
+  __shared__ float s_f[128];
+  const int c = blockIdx.y * 128 + threadIdx.x;  // this thread's four columns
+  for (int i = blockIdx.x; i < tokens; i += gridDim.x) {
+    const int v = sorted[i];
+    // a label left out (ignored or outside the vocabulary) is left out for all its tokens
+    if ((i > 0 && sorted[i - 1] == v) || inverse[token[i]] < 0) continue;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = i;; j0 += 128) {
+      const int j = j0 + threadIdx.x;
+      const bool mine = j < tokens && sorted[j] == v;
+      if (mine) {
+        const int r = inverse[token[j]];
+        s_row[threadIdx.x] = r;
+        s_f[threadIdx.x] = factor[r].y;
+      }
+      const int n = __syncthreads_count(mine);  // the run is contiguous: the first n
+      if (c * 4 < D) {
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) {
+          const float f = s_f[k];
+          const uint2 u = reinterpret_cast<const uint2*>(h + static_cast<long long>(s_row[k]) * D)[c];
+          const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
+          s.x = fmaf(f, a.x, s.x);
+          s.y = fmaf(f, a.y, s.y);
+          s.z = fmaf(f, b.x, s.z);
+          s.w = fmaf(f, b.y, s.w);
+        }
+      }
+      __syncthreads();
+      if (n < 128) break;
+    }
+    if (c * 4 >= D) continue;
+    if (sizeof(T) == 2) {
+      uint2* p = reinterpret_cast<uint2*>(dw + static_cast<long long>(v) * D) + c;
+      const float2 a = unpack_bf16x2(p->x), b = unpack_bf16x2(p->y);
+      *p = make_uint2(pack_bf16x2(a.x + s.x, a.y + s.y), pack_bf16x2(b.x + s.z, b.y + s.w));
+    } else {
+      float4* p = reinterpret_cast<float4*>(dw + static_cast<long long>(v) * D) + c;
+      const float4 o = *p;
+      *p = make_float4(o.x + s.x, o.y + s.y, o.z + s.z, o.w + s.w);
     }
   }
 }
@@ -1255,6 +1312,21 @@ void head_gather(const HeadProblem& p, const void* h, bool fp32, long long ldh, 
     gather_kernel<__nv_bfloat16><<<blocks, 128, 0, st>>>(static_cast<const __nv_bfloat16*>(h), ldh, D, p.row_map,
                                                          p.n_rows, static_cast<__nv_bfloat16*>(out), cap_rows, w,
                                                          p.ldw, p.labels, k, p.softcap, ref);
+  PLG_CUDA_CHECK(cudaGetLastError());
+}
+
+void head_label_rows(const HeadProblem& p, const int* sorted, const int64_t* token, const int* inverse,
+                     const float* factor, void* dw, bool fp32, int tokens, cudaStream_t st) {
+  if (tokens <= 0) return;
+  const dim3 grid(std::min(tokens, 148 * 16), (p.D + 511) / 512);
+  const float2* f = reinterpret_cast<const float2*>(factor);
+  const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(p.h);
+  if (fp32)
+    label_rows_kernel<float><<<grid, 128, 0, st>>>(sorted, token, inverse, f, h, p.D, static_cast<float*>(dw),
+                                                   tokens);
+  else
+    label_rows_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(sorted, token, inverse, f, h, p.D,
+                                                           static_cast<__nv_bfloat16*>(dw), tokens);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 

@@ -187,10 +187,14 @@ void head_join(const HeadProblem& p, const void* part, const float* target, long
 // X = the gradient rows themselves; nothing happens unless *only_if (when given)
 void head_recompute(const HeadProblem& p, const float* lse2, const float* label_grad, const float* gout,
                     const int* only_if, void* X, long long ldx, cudaStream_t stream);
-// Completes a kept X: the labels' entries, hs [rows, D] = bf16(c h) (zero rows up to the
-// tile's end) and factor [rows][2] = c and the part of the label's entry that X lacks
+// Completes a kept X: 0 at the labels, hs [rows, D] = bf16(c h) (zero rows up to the tile's
+// end) and factor [rows][2] = c and the label's own factor
 void head_scale_rows(const HeadProblem& p, const float* lse2, const float* label_grad, const float* ref,
                      const float* gout, void* X, long long ldx, float* factor, void* hs, cudaStream_t stream);
+// dw[label] += label factor * hidden row; sorted [tokens] labels and their tokens, inverse as
+// head_compact gives it, p.h the packed rows (contiguous)
+void head_label_rows(const HeadProblem& p, const int* sorted, const int64_t* token, const int* inverse,
+                     const float* factor, void* dw, bool fp32, int tokens, cudaStream_t stream);
 // row_map [T], inverse [T] (token -> row or -1), count [3] = {rows, 0, 1}, and out = 0 / NaN of
 // the tokens left out
 void head_compact(const int64_t* labels, long long T, long long V, long long ignore_index, int* row_map,
@@ -199,8 +203,8 @@ void head_compact(const int64_t* labels, long long T, long long V, long long ign
 // ref [rows] (optional): the reference of X
 void head_gather(const HeadProblem& p, const void* h, bool fp32, long long ldh, void* out, int cap_rows,
                  float* ref, cudaStream_t stream);
-// dh[token] = src row, summed over *splits parts (with factor: times c, plus the missing part times the label's weight
-// row), 0 for the tokens left out
+// dh[token] = src row, summed over *splits parts (with factor: times c, plus the label's factor times its
+// weight row), 0 for the tokens left out
 void head_scatter(const HeadProblem& p, const float* src, long long split_stride, const int* splits,
                   const float* factor, const int* inverse, void* dh, bool fp32, long long tokens,
                   cudaStream_t stream);

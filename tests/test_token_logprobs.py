@@ -364,3 +364,28 @@ def test_refusals_on_the_gpu(status):
                                torch.zeros(9, 16, device="cuda"), y[:0])
     assert lp.shape == (0,)
     lp.sum().backward()
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_kernel_kept_repeated_labels(dtype, kept, status):
+    """Long runs of one label (more than one block lists at a time), an ignore_index that is a
+    vocabulary entry, and labels outside the vocabulary."""
+    h, w, y, g = make(700, 648, 300, "cuda", ignored=0.0)
+    y[100:500] = 7
+    y[3:40] = 299
+    y[600:650] = 11
+    for ign in (-100, 11):
+        z = torch.where(y == 11, IGN, y) if ign == 11 else y
+        hr, wr = h.to(dtype).requires_grad_(True), w.to(dtype).requires_grad_(True)
+        lp = linear_token_logprobs(hr, wr, y, ign)
+        dh, dw = torch.autograd.grad(lp, (hr, wr), g)
+        ref, rdh, rdw, bdh, bdw, bound = exact(h, w, z, g)
+        assert ((lp - ref).abs() <= 2.0 ** -22 * 648 ** 0.5 * bound + 2.0 ** -20 * ref.abs()).all()
+        assert ((dh - rdh).abs() <= 2.0 ** -7 * bdh + 1e-6).all()
+        assert ((dw - rdw).abs() <= KEPT_DW * 2.0 ** -7 * bdw + 1e-6).all()
+    y2 = y.clone()
+    y2[5], y2[6] = 1 << 40, -5
+    lp = linear_token_logprobs(h.requires_grad_(True), w.requires_grad_(True), y2)
+    dh, dw = torch.autograd.grad(lp, (h, w), g)
+    assert torch.isnan(lp[5:7]).all() and torch.isfinite(dh).all() and torch.isfinite(dw).all()
