@@ -63,30 +63,6 @@ def _round_up(n: int, m: int) -> int:
     return (n + m - 1) // m * m
 
 
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, labels, ignore_index, w, softcap, temperature, workspace):
-        T, D = hidden.shape
-        V = w.shape[0]
-        keep = 2 * _round_up(T, 256) * V <= workspace and T * V * D >= KEEP_PRODUCT
-        out, *saved = ext().token_logprobs_fwd(hidden, w, labels, ignore_index, softcap, temperature,
-                                               True, True, keep, status_word(hidden.device))
-        ctx.save_for_backward(w, labels, *saved)
-        ctx.cfg = (softcap, temperature, workspace, hidden.dtype, weight.dtype)
-        return out
-
-    @staticmethod
-    def backward(ctx, gout):
-        w, labels, h, ints, stats, kept = ctx.saved_tensors
-        softcap, temperature, workspace, h_dtype, w_dtype = ctx.cfg
-        need_h, need_w = ctx.needs_input_grad[:2]
-        dh, dw = ext().token_logprobs_bwd(h, w, labels, ints, stats, kept, gout.contiguous(), softcap,
-                                          temperature, workspace, SPLIT_WORKSPACE,
-                                          h_dtype == torch.float32, w_dtype == torch.float32, need_h,
-                                          need_w, status_word(h.device))
-        return (dh, dw) + (None,) * 6
-
-
 def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                           ignore_index: int = -100, *, weight_lowp: torch.Tensor | None = None,
                           softcap: float | None = None, temperature: float = 1.0,
@@ -132,12 +108,10 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: to
     w = weight_lowp if weight_lowp is not None else weight.detach().to(torch.bfloat16)
     h = hidden.reshape(-1, D)
     h, w = _rows_aligned(h), _rows_aligned(w)
-    y = labels.reshape(-1).contiguous()
-    cap, tau = float(softcap or 0.0), float(temperature)
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        out = _TokenLogprobs.apply(h, weight, y, int(ignore_index), w, cap, tau,
-                                   WORKSPACE if workspace_bytes is None else int(workspace_bytes))
-    else:
-        (out,) = ext().token_logprobs_fwd(h.detach(), w, y, int(ignore_index), cap, tau,
-                                          h.shape[0] > UNPACKED_ROWS, False, False, status_word(h.device))
+    T, V = h.shape[0], w.shape[0]
+    workspace = WORKSPACE if workspace_bytes is None else int(workspace_bytes)
+    keep = 2 * _round_up(T, 256) * V <= workspace and T * V * D >= KEEP_PRODUCT
+    out = ext().token_logprobs(h, weight, w, labels.reshape(-1).contiguous(), int(ignore_index),
+                               float(softcap or 0.0), float(temperature), T > UNPACKED_ROWS, keep,
+                               workspace, SPLIT_WORKSPACE, status_word(h.device))
     return out.view(labels.shape)

@@ -101,27 +101,6 @@ def router_balance_loss_reference(router_logits, top_indices, balance_coef=1.0, 
     return loss, counts
 
 
-class _RouterBalanceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, idx, mask, balance_coef, z_coef, *logits):
-        from pluggy_b200.ops._ext import ext
-
-        loss, counts, lse, slope = ext().router_balance_fwd(logits, idx, mask, balance_coef, z_coef)
-        ctx.save_for_backward(lse, slope, mask, *logits)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(counts)
-        return loss, counts
-
-    @staticmethod
-    def backward(ctx, gout, _):
-        from pluggy_b200.ops._ext import ext
-
-        lse, slope, mask, *logits = ctx.saved_tensors
-        if gout is None:
-            return (None,) * (4 + len(logits))
-        return (None, None, None, None, *ext().router_balance_bwd(logits, mask, lse, slope, gout))
-
-
 def router_balance_loss(router_logits, top_indices, *, balance_coef: float = 1.0, z_coef: float = 0.0,
                         mask: torch.Tensor | None = None):
     """Balance and z loss of one or several MoE routers, and the tokens sent to each expert.
@@ -152,7 +131,9 @@ def router_balance_loss(router_logits, top_indices, *, balance_coef: float = 1.0
     if x0.dim() != 2 or x0.shape[1] == 0:
         raise ValueError(f"router_balance_loss: logits must be [T, E] with E > 0, got {tuple(x0.shape)}")
     if x0.is_cuda:  # the extension checks every layer
-        return _RouterBalanceLoss.apply(idx, mask, float(balance_coef), float(z_coef), *logits)
+        from pluggy_b200.ops._ext import ext
+
+        return tuple(ext().router_balance_loss(logits, idx, mask, float(balance_coef), float(z_coef)))
     for x, i in zip(logits, idx):
         if x.shape != x0.shape or x.dtype != x0.dtype or x.device != x0.device:
             raise ValueError("router_balance_loss: the routers' logits must be [T, E], alike")

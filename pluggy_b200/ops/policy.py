@@ -70,29 +70,6 @@ def policy_loss_reference(logps, old_logps, advantages, mask, ref_logps=None, cl
             ((up | dn) & mask).sum() / tokens)
 
 
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logps, old_logps, advantages, mask, ref_logps, clip_low, clip_high, kl_coef,
-                by_sequence):
-        loss, kl, clipped, ctx.grad = ext().policy_fwd(logps, old_logps, advantages, mask, ref_logps,
-                                                       clip_low, clip_high, kl_coef, by_sequence, True)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(kl, clipped)
-        return loss, kl, clipped
-
-    @staticmethod
-    def backward(ctx, gout, *_):
-        if gout is None:
-            return (None,) * 9
-        grad = ctx.grad
-        if grad is None:
-            raise RuntimeError("policy_loss: backward called twice; the stored gradient is handed out "
-                               "by the first call, so retain_graph does not work through this op")
-        ctx.grad = None
-        ext().scale_unless_one(grad, gout)
-        return (grad,) + (None,) * 8
-
-
 def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages: torch.Tensor,
                 mask: torch.Tensor, *, ref_logps: torch.Tensor | None = None, clip_low: float = 0.2,
                 clip_high: float = 0.2, kl_coef: float = 0.0, reduction: str = "token"):
@@ -120,8 +97,6 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
                      advantages=(advantages, fp32))
         return policy_loss_reference(logps, old_logps, advantages, mask, ref_logps, clip_low, clip_high,
                                      kl_coef, reduction)
-    args = (logps, old_logps, advantages, tokens_contiguous(mask), ref_logps, float(clip_low),
-            float(clip_high), float(kl_coef), reduction == "sequence")
-    if torch.is_grad_enabled() and logps.requires_grad:
-        return _PolicyLoss.apply(*args)
-    return tuple(ext().policy_fwd(*args, False))
+    return tuple(ext().policy_loss(logps, old_logps, advantages, tokens_contiguous(mask), ref_logps,
+                                   float(clip_low), float(clip_high), float(kl_coef),
+                                   reduction == "sequence"))

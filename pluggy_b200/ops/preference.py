@@ -46,23 +46,6 @@ def preference_loss_reference(logps, ref_logps, mask, beta=0.1, kind="sigmoid", 
     return loss, (beta * s[0]).detach(), (beta * s[1]).detach()
 
 
-class _PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logps, ref_logps, mask, beta, kind, label_smoothing, length_normalized):
-        loss, chosen, rejected, row_scale = ext().preference_fwd(
-            logps, ref_logps, mask, KINDS[kind], beta, label_smoothing, length_normalized)
-        ctx.save_for_backward(mask, row_scale)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(chosen, rejected)
-        return loss, chosen, rejected
-
-    @staticmethod
-    def backward(ctx, gout, *_):
-        mask, row_scale = ctx.saved_tensors
-        grad = None if gout is None else ext().preference_bwd(mask, row_scale, gout)
-        return (grad,) + (None,) * 6
-
-
 def check_tokens(op: str, mask: torch.Tensor, **tensors) -> None:
     """Shapes, devices and types of (tensor or None, allowed types) against the mask's, for CPU
     tensors; the CUDA entry points check the same."""
@@ -112,5 +95,5 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
                      ref_logps=(ref_logps, (torch.float32, torch.bfloat16)))
         return preference_loss_reference(logps, ref_logps, mask, beta, kind, label_smoothing,
                                          length_normalized)
-    return _PreferenceLoss.apply(logps, ref_logps, tokens_contiguous(mask), float(beta), kind,
-                                 float(label_smoothing), bool(length_normalized))
+    return tuple(ext().preference_loss(logps, ref_logps, tokens_contiguous(mask), KINDS[kind], float(beta),
+                                       float(label_smoothing), bool(length_normalized)))
