@@ -464,7 +464,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // are swapped: 128 vocabulary entries are the tensor core's rows and the NT (32, 64 or 128)
 // hidden rows its columns, so that an MMA costs in proportion to the rows in use. CTA c takes
 // the entries [V c / CTAs, V (c + 1) / CTAs), equal shares of the bytes for every SM, in
-// equal tiles of at most 128 entries (256-column tiles leave 11 waves of 8 for 594 tiles).
+// equal tiles of at most 128 entries (the other kernel's 594 tiles of 256 columns are 9 waves
+// over 74 SM pairs for 8.03 waves of work).
 // Accumulator lane = entry, column = hidden row: a warp reduces 32 entries x 32 rows by
 // exchanging halves (31 shuffles instead of 160), which leaves lane j with row j's result,
 // and keeps each row's running (reference, sum) there. One pair per row, CTA and quadrant.

@@ -302,8 +302,10 @@ __device__ __forceinline__ void kl_terms(float d, float& em1, float& k3) {
 //   loss = -A e^r (the bound instead of e^r once A pushes r past it) + kl_coef (e^d - 1 - d)
 //   grad = -A e^r (0 past the bound) - kl_coef (e^d - 1)
 // each times the token's weight in the mean, known from the counts.
-template <int VEC>
-__global__ void __launch_bounds__(256, 3) policy_kernel(const PolicyArgs a, const int* __restrict__ counts,
+// OLD, REF, ADV: old log-probabilities, reference and per-token advantages are given
+constexpr int kPolicyResident = 3;
+template <int VEC, bool OLD, bool REF, bool ADV>
+__global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const PolicyArgs a, const int* __restrict__ counts,
                                                      const longlong2* __restrict__ block_counts, int nblocks,
                                                      double* __restrict__ block_sums,
                                                      unsigned* __restrict__ ticket, float* __restrict__ grad,
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(256, 3) policy_kernel(const PolicyArgs a, cons
     const int t1 = min(a.S, t0 + len);
     const float* __restrict__ lp = a.logps + r * a.lp_row;
     const uint8_t* __restrict__ mk = a.mask + r * a.mk_row;
-    const float row_adv = a.adv_tok == 0 ? a.adv[r * a.adv_row] : 0.f;
+    const float row_adv = ADV ? 0.f : a.adv[r * a.adv_row];
     const float w = static_cast<float>(a.by_sequence ? inv_rows / max(counts[r], 1) : inv_tokens);
     float* __restrict__ gp = grad + r * a.S;
     float sl = 0.f, sk = 0.f;
@@ -356,9 +358,9 @@ __global__ void __launch_bounds__(256, 3) policy_kernel(const PolicyArgs a, cons
     auto fetch = [&](int t) {
       load_f<VEC>(lp + t, x);
       load_mask<VEC>(mk + t, m);
-      if (a.old != nullptr) load_any<VEC>(a.old, a.old_bf16, r * a.old_row + t, o);
-      if (a.ref != nullptr) load_any<VEC>(a.ref, a.ref_bf16, r * a.ref_row + t, f);
-      if (a.adv_tok != 0) load_f<VEC>(a.adv + r * a.adv_row + t, A);
+      if (OLD) load_any<VEC>(a.old, a.old_bf16, r * a.old_row + t, o);
+      if (REF) load_any<VEC>(a.ref, a.ref_bf16, r * a.ref_row + t, f);
+      if (ADV) load_f<VEC>(a.adv + r * a.adv_row + t, A);
     };
     int t = t0 + lane * VEC;
     if (t < t1) fetch(t);
@@ -368,20 +370,20 @@ __global__ void __launch_bounds__(256, 3) policy_kernel(const PolicyArgs a, cons
       bool mm[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        lr[j] = a.old != nullptr ? x[j] - o[j] : 0.f;
-        df[j] = a.ref != nullptr ? f[j] - x[j] : 0.f;
-        adv[j] = a.adv_tok != 0 ? A[j] : row_adv;
+        lr[j] = OLD ? x[j] - o[j] : 0.f;
+        df[j] = REF ? f[j] - x[j] : 0.f;
+        adv[j] = ADV ? A[j] : row_adv;
         mm[j] = m[j];
       }
       if (t + 32 * VEC < t1) fetch(t + 32 * VEC);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float ratio = a.old != nullptr ? expf(lr[j]) : 1.f;
+        const float ratio = OLD ? expf(lr[j]) : 1.f;
         const bool up = adv[j] > 0.f && lr[j] > a.log_hi, dn = adv[j] < 0.f && lr[j] < a.log_lo;
         const bool clip = up || dn;
         float l = -(up ? a.hi : dn ? a.lo : ratio) * adv[j];
         float d = clip ? 0.f : -adv[j] * ratio;
-        if (a.ref != nullptr) {
+        if (REF) {
           float em1, k3;
           kl_terms(df[j], em1, k3);
           sk += mm[j] ? k3 : 0.f;
@@ -916,7 +918,10 @@ int policy_count_blocks(int R, int S) {
   return static_cast<int>(std::max<long long>(1, std::min<long long>(b, 148 * 4)));
 }
 
-int policy_blocks(int R, int S) { return warp_grid(static_cast<long long>(R) * chunks_of(R, S)); }
+// as many blocks as stay resident (registers allow 3 an SM): each warp takes several units
+int policy_blocks(int R, int S) {
+  return std::min(warp_grid(static_cast<long long>(R) * chunks_of(R, S)), 148 * kPolicyResident);
+}
 
 void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double* block_sums,
                     unsigned* ticket, float* grad, float* out, cudaStream_t st) {
@@ -932,8 +937,24 @@ void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double
                    (a.ref == nullptr || aligned4(a.ref, a.ref_bf16 ? 2 : 4, {a.ref_row})) &&
                    (a.adv_tok == 0 || aligned4(a.adv, 4, {a.adv_row})) && aligned4(grad, 4, {});
   const int grid = policy_blocks(a.R, a.S);
-  if (vec) policy_kernel<4><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket, grad, out, chunks, len);
-  else policy_kernel<1><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket, grad, out, chunks, len);
+  auto launch = [&](auto old, auto ref, auto adv) {
+    if (vec)
+      policy_kernel<4, old.value, ref.value, adv.value><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket,
+                                                                              grad, out, chunks, len);
+    else
+      policy_kernel<1, old.value, ref.value, adv.value><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket,
+                                                                              grad, out, chunks, len);
+  };
+  auto pick = [&](auto old, auto ref) {
+    if (a.adv_tok) launch(old, ref, std::true_type{});
+    else launch(old, ref, std::false_type{});
+  };
+  auto pick_ref = [&](auto old) {
+    if (a.ref != nullptr) pick(old, std::true_type{});
+    else pick(old, std::false_type{});
+  };
+  if (a.old != nullptr) pick_ref(std::true_type{});
+  else pick_ref(std::false_type{});
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 

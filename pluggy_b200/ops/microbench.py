@@ -336,6 +336,68 @@ def case_router(a, small):
     return fn, {"bytes": T * E * (2 + 4) + T * k * 12, "shape": {"T": T, "E": E, "k": k}}
 
 
+def case_token_logprobs(a, small):
+    """Log-probabilities of given tokens under a [V, D] head: ``--layout nt`` scores T tokens,
+    ``tn`` adds both gradients (6 T V D operations, whatever the kernels recompute)."""
+    from pluggy_b200.ops.logprob import linear_token_logprobs
+
+    T, D, V = (4096 if small else a.m), a.dim, (32768 if small else a.vocab)
+    h, w = _bf16(T, D), _bf16(V, D) * (2.0 / D ** 0.5)
+    y = torch.randint(0, V, (T,), device="cuda")
+    flops, shape = 2.0 * T * V * D, {"T": T, "D": D, "V": V}
+    if a.layout != "tn":
+        info = {"flops": flops, "shape": shape} if T > 128 else {"bytes": V * D * 2, "shape": shape}
+        return (lambda: linear_token_logprobs(h, w, y)), info
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    g = torch.randn(T, device="cuda")
+    fn = lambda: torch.autograd.grad(linear_token_logprobs(h, w, y), (h, w), g)  # noqa: E731
+    return fn, {"flops": 3 * flops, "shape": {**shape, "gradients": True}}
+
+
+def case_preference(a, small):
+    """Preference loss of P pairs of S tokens with its gradient (log-probabilities, reference and
+    mask read once, the gradient written)."""
+    from pluggy_b200.ops.preference import preference_loss
+
+    P, S = (128 if small else 512), a.seq
+    lp = -torch.rand(2, P, S, device="cuda")
+    ref, mask = lp - 0.1, torch.rand(2, P, S, device="cuda") < 0.8
+    lp.requires_grad_(True)
+    fn = lambda: torch.autograd.grad(preference_loss(lp, ref, mask)[0], lp)  # noqa: E731
+    return fn, {"bytes": 2 * P * S * 13, "shape": {"P": P, "S": S}}
+
+
+def case_policy(a, small):
+    """Clipped policy loss with a KL term over [R, S] tokens, with its gradient."""
+    from pluggy_b200.ops.policy import policy_loss
+
+    R, S = (512 if small else 2048), a.seq
+    lp = -torch.rand(R, S, device="cuda")
+    old, ref = (lp + s * torch.randn_like(lp) for s in (0.1, 0.2))
+    adv, mask = torch.randn_like(lp), torch.rand(R, S, device="cuda") < 0.8
+    lp.requires_grad_(True)
+
+    def fn():
+        return torch.autograd.grad(policy_loss(lp, old, adv, mask, ref_logps=ref, kl_coef=0.05)[0], lp)
+    return fn, {"bytes": R * S * 21, "shape": {"R": R, "S": S}}
+
+
+def case_router_balance(a, small):
+    """Balance and z loss of 24 routers with their gradients (logits read twice, written once)."""
+    from pluggy_b200.ops.moe import router_balance_loss
+
+    L, T, E, k = 24, (8192 if small else _tokens(a, small)), a.experts, a.topk
+    xs = [_bf16(T, E) for _ in range(L)]
+    idx = [torch.topk(x, k).indices for x in xs]
+    for x in xs:
+        x.requires_grad_(True)
+
+    def fn():
+        return torch.autograd.grad(router_balance_loss(xs, idx, balance_coef=1e-2, z_coef=1e-3)[0], xs)
+    return fn, {"bytes": L * T * (E * 2 * 3 + k * 8), "shape": {"L": L, "T": T, "E": E, "k": k}}
+
+
 CASES = {
     "gemm": case_gemm, "attn_fwd": case_attn_fwd, "attn_bwd": case_attn_bwd,
     "qk_rope_fwd": case_qk_rope_fwd, "qk_rope_bwd": case_qk_rope_bwd,
@@ -343,7 +405,8 @@ CASES = {
     "glu_fwd": case_glu_fwd, "glu_bwd": case_glu_bwd,
     "ce_rows": case_ce_rows, "adamw": case_adamw, "sumsq": case_sumsq, "embedding": case_embedding,
     "embedding_bwd": case_embedding_bwd, "grouped_gemm": case_grouped_gemm, "zero1": case_zero1,
-    "rope": case_rope, "router": case_router,
+    "rope": case_rope, "router": case_router, "token_logprobs": case_token_logprobs,
+    "preference": case_preference, "policy": case_policy, "router_balance": case_router_balance,
 }
 
 

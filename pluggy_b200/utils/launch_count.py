@@ -17,6 +17,8 @@ KERNELS_PER_CALL = {
     "glu_fwd": 1, "glu_bwd": 1, "cast_f32_bf16": 1, "embedding_fwd": 1, "embedding_bwd": 1,
     "softcap": 1, "ce_rows": 1, "multi_sumsq": 2, "multi_scale": 1, "adamw_multi": 1,
     "attn_fwd": 1, "attn_bwd": 4,
+    # forward kernels; the backward's are launched by the extension's own autograd functions
+    "token_logprobs": 4, "preference_loss": 2, "policy_loss": 2, "router_balance_loss": 2,
 }
 
 
