@@ -168,3 +168,51 @@ def test_example_runs(dev):
     ex = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(ex)
     assert ex.main(["--device", dev, "--steps", "3"]) == 0
+
+
+@GPU
+@pytest.mark.parametrize("keep", [False, True])
+def test_operators_replay_from_a_cuda_graph(keep, monkeypatch):
+    """Forward and backward captured once: a replay on new inputs, other rows ignored among them,
+    gives what eager calls give."""
+    from pluggy_b200.ops import linear_token_logprobs, logprob, policy_loss, preference_loss, router_balance_loss
+
+    monkeypatch.setattr(logprob, "KEEP_PRODUCT", 0 if keep else 1 << 62)
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def inputs():
+        y = torch.randint(0, 700, (8, 40), generator=g, device="cuda")
+        y[torch.rand(8, 40, generator=g, device="cuda") < 0.3] = IGN
+        return [torch.randn(8, 40, 64, generator=g, device="cuda").bfloat16(),
+                torch.randn(700, 64, generator=g, device="cuda").bfloat16() * 0.2, y,
+                torch.randn(8, generator=g, device="cuda"),
+                torch.randn(300, 64, generator=g, device="cuda").bfloat16()]
+
+    def step(h, w, y, adv, x):
+        h, w, x = (t.detach().requires_grad_(True) for t in (h, w, x))
+        lp = linear_token_logprobs(h, w, y)
+        mask = y != IGN
+        pol = policy_loss(lp, None, adv, mask, reduction="sequence")[0]
+        pref = preference_loss(lp.view(2, 4, 40), None, mask.view(2, 4, 40))[0]
+        idx = (torch.arange(600, device="cuda") % 64).view(300, 2)
+        bal, counts = router_balance_loss(x, idx, balance_coef=0.1, z_coef=0.1)
+        return [lp.detach(), pol.detach(), counts, *torch.autograd.grad(pol + 0.5 * pref + bal, (h, w, x))]
+
+    static = inputs()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for _ in range(2):
+        new = inputs()
+        for s, n in zip(static, new):
+            s.copy_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step(*new)):
+            assert torch.equal(a, b)
