@@ -612,6 +612,33 @@ inline CUresult encode_tensor_map(CUtensorMap* m, CUtensorMapDataType dtype, cuu
             swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
+// Launch a kernel that may start while its predecessor in the stream still runs (programmatic
+// dependent launch): its launch latency hides behind the predecessor, whose results it reads
+// only after dependency_wait(). The predecessor calls dependents_may_start().
+template <typename... P, typename... A>
+inline void launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PLG_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+__device__ __forceinline__ void dependents_may_start() {
+#if defined(__CUDA_ARCH__)
+  cudaTriggerProgrammaticLaunchCompletion();
+#endif
+}
+__device__ __forceinline__ void dependency_wait() {
+#if defined(__CUDA_ARCH__)
+  cudaGridDependencySynchronize();
+#endif
+}
+
 // Raise a kernel's dynamic shared memory limit once per (kernel, device): the
 // attribute belongs to the device context, so a process driving several GPUs
 // must set it on each.

@@ -529,6 +529,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
   uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(bar + 2 * C_::kStages + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_smem + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  dependents_may_start();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C_::kStages; ++s) {
@@ -850,6 +851,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ pa
                                                    float* __restrict__ lse2, float* __restrict__ label_grad,
                                                    int* __restrict__ flag) {
   __shared__ float2 s_part[8];
+  dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kRows = 8 / WARPS;  // rows of a block
   const int sub = WARPS == 1 ? lane : threadIdx.x;
@@ -1250,14 +1252,10 @@ void head_join(const HeadProblem& p, const void* part, const float* target, long
   const float2* pp = static_cast<const float2*>(part);
   const float k = kLog2e / p.temperature;
   // a warp per row fills the machine from about 148 * 8 rows on
-  if (p.rows >= 1024)
-    join_kernel<1><<<std::min((p.rows + 7) / 8, 148 * 8), 256, 0, st>>>(
-        pp, parts, p.rows, p.n_rows, p.row_map, p.labels, V, ignore_index, target, k, p.softcap, out, ref, lse2,
-        label_grad, flag);
-  else
-    join_kernel<8><<<p.rows, 256, 0, st>>>(pp, parts, p.rows, p.n_rows, p.row_map, p.labels, V, ignore_index,
-                                           target, k, p.softcap, out, ref, lse2, label_grad, flag);
-  PLG_CUDA_CHECK(cudaGetLastError());
+  const bool many = p.rows >= 1024;
+  launch_dependent(many ? join_kernel<1> : join_kernel<8>, many ? std::min((p.rows + 7) / 8, 148 * 8) : p.rows, 256,
+                   st, pp, parts, p.rows, p.n_rows, p.row_map, p.labels, V, ignore_index, target, k, p.softcap, out,
+                   ref, lse2, label_grad, flag);
 }
 
 void head_recompute(const HeadProblem& p, const float* lse2, const float* label_grad, const float* gout,

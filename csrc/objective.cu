@@ -69,6 +69,7 @@ __device__ __forceinline__ void load_mask(const uint8_t* p, bool (&m)[VEC]) {
 template <int VEC>
 __global__ void __launch_bounds__(256) pref_sums_kernel(const PrefArgs a, float2* __restrict__ part,
                                                         int chunks, int len, unsigned* __restrict__ ticket) {
+  dependents_may_start();
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
   const int lane = threadIdx.x & 31;
   const long long units = 2LL * a.P * chunks;
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(256) pref_pairs_kernel(const PrefArgs a, const
                                                          float* __restrict__ rewards) {
   __shared__ double s_loss[8];
   __shared__ bool s_last;
+  dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double acc = 0.0;
   for (long long i = blockIdx.x * 8LL + warp; i < a.P; i += gridDim.x * 8LL) {
@@ -227,6 +229,7 @@ __global__ void __launch_bounds__(256) policy_counts_kernel(const PolicyArgs a, 
   __shared__ int s_n[8];
   __shared__ long long s_tok[8];
   __shared__ int s_rows[8];
+  dependents_may_start();
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = BLOCK_ROW ? threadIdx.x : lane;
@@ -313,6 +316,7 @@ __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const Poli
   __shared__ long long s_cnt[2][8];
   __shared__ double s_sum[3][8];
   __shared__ bool s_last;
+  dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long tokens = 0, rows = 0;
   for (int b = threadIdx.x; b < nblocks; b += 256) {
@@ -559,6 +563,7 @@ __global__ void __launch_bounds__(kRouterThreads, kRouterSumsResident) router_su
                                                                      int* __restrict__ part_n,
                                                                      double* __restrict__ part_z,
                                                                      unsigned* __restrict__ ticket) {
+  dependents_may_start();
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
   constexpr int kEl = NV * VEC, kCover = G * kEl, kGroups = 32 / G, kWarps = kRouterThreads / 32;
   static_assert(kEl % 2 == 0, "values are processed in pairs");
@@ -612,17 +617,17 @@ __global__ void __launch_bounds__(kRouterThreads, kRouterSumsResident) router_su
     float s = 0.f, s1 = 0.f;
 #pragma unroll
     for (int e = 0; e < kEl; e += 2) {
-      x[e] = fast_exp2(fmaf(x[e], kLog2e, -off));
-      x[e + 1] = fast_exp2(fmaf(x[e + 1], kLog2e, -off));
-      s += x[e];
-      s1 += x[e + 1];
+      ffma2(x[e], x[e + 1], x[e], x[e + 1], kLog2e, kLog2e, -off, -off);
+      x[e] = fast_exp2(x[e]);
+      x[e + 1] = fast_exp2(x[e + 1]);
+      fadd2(s, s1, s, s1, x[e], x[e + 1]);
     }
     const float m = group_max<G>(ml), to_row = fast_exp2(ml - m);
     s = group_sum<G>((s + s1) * to_row);
     const float inv = __fdividef(to_row, s), lse = kLn2 * (m + log2f(s));
     if (kept_row) {
 #pragma unroll
-      for (int e = 0; e < kEl; ++e) acc[e] = fmaf(x[e], inv, acc[e]);
+      for (int e = 0; e < kEl; e += 2) ffma2(acc[e], acc[e + 1], x[e], x[e + 1], inv, inv, acc[e], acc[e + 1]);
       if (sub == 0) {
         zf = fmaf(lse, lse, zf);
         ++kept;
@@ -688,6 +693,7 @@ __global__ void __launch_bounds__(1024) router_join_kernel(const float* __restri
   __shared__ int s_n[32][33];
   __shared__ double s_tot[2];
   __shared__ bool s_last;
+  dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   double p = 0.0;
@@ -898,9 +904,8 @@ void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* t
   if (vec) pref_sums_kernel<4><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, len, ticket);
   else pref_sums_kernel<1><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, len, ticket);
   PLG_CUDA_CHECK(cudaGetLastError());
-  pref_pairs_kernel<<<pref_blocks(a.P), 256, 0, st>>>(a, static_cast<const float2*>(part), chunks, block_loss,
-                                                      ticket, row_scale, loss, rewards);
-  PLG_CUDA_CHECK(cudaGetLastError());
+  launch_dependent(pref_pairs_kernel, pref_blocks(a.P), 256, st, a, static_cast<const float2*>(part), chunks,
+                   block_loss, ticket, row_scale, loss, rewards);
 }
 
 void pref_backward(const PrefArgs& a, const float* row_scale, const float* gout, float* grad, cudaStream_t st) {
@@ -938,12 +943,9 @@ void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double
                    (a.adv_tok == 0 || aligned4(a.adv, 4, {a.adv_row})) && aligned4(grad, 4, {});
   const int grid = policy_blocks(a.R, a.S);
   auto launch = [&](auto old, auto ref, auto adv) {
-    if (vec)
-      policy_kernel<4, old.value, ref.value, adv.value><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket,
-                                                                              grad, out, chunks, len);
-    else
-      policy_kernel<1, old.value, ref.value, adv.value><<<grid, 256, 0, st>>>(a, counts, bc, cb, block_sums, ticket,
-                                                                              grad, out, chunks, len);
+    auto kern = vec ? policy_kernel<4, old.value, ref.value, adv.value>
+                    : policy_kernel<1, old.value, ref.value, adv.value>;
+    launch_dependent(kern, grid, 256, st, a, counts, bc, cb, block_sums, ticket, grad, out, chunks, len);
   };
   auto pick = [&](auto old, auto ref) {
     if (a.adv_tok) launch(old, ref, std::true_type{});
@@ -993,9 +995,8 @@ void router_balance_forward(const RouterArgs& a, bool bf16, float balance, float
     else run(static_cast<float*>(nullptr), router_vec<float>(a));
     PLG_CUDA_CHECK(cudaGetLastError());
   }
-  router_join_kernel<<<(a.E + 31) / 32, 1024, 0, st>>>(part_p, part_n, part_z, rows > 0 ? blocks : 0, a.E, balance,
-                                                       zcoef, dots, ticket, loss, counts, slope);
-  PLG_CUDA_CHECK(cudaGetLastError());
+  launch_dependent(router_join_kernel, (a.E + 31) / 32, 1024, st, part_p, part_n, part_z, rows > 0 ? blocks : 0, a.E,
+                   balance, zcoef, dots, ticket, loss, counts, slope);
 }
 
 void router_balance_backward(const RouterArgs& a, bool bf16, const float* lse, const float* slope,
