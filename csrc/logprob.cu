@@ -57,8 +57,11 @@ constexpr float kRefLimit = 100.f;   // lse2 - r_t beyond which X is recomputed
 // Reduction length of one accumulator of the statistics: the tensor cores truncate each
 // addition, a bias of about 1e-9 of the sum per column of D (measured: 2.5e-6 of a logit at
 // D = 2560, 1e-6 at 1024; an fp32 chain's rounding is about 5e-7), so longer sums are cut
-// into pieces that the epilogue adds in fp32. Pieces of 512 cost 17% of the time at D = 1024.
-constexpr int kSegBlocks = 1024 / kBK;
+// into pieces that the epilogue adds in fp32: of 1024 (512 cost 17% of the time at D = 1024;
+// 1280 save 2% at D = 2560). Where the head's bytes bound the call, thin_kernel, pieces of 512
+// are within 3% of those of 1024 (58.1 against 58.3 us for one row, D = 1024; relative error
+// 5.8e-8 instead of 8.0e-8 rms, 3.9e-8 for fp32 throughout) and 256 cost 10%.
+constexpr int kSegBlocks = 1024 / kBK, kThinSegBlocks = 512 / kBK;
 
 struct HeadArgs {
   int rows, N, k_blocks, segs;
@@ -1214,7 +1217,7 @@ static void head_thin(const HeadProblem& p, void* part, float* target, cudaStrea
   const int tiles = (share + kThinEntries - 1) / kThinEntries;
   a.tile = (share + tiles - 1) / tiles;
   a.k_blocks = (p.D + kBK - 1) / kBK;
-  a.segs = (a.k_blocks + kSegBlocks - 1) / kSegBlocks;
+  a.segs = (a.k_blocks + kThinSegBlocks - 1) / kThinSegBlocks;
   a.labels = p.labels;
   a.k = kLog2e / p.temperature;
   a.cap = p.softcap;
