@@ -834,6 +834,23 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = c10::optional<at::Tensor>;
 
+// The gradients below come from kernels without gradients of their own. Where a graph of the
+// backward pass is asked for, they pass through this node, so that differentiating them raises
+// instead of taking them for constants.
+struct FirstOrderFn : torch::autograd::Function<FirstOrderFn> {
+  static at::Tensor forward(AutogradContext*, const at::Tensor& x) { return x.detach(); }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "the gradients of the post-training operators cannot be differentiated again");
+  }
+};
+
+variable_list first_order(variable_list g) {
+  if (at::GradMode::is_enabled())
+    for (at::Tensor& t : g)
+      if (t.defined()) t = FirstOrderFn::apply(t.set_requires_grad(true));
+  return g;
+}
+
 struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& hidden, const at::Tensor& weight,
                             const at::Tensor& w, const at::Tensor& labels, int64_t ignore_index, double softcap,
@@ -859,7 +876,7 @@ struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
     variable_list out(11);
     if (r[0].has_value()) out[0] = *r[0];
     if (r[1].has_value()) out[1] = *r[1];
-    return out;
+    return first_order(std::move(out));
   }
 };
 
@@ -891,7 +908,7 @@ struct PreferenceFn : torch::autograd::Function<PreferenceFn> {
       const auto s = ctx->get_saved_variables();
       out[0] = preference_bwd(s[0], s[1], g[0]);
     }
-    return out;
+    return first_order(std::move(out));
   }
 };
 
@@ -921,7 +938,7 @@ struct PolicyFn : torch::autograd::Function<PolicyFn> {
     out[0] = it->second.toTensor();
     ctx->saved_data.erase(it);
     scale_unless_one_b(out[0], g[0]);
-    return out;
+    return first_order(std::move(out));
   }
 };
 
@@ -953,7 +970,7 @@ struct RouterBalanceFn : torch::autograd::Function<RouterBalanceFn> {
       out = router_balance_bwd({s.begin() + 3, s.end()}, s[2].defined() ? OptTensor(s[2]) : c10::nullopt, s[0],
                                s[1], g[0]);
     out.resize(out.size() + 4);  // none for the indices, the mask and the coefficients
-    return out;
+    return first_order(std::move(out));
   }
 };
 

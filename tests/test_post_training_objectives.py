@@ -139,9 +139,12 @@ def test_fused_router_losses_match_the_default(dev, padded):
         mask = torch.ones(2, 128, dtype=torch.long, device=dev)
         mask[0, 100:] = 0
     got = []
+    # both read one forward pass: on the GPU two passes differ in the last bits of the logits
+    # (the model's split sums add in any order)
+    m = small("qwen3_moe", dev, router_aux_loss_coef=0.1)
+    m(ids, attention_mask=mask)
     for fused in (False, True):
-        m = small("qwen3_moe", dev, fused_router_losses=fused, router_aux_loss_coef=0.1)
-        m(ids, attention_mask=mask)
+        m.fused_router_losses = fused
         aux = m.aux_loss()
         if padded and not fused:  # the default counts padded tokens: restate it without them
             from pluggy_b200.models.qwen3_moe import load_balancing_loss, router_z_loss
@@ -149,7 +152,7 @@ def test_fused_router_losses_match_the_default(dev, padded):
             keep = mask.bool().reshape(-1)
             logits = [x[keep] for x in m._router_logits]
             aux = 0.1 * load_balancing_loss(logits, 32, 4) + 0.001 * router_z_loss(logits)
-        grads = torch.autograd.grad(aux, [b.ffn.router.weight for b in m.blocks])
+        grads = torch.autograd.grad(aux, [b.ffn.router.weight for b in m.blocks], retain_graph=True)
         got.append((aux.detach(), grads, m.last_tokens_per_expert))
     (a, ga, ca), (b, gb, cb) = got
     assert abs(a - b) <= 2.0 ** -16 * a
@@ -216,3 +219,29 @@ def test_operators_replay_from_a_cuda_graph(keep, monkeypatch):
         torch.cuda.synchronize()
         for a, b in zip(out, step(*new)):
             assert torch.equal(a, b)
+
+
+@GPU
+def test_gradients_are_not_differentiated_again():
+    """With a graph of the backward pass asked for, the first gradient is as ever and a second
+    one is refused, not zero."""
+    from pluggy_b200.ops import linear_token_logprobs, policy_loss, preference_loss, router_balance_loss
+
+    def leaf(*shape, dtype=torch.float32):
+        return torch.randn(*shape, device="cuda").to(dtype).requires_grad_(True)
+
+    h, w = leaf(40, 64, dtype=torch.bfloat16), leaf(300, 64, dtype=torch.bfloat16)
+    lp, x = leaf(2, 4, 40), leaf(50, 16)
+    mask = torch.ones(2, 4, 40, dtype=torch.bool, device="cuda")
+    y = torch.randint(0, 300, (40,), device="cuda")
+    idx = torch.arange(100, device="cuda").view(50, 2) % 16
+    for leaves, run in (((h, w), lambda: linear_token_logprobs(h, w, y).sum()),
+                        ((lp,), lambda: preference_loss(lp, None, mask)[0]),
+                        ((lp,), lambda: policy_loss(lp[0], None, torch.ones(4, device="cuda"), mask[0])[0]),
+                        ((x,), lambda: router_balance_loss(x, idx, z_coef=0.1)[0])):
+        plain = torch.autograd.grad(run(), leaves)
+        again = torch.autograd.grad(run(), leaves, create_graph=True)
+        for a, b in zip(plain, again):
+            assert torch.equal(a, b)
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                b.float().sum().backward()
