@@ -505,14 +505,14 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
   p.row_map = ip;
   p.n_rows = count;
   int64_t width = V;
-  at::Tensor x, hs = h, factor;
+  at::Tensor x, hs = h, scale;
   if (kept.has_value()) {
     x = *kept;
-    plg::head_recompute(p, sp, sp + R, g, count + 1, x.data_ptr(), x.stride(0), st);  // only if flagged
+    plg::head_recompute(p, sp, g, count + 1, x.data_ptr(), x.stride(0), st);  // only if flagged
     hs = at::empty_like(h);
-    factor = at::empty({R, 2}, f32);
-    plg::head_scale_rows(p, sp, sp + R, sp + 2 * R, g, x.data_ptr(), x.stride(0), factor.data_ptr<float>(),
-                         hs.data_ptr(), st);
+    scale = at::empty({R}, f32);
+    plg::head_scale_rows(p, sp, sp + 2 * R, g, x.data_ptr(), x.stride(0), scale.data_ptr<float>(), hs.data_ptr(),
+                         st);
   } else {
     if (2 * R * V > workspace)  // ranges of whole 256-column tiles within the workspace
       width = std::min(V, std::max<int64_t>(1, workspace / (2 * R * 256)) * 256);
@@ -523,7 +523,20 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
       width >= V ? std::max<int64_t>(1, std::min<int64_t>(16, split_workspace / (4 * R * D))) : 1;
   at::Tensor dh_rows, dh, dw;
   if (need_h) dh_rows = at::empty({splits, R, D}, f32);
-  if (need_w) dw = at::empty({V, D}, dw_f32 ? f32 : h.options());
+  at::Tensor label_sums, label_row;  // the labels' part of dW
+  if (need_w) {
+    dw = at::empty({V, D}, dw_f32 ? f32 : h.options());
+    label_sums = at::empty({T, D}, f32);
+    label_row = at::empty({V}, labels.options().dtype(at::kInt));
+    at::Tensor sorted, token;
+    if (T > plg::kLabelScanTokens)
+      // labels as int32 (half the sort's passes); those outside the vocabulary are left out anyway
+      std::tie(sorted, token) =
+          at::sort(labels.clamp(-1, V).to(at::kInt), /*stable=*/true, 0, /*descending=*/false);
+    plg::head_label_rows(p, sorted.defined() ? sorted.data_ptr<int>() : nullptr,
+                         token.defined() ? token.data_ptr<int64_t>() : nullptr, ip + T, sp + R, g,
+                         label_sums.data_ptr<float>(), label_row.data_ptr<int>(), static_cast<int>(T), st);
+  }
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int64_t n = std::min(width, V - v0);
     if (!kept.has_value()) {
@@ -532,7 +545,7 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
       r.N = static_cast<int>(n);
       r.bn = plg::head_tile_n(r.rows, r.N);
       r.label0 = v0;
-      plg::head_recompute(r, sp, sp + R, g, nullptr, x.data_ptr(), x.stride(0), st);
+      plg::head_recompute(r, sp, g, nullptr, x.data_ptr(), x.stride(0), st);
     }
     plg::GemmProblem q;
     q.A = x.data_ptr();
@@ -574,19 +587,19 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
       b.C = static_cast<char*>(dw.data_ptr()) + v0 * D * (dw_f32 ? 4 : 2);
       b.c_fp32 = dw_f32;
       b.k_limit = count;
+      b.D = label_sums.data_ptr();
+      b.ldd = D;
+      b.d_fp32 = true;
+      b.d_rows = label_row.data_ptr<int>() + v0;
+      b.beta = 1.f;
       plg::gemm_bf16(b, st);
     }
-  }
-  if (need_w && kept.has_value()) {
-    // labels as int32 (half the sort's passes); those outside the vocabulary are left out anyway
-    const auto order = at::sort(labels.clamp(-1, V).to(at::kInt), /*stable=*/true, 0, /*descending=*/false);
-    plg::head_label_rows(p, std::get<0>(order).data_ptr<int>(), std::get<1>(order).data_ptr<int64_t>(), ip + T,
-                         factor.data_ptr<float>(), dw.data_ptr(), dw_f32, static_cast<int>(T), st);
   }
   if (need_h) {
     dh = at::empty({T, D}, dh_f32 ? f32 : h.options());
     plg::head_scatter(p, dh_rows.data_ptr<float>(), R * D, count + 2,
-                      kept.has_value() ? factor.data_ptr<float>() : nullptr, ip + T, dh.data_ptr(), dh_f32, T, st);
+                      kept.has_value() ? scale.data_ptr<float>() : nullptr, sp + R, g, ip + T, dh.data_ptr(), dh_f32,
+                      T, st);
   }
   return {need_h ? c10::optional<at::Tensor>(dh) : c10::nullopt,
           need_w ? c10::optional<at::Tensor>(dw) : c10::nullopt};

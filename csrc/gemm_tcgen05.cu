@@ -47,6 +47,7 @@ struct Args {
   long long ldd;
   float alpha, beta;
   int c_fp32, d_fp32;
+  const int* d_rows;  // row of D for each row of C, -1: nothing to add (null: the same row)
   int splits;        // >1: fp32 atomic accumulation into C
   int m_tiles, n_tiles, k_blocks;
   int raster_m;      // 1: m-tiles vary fastest
@@ -193,6 +194,12 @@ __device__ __forceinline__ void store_acc_row(const Args& args, uint32_t t_row, 
     store_acc_rows_rs<BN>(args, t_row, row, col_base, stage);
     return;
   }
+  bool add = args.D != nullptr && args.beta != 0.f && kb0 == 0;
+  long long drow = row;
+  if (add && row_ok && args.d_rows != nullptr) {
+    drow = args.d_rows[row];
+    add = drow >= 0;
+  }
 #pragma unroll 1
   for (int c = 0; c < BN / 32; ++c) {
     uint32_t r[32];
@@ -205,9 +212,9 @@ __device__ __forceinline__ void store_acc_row(const Args& args, uint32_t t_row, 
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = zero ? 0.f : __uint_as_float(r[i]) * args.alpha;
     const bool full = col0 + 32 <= args.N;
-    if (args.D != nullptr && args.beta != 0.f && kb0 == 0) {
+    if (add) {
       if (args.d_fp32) {
-        const float* dp = reinterpret_cast<const float*>(args.D) + row * args.ldd + col0;
+        const float* dp = reinterpret_cast<const float*>(args.D) + drow * args.ldd + col0;
         if (full) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
@@ -222,7 +229,7 @@ __device__ __forceinline__ void store_acc_row(const Args& args, uint32_t t_row, 
         }
       } else {
         const __nv_bfloat16* dp =
-            reinterpret_cast<const __nv_bfloat16*>(args.D) + row * args.ldd + col0;
+            reinterpret_cast<const __nv_bfloat16*>(args.D) + drow * args.ldd + col0;
         if (full) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -870,7 +877,7 @@ static void launch(const GemmProblem& p, cudaStream_t stream) {
   a.M = p.M; a.N = p.N; a.K = p.K;
   a.C = p.C; a.ldc = p.ldc; a.D = p.D; a.ldd = p.ldd;
   a.alpha = p.alpha; a.beta = p.beta;
-  a.c_fp32 = p.c_fp32; a.d_fp32 = p.d_fp32;
+  a.c_fp32 = p.c_fp32; a.d_fp32 = p.d_fp32; a.d_rows = p.d_rows;
   a.m_tiles = (p.M + BM - 1) / BM;
   a.n_tiles = (p.N + BN - 1) / BN;
   a.k_blocks = (p.K + BK - 1) / BK;
@@ -931,7 +938,7 @@ static void launch_pair(const GemmProblem& p, cudaStream_t stream) {
   a.M = p.M; a.N = p.N; a.K = p.K;
   a.C = p.C; a.ldc = p.ldc; a.D = p.D; a.ldd = p.ldd;
   a.alpha = p.alpha; a.beta = p.beta;
-  a.c_fp32 = p.c_fp32; a.d_fp32 = p.d_fp32;
+  a.c_fp32 = p.c_fp32; a.d_fp32 = p.d_fp32; a.d_rows = p.d_rows;
   a.m_tiles = (p.M + 2 * BM - 1) / (2 * BM);
   a.n_tiles = (p.N + BN - 1) / BN;
   a.k_blocks = (p.K + BK - 1) / BK;
@@ -1018,6 +1025,8 @@ void gemm_bf16(const GemmProblem& p, cudaStream_t stream) {
   if (p.max_split > 1 && (!p.c_fp32 || p.D != nullptr || p.allow_split || p.split_out == nullptr ||
                           p.split_stride < (long long)p.M * p.ldc || p.split_stride % p.ldc || p.grp_mode || p.rs_n))
     throw std::invalid_argument("gemm: k splits stored apart need a plain fp32 output with room for each");
+  if (p.d_rows != nullptr && (p.D == nullptr || p.D == p.C || p.allow_split || p.splits > 1 || p.grp_mode || p.rs_n))
+    throw std::invalid_argument("gemm: a row table needs an addend of its own and a plain product");
   const bool wide = p.N >= 256 && p.bn != 128;
   // large problems: 256 x 256 tiles on SM pairs (bn == 256 keeps the one-SM kernel)
   const bool pair = wide && p.bn == 0 && p.M >= 256 && num_sms() >= 2 && !p.grp_mode;

@@ -9,18 +9,21 @@
 // tile into a running (reference, sum of 2^(z log2e - reference)) pair, and a second small
 // kernel joins a row's pairs in a fixed order.
 //
-// Gradient. dh = G W and dW = G^T h with G[t, v] = g_t * d out[t] / d a[t, v], in bf16. The
-// plain way recomputes each tile of the product in the backward pass (head_kernel STORE):
-// 8 T V D operations in all. Large problems need 6: dh = diag(c) X W and dW = X^T diag(c) h
-// hold for any X whose rows are G's up to factors c_t, so the forward pass already stores
+// Gradient. dh = G W and dW = G^T h with G[t, v] = g_t * d out[t] / d a[t, v], in bf16, but for
+// the labels' entries, most of a gradient's norm: G has zeros there, and their part is added in
+// fp32: one weight row to each row of dh (scatter_kernel), one hidden row for each token to dW
+// (label_rows_kernel sums them, the product's epilogue adds them before its rounding). With them in G its rounding to bf16 would be as large as the output's
+// (error of dW against 64 bits 0.0026, now the output's own 0.0017). The plain way recomputes
+// each tile of the product in the backward pass (head_kernel STORE): 8 T V D operations in all.
+// Large problems need 6: dh = diag(c) X W and dW = X^T diag(c) h hold for any X whose rows are
+// G's up to factors c_t, so the forward pass already stores
 //   X[t, v] = bf16(2^(z log2e - r_t) * softcap'(a)),   r_t = z[t, y_t] log2e + 40
 // with a reference r_t that one dot product gives beforehand, and the backward pass folds
 // c_t = -(g_t / temperature) 2^(r_t - lse2_t) into the hidden rows (for dW) and into the result
-// (for dh). The labels' entries, most of a gradient's norm, are left out of X and added in
-// fp32: one weight row to each row of dh, one hidden row for each token to dW. Since lse2 >= z_y log2e, the entries that matter
-// lie above 2^-100 and below 2^(-out log2e - 40): bf16's range holds them unless out < -97 or
-// so. If any row is beyond that, a flag in device memory makes the backward pass recompute.
-// What it costs: c_t h_t is rounded to bf16 (2^-8 of a term of dW other than the labels').
+// (for dh). Since lse2 >= z_y log2e, the entries that matter lie above 2^-100 and below
+// 2^(-out log2e - 40): bf16's range holds them unless out < -97 or so. If any row is beyond
+// that, a flag in device memory makes the backward pass recompute. What it costs: c_t h_t is
+// rounded to bf16 (2^-8 of a term of dW other than the labels').
 //
 // Rows whose label is ignore_index are left out of the products: compact_kernel lists
 // the others on the device, gather_kernel packs their hidden rows, and every later kernel reads
@@ -76,7 +79,6 @@ struct HeadArgs {
   float2* part;                 // statistics: [rows][2 * n_tiles]
   float* target;                // statistics: [rows] a (after the softcap) of the label
   const float* ref;             // X: [rows] r_t
-  const float* label_grad;      // X alone: [rows] (1 - p_y) softcap'(a_y)
   const float* gout;            // X alone: per token
   float inv_temp;
   const int* only_if;           // X alone: nothing to do unless this device flag is set
@@ -184,15 +186,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = row < rows;
       // this row's label as a column of this launch, and its constants
       long long lab = -1;
-      float rref = 0.f, lgrad = 0.f, coef = 0.f;
+      float rref = 0.f, coef = 0.f;
       if (live) {
         const int tok = args.row_map != nullptr ? args.row_map[row] : row;
         lab = args.labels[tok] - args.label0;
         if (STORE) rref = args.ref[row];
-        if (STORE && !STATS) {
-          coef = args.gout[tok] * args.inv_temp;
-          lgrad = args.label_grad[row] * coef;
-        }
+        if (STORE && !STATS) coef = args.gout[tok] * args.inv_temp;
       }
       // warps without any row in use skip the math (X gets its zero rows all the same)
       const bool busy = STORE ? row0 < args.rows : row0 < rows;
@@ -296,8 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                   v[i + 1] *= slope[(i + 1) % (CAP && STORE ? 32 : 1)];
                 }
                 if (!STATS) {
-                  v[i] = i == lc ? lgrad : -coef * v[i];
-                  v[i + 1] = i + 1 == lc ? lgrad : -coef * v[i + 1];
+                  v[i] = i == lc ? 0.f : -coef * v[i];
+                  v[i + 1] = i + 1 == lc ? 0.f : -coef * v[i + 1];
                 }
                 // rows past the count up to the tile's end: zero padding of the products
                 o[i / 2] = live ? pack_bf16x2(v[i], v[i + 1]) : 0u;
@@ -910,19 +909,17 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ pa
   }
 }
 
-// Completes a kept X. Per row: c_t, the bf16 row c_t h_t, and the label's own factor, whose
-// entry of X becomes 0. Under the flag X has been recomputed as the gradient rows themselves,
-// labels included: the factors are 1 and 0.
+// Completes a kept X. Per row: c_t, the bf16 row c_t h_t, and a 0 at the label. Under the flag X
+// has been recomputed as the gradient rows themselves: c_t = 1.
 __global__ void __launch_bounds__(128) scale_rows_kernel(const __nv_bfloat16* __restrict__ h, int D,
                                                          const int* __restrict__ row_map,
                                                          const int* __restrict__ count,
                                                          const int64_t* __restrict__ labels,
                                                          const float* __restrict__ lse2,
-                                                         const float* __restrict__ label_grad,
                                                          const float* __restrict__ ref,
                                                          const float* __restrict__ gout, float inv_temp,
                                                          __nv_bfloat16* __restrict__ X, long long ldx,
-                                                         float2* __restrict__ factor,
+                                                         float* __restrict__ scale,
                                                          __nv_bfloat16* __restrict__ hs, int cap_rows) {
   const int n = count[0];
   const bool whole = count[1] != 0;
@@ -936,15 +933,10 @@ __global__ void __launch_bounds__(128) scale_rows_kernel(const __nv_bfloat16* __
     const int tok = row_map[r];
     float c = 1.f;
     if (!whole) {
-      const float gap = lse2[r] - ref[r], g = gout[tok] * inv_temp;
-      c = -g * exp2f(-gap);
-      if (threadIdx.x == 0) {
-        X[r * ldx + labels[tok]] = __float2bfloat16(0.f);
-        factor[r] = make_float2(c, g * label_grad[r]);
-      }
-    } else if (threadIdx.x == 0) {
-      factor[r] = make_float2(1.f, 0.f);
+      c = -gout[tok] * inv_temp * exp2f(ref[r] - lse2[r]);
+      if (threadIdx.x == 0) X[r * ldx + labels[tok]] = __float2bfloat16(0.f);
     }
+    if (threadIdx.x == 0) scale[r] = c;
     const uint4* src = reinterpret_cast<const uint4*>(h + static_cast<long long>(r) * D);
     for (int i = threadIdx.x; i < D / 8; i += blockDim.x) {
       uint4 u = src[i];
@@ -960,12 +952,14 @@ __global__ void __launch_bounds__(128) scale_rows_kernel(const __nv_bfloat16* __
 }
 
 // dh[token] in dh's type from the compact fp32 rows (the sum of the product's k splits, in
-// their order), zeros for the tokens left out; with a kept X, c_t times the row plus the
-// label's factor times its weight row
+// their order; times c_t with a kept X) plus the label's part, its entry of G times its weight
+// row; zeros for the tokens left out
 template <typename T>
 __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ src, long long split_stride,
                                                       const int* __restrict__ splits,
-                                                      const float2* __restrict__ factor,
+                                                      const float* __restrict__ scale,
+                                                      const float* __restrict__ label_grad,
+                                                      const float* __restrict__ gout, float inv_temp,
                                                       const __nv_bfloat16* __restrict__ w, long long ldw,
                                                       const int64_t* __restrict__ labels,
                                                       const int* __restrict__ inverse,
@@ -974,8 +968,9 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ 
   for (long long t = blockIdx.x; t < tokens; t += gridDim.x) {
     const int r = inverse[t];
     const float4* s = reinterpret_cast<const float4*>(src + static_cast<long long>(r < 0 ? 0 : r) * D);
-    const float2 c = r < 0 || factor == nullptr ? make_float2(1.f, 0.f) : factor[r];
-    const uint2* wr = c.y != 0.f ? reinterpret_cast<const uint2*>(w + labels[t] * ldw) : nullptr;
+    const float c = r < 0 || scale == nullptr ? 1.f : scale[r];
+    const float own = r < 0 ? 0.f : gout[t] * inv_temp * label_grad[r];
+    const uint2* wr = own != 0.f ? reinterpret_cast<const uint2*>(w + labels[t] * ldw) : nullptr;
     for (int i = threadIdx.x; i < D / 4; i += blockDim.x) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r >= 0) {
@@ -984,13 +979,13 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ 
           const float4 a = s[i + k * (split_stride / 4)];
           v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
         }
-        v.x *= c.x; v.y *= c.x; v.z *= c.x; v.w *= c.x;
+        v.x *= c; v.y *= c; v.z *= c; v.w *= c;
         if (wr != nullptr) {
           const float2 a = unpack_bf16x2(wr[i].x), b = unpack_bf16x2(wr[i].y);
-          v.x = fmaf(c.y, a.x, v.x);
-          v.y = fmaf(c.y, a.y, v.y);
-          v.z = fmaf(c.y, b.x, v.z);
-          v.w = fmaf(c.y, b.y, v.w);
+          v.x = fmaf(own, a.x, v.x);
+          v.y = fmaf(own, a.y, v.y);
+          v.z = fmaf(own, b.x, v.z);
+          v.w = fmaf(own, b.y, v.w);
         }
       }
       if (sizeof(T) == 2)
@@ -1001,7 +996,6 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* __restrict__ 
   }
 }
 
-// eight neighbouring values of a row, 16-byte aligned
 __device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -1011,62 +1005,69 @@ __device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
     x[2 * j + 1] = a.y;
   }
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  unpack8(*reinterpret_cast<const uint4*>(p), x);
-}
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                                            pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-}
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
-
-// The labels' part of dW with a kept X: dW[v] += sum of the label factors times the hidden
-// rows of the tokens with label v. Tokens come sorted by label (stable); the block at a run's
-// first token (and, in y, at eight columns a thread) adds up the run in token order: no
-// atomics. A run's rows and factors are listed a block's width at a time, so that the row loads
+// The labels' part of dW, which the product's epilogue adds in fp32: for every label v, the sum
+// over its tokens of their entry of G times their hidden row. The block at a label's first token
+// (and, in y, at eight columns a thread) adds up that label's rows in token order: no atomics.
+// SORTED: tokens come sorted by label (stable), so a label's are neighbours; otherwise every
+// block looks through all labels, which for up to kLabelScanTokens tokens costs less than the
+// sort's launches (with them, D = 256: 10 against 30 us for 777 tokens, 23 against 38 for 2048,
+// 111 against 95 for 8192). Rows and entries are listed a block's width at a time, so that the row loads
 // do not wait for them, and eight rows are fetched at once. Bound by latency: the chain of loads
 // that leads to a row and the longest run (16384 tokens, 300 of them with one label, D = 1024:
 // 90 us; 149 with four columns a thread and the rows' loads left to the compiler).
-template <typename T>
+template <bool SORTED>
 __global__ void __launch_bounds__(128) label_rows_kernel(const int* __restrict__ sorted,
                                                          const int64_t* __restrict__ token,
+                                                         const int64_t* __restrict__ labels,
                                                          const int* __restrict__ inverse,
-                                                         const float2* __restrict__ factor,
+                                                         const float* __restrict__ label_grad,
+                                                         const float* __restrict__ gout, float inv_temp,
                                                          const __nv_bfloat16* __restrict__ h, int D,
-                                                         T* __restrict__ dw, int tokens) {
-  __shared__ int s_row[128];
+                                                         float* __restrict__ sums, int* __restrict__ row_of,
+                                                         int tokens) {
+  __shared__ int s_row[128], s_warp[4];
   __shared__ float s_f[128];
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;  // this thread's first column
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, step = blockDim.x;
   for (int i = blockIdx.x; i < tokens; i += gridDim.x) {
-    const int v = sorted[i];
+    const long long v = SORTED ? sorted[i] : labels[i];
     // a label left out (ignored or outside the vocabulary) is left out for all its tokens
-    if ((i > 0 && sorted[i - 1] == v) || inverse[token[i]] < 0) continue;
-    T* p = dw + static_cast<long long>(v) * D + c;
-    float s[8] = {}, o[8];
-    if (c < D) load8(p, o);
-    for (int j0 = i;; j0 += blockDim.x) {
+    if (inverse[SORTED ? token[i] : i] < 0) continue;
+    if (SORTED) {
+      if (i > 0 && sorted[i - 1] == v) continue;
+    } else {
+      bool earlier = false;
+#pragma unroll 8
+      for (int j = threadIdx.x; j < i; j += step) earlier |= labels[j] == v;
+      if (__syncthreads_or(earlier)) continue;
+    }
+    if (blockIdx.y == 0 && threadIdx.x == 0) row_of[v] = i;
+    float s[8] = {};
+    for (int j0 = i; j0 < tokens; j0 += step) {
       const int j = j0 + threadIdx.x;
-      const bool mine = j < tokens && sorted[j] == v;
-      if (mine) {
-        const int r = inverse[token[j]];
-        s_row[threadIdx.x] = r;
-        s_f[threadIdx.x] = factor[r].y;
+      const bool mine = j < tokens && (SORTED ? sorted[j] == v : labels[j] == v);
+      int at = threadIdx.x;
+      if (!SORTED) {  // the place among the block's matches
+        const unsigned all = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) s_warp[warp] = __popc(all);
+        __syncthreads();
+        at = __popc(all & ((1u << lane) - 1u));
+        for (int k = 0; k < warp; ++k) at += s_warp[k];
       }
-      const int n = __syncthreads_count(mine);  // the run is contiguous: the first n
+      if (mine) {
+        const long long t = SORTED ? token[j] : j;
+        const int r = inverse[t];
+        s_row[at] = r;
+        s_f[at] = gout[t] * inv_temp * label_grad[r];
+      }
+      const int n = __syncthreads_count(mine);
       if (c < D) {
         for (int k0 = 0; k0 < n; k0 += 8) {
           uint4 u[8];  // eight rows on their way at once
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (k0 + k < n) u[k] = *reinterpret_cast<const uint4*>(h + static_cast<long long>(s_row[k0 + k]) * D + c);
+            if (k0 + k < n)
+              u[k] = *reinterpret_cast<const uint4*>(h + static_cast<long long>(s_row[k0 + k]) * D + c);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             if (k0 + k >= n) continue;
@@ -1078,12 +1079,12 @@ __global__ void __launch_bounds__(128) label_rows_kernel(const int* __restrict__
         }
       }
       __syncthreads();
-      if (n < static_cast<int>(blockDim.x)) break;
+      if (SORTED && n < step) break;
     }
     if (c >= D) continue;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] += s[e];
-    store8(p, o);
+    float4* p = reinterpret_cast<float4*>(sums + static_cast<long long>(i) * D + c);
+    p[0] = make_float4(s[0], s[1], s[2], s[3]);
+    p[1] = make_float4(s[4], s[5], s[6], s[7]);
   }
 }
 
@@ -1291,29 +1292,27 @@ void head_join(const HeadProblem& p, const void* part, const float* target, long
                    ref, lse2, label_grad, flag);
 }
 
-void head_recompute(const HeadProblem& p, const float* lse2, const float* label_grad, const float* gout,
-                    const int* only_if, void* X, long long ldx, cudaStream_t st) {
+void head_recompute(const HeadProblem& p, const float* lse2, const float* gout, const int* only_if, void* X,
+                    long long ldx, cudaStream_t st) {
   if (p.rows <= 0) return;
   check_head(p);
   check_x(X, ldx);
   HeadArgs a = base_args(p);
   a.ref = lse2;
-  a.label_grad = label_grad;
   a.gout = gout;
   a.inv_temp = 1.f / p.temperature;
   a.only_if = only_if;
   dispatch_head<false, true>(p, a, X, ldx, st);
 }
 
-void head_scale_rows(const HeadProblem& p, const float* lse2, const float* label_grad, const float* ref,
-                     const float* gout, void* X, long long ldx, float* factor, void* hs, cudaStream_t st) {
+void head_scale_rows(const HeadProblem& p, const float* lse2, const float* ref, const float* gout, void* X,
+                     long long ldx, float* scale, void* hs, cudaStream_t st) {
   if (p.rows <= 0) return;
   if (p.ldh != p.D || p.D % 8)
     throw std::invalid_argument("linear_token_logprobs: packed rows of a multiple of 8 columns");
   scale_rows_kernel<<<std::min(p.rows, 148 * 16), 128, 0, st>>>(
-      static_cast<const __nv_bfloat16*>(p.h), p.D, p.row_map, p.n_rows, p.labels, lse2, label_grad, ref, gout,
-      1.f / p.temperature, static_cast<__nv_bfloat16*>(X), ldx, reinterpret_cast<float2*>(factor),
-      static_cast<__nv_bfloat16*>(hs), p.rows);
+      static_cast<const __nv_bfloat16*>(p.h), p.D, p.row_map, p.n_rows, p.labels, lse2, ref, gout, 1.f / p.temperature,
+      static_cast<__nv_bfloat16*>(X), ldx, scale, static_cast<__nv_bfloat16*>(hs), p.rows);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
@@ -1348,35 +1347,31 @@ void head_gather(const HeadProblem& p, const void* h, bool fp32, long long ldh, 
 }
 
 void head_label_rows(const HeadProblem& p, const int* sorted, const int64_t* token, const int* inverse,
-                     const float* factor, void* dw, bool fp32, int tokens, cudaStream_t st) {
+                     const float* label_grad, const float* gout, float* sums, int* row_of, int tokens,
+                     cudaStream_t st) {
+  PLG_CUDA_CHECK(cudaMemsetAsync(row_of, 0xff, sizeof(int) * static_cast<size_t>(p.N), st));
   if (tokens <= 0) return;
-  const int threads = std::min(128, (p.D / 8 + 31) / 32 * 32);
+  // the search through all labels takes whole blocks
+  const int threads = sorted == nullptr ? 128 : std::min(128, (p.D / 8 + 31) / 32 * 32);
   const dim3 grid(std::min(tokens, 148 * 16), (p.D / 8 + threads - 1) / threads);
-  const float2* f = reinterpret_cast<const float2*>(factor);
-  const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(p.h);
-  if (fp32)
-    label_rows_kernel<float><<<grid, threads, 0, st>>>(sorted, token, inverse, f, h, p.D, static_cast<float*>(dw),
-                                                   tokens);
-  else
-    label_rows_kernel<__nv_bfloat16><<<grid, threads, 0, st>>>(sorted, token, inverse, f, h, p.D,
-                                                           static_cast<__nv_bfloat16*>(dw), tokens);
+  auto kern = sorted != nullptr ? label_rows_kernel<true> : label_rows_kernel<false>;
+  kern<<<grid, threads, 0, st>>>(sorted, token, p.labels, inverse, label_grad, gout, 1.f / p.temperature,
+                                 static_cast<const __nv_bfloat16*>(p.h), p.D, sums, row_of, tokens);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
 void head_scatter(const HeadProblem& p, const float* src, long long split_stride, const int* splits,
-                  const float* factor, const int* inverse, void* dh, bool fp32, long long tokens,
-                  cudaStream_t st) {
+                  const float* scale, const float* label_grad, const float* gout, const int* inverse, void* dh,
+                  bool fp32, long long tokens, cudaStream_t st) {
   if (tokens <= 0) return;
   const int blocks = static_cast<int>(std::min<long long>(tokens, 148 * 16));
-  const float2* f = reinterpret_cast<const float2*>(factor);
-  const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(p.w);
-  if (fp32)
-    scatter_kernel<float><<<blocks, 256, 0, st>>>(src, split_stride, splits, f, w, p.ldw, p.labels, inverse,
-                                                  static_cast<float*>(dh), tokens, p.D);
-  else
-    scatter_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(src, split_stride, splits, f, w, p.ldw, p.labels,
-                                                          inverse, static_cast<__nv_bfloat16*>(dh), tokens,
-                                                          p.D);
+  auto run = [&](auto kern, auto* out) {
+    kern<<<blocks, 256, 0, st>>>(src, split_stride, splits, scale, label_grad, gout, 1.f / p.temperature,
+                                 static_cast<const __nv_bfloat16*>(p.w), p.ldw, p.labels, inverse, out, tokens,
+                                 p.D);
+  };
+  if (fp32) run(scatter_kernel<float>, static_cast<float*>(dh));
+  else run(scatter_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(dh));
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 

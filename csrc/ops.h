@@ -24,6 +24,7 @@ struct GemmProblem {
   const void* D = nullptr;  // optional addend [M, N] (may alias C)
   long long ldd = 0;
   bool d_fp32 = false;
+  const int* d_rows = nullptr;  // device: row of D added to each row of C, -1 for none (null: the same)
   float alpha = 1.f, beta = 0.f;
   int splits = 0;           // 0: automatic split-K for fp32 outputs (when allow_split)
   bool allow_split = true;
@@ -184,17 +185,21 @@ void head_stats(const HeadProblem& p, void* part, float* target, const float* re
 void head_join(const HeadProblem& p, const void* part, const float* target, long long V,
                long long ignore_index, float* out, const float* ref, float* lse2, float* label_grad,
                int* flag, cudaStream_t stream);
-// X = the gradient rows themselves; nothing happens unless *only_if (when given)
-void head_recompute(const HeadProblem& p, const float* lse2, const float* label_grad, const float* gout,
-                    const int* only_if, void* X, long long ldx, cudaStream_t stream);
-// Completes a kept X: 0 at the labels, hs [rows, D] = bf16(c h) (zero rows up to the tile's
-// end) and factor [rows][2] = c and the label's own factor
-void head_scale_rows(const HeadProblem& p, const float* lse2, const float* label_grad, const float* ref,
-                     const float* gout, void* X, long long ldx, float* factor, void* hs, cudaStream_t stream);
-// dw[label] += label factor * hidden row; sorted [tokens] labels and their tokens, inverse as
-// head_compact gives it, p.h the packed rows (contiguous)
+// X = the gradient rows themselves, 0 at the labels; nothing happens unless *only_if (when given)
+void head_recompute(const HeadProblem& p, const float* lse2, const float* gout, const int* only_if, void* X,
+                    long long ldx, cudaStream_t stream);
+// Completes a kept X: 0 at the labels, scale [rows] = c, hs [rows, D] = bf16(c h) (zero rows up
+// to the tile's end)
+void head_scale_rows(const HeadProblem& p, const float* lse2, const float* ref, const float* gout, void* X,
+                     long long ldx, float* scale, void* hs, cudaStream_t stream);
+// The labels' part of dW in fp32: row_of [V] = the row of sums (< tokens) of each label in use
+// and -1 elsewhere, sums [tokens, D] = gout label_grad / temperature times the hidden rows.
+// Up to kLabelScanTokens tokens need no order (sorted null); more come as sorted [tokens] labels
+// and their tokens. inverse as head_compact gives it, p.h the packed rows (contiguous).
+constexpr int kLabelScanTokens = 4096;
 void head_label_rows(const HeadProblem& p, const int* sorted, const int64_t* token, const int* inverse,
-                     const float* factor, void* dw, bool fp32, int tokens, cudaStream_t stream);
+                     const float* label_grad, const float* gout, float* sums, int* row_of, int tokens,
+                     cudaStream_t stream);
 // row_map [T], inverse [T] (token -> row or -1), count [3] = {rows, 0, 1}, and out = 0 / NaN of
 // the tokens left out
 void head_compact(const int64_t* labels, long long T, long long V, long long ignore_index, int* row_map,
@@ -203,11 +208,11 @@ void head_compact(const int64_t* labels, long long T, long long V, long long ign
 // ref [rows] (optional): the reference of X
 void head_gather(const HeadProblem& p, const void* h, bool fp32, long long ldh, void* out, int cap_rows,
                  float* ref, cudaStream_t stream);
-// dh[token] = src row, summed over *splits parts (with factor: times c, plus the label's factor times its
-// weight row), 0 for the tokens left out
+// dh[token] = src row, summed over *splits parts (times scale [rows] if given) plus gout
+// label_grad / temperature times the label's weight row; 0 for the tokens left out
 void head_scatter(const HeadProblem& p, const float* src, long long split_stride, const int* splits,
-                  const float* factor, const int* inverse, void* dh, bool fp32, long long tokens,
-                  cudaStream_t stream);
+                  const float* scale, const float* label_grad, const float* gout, const int* inverse, void* dh,
+                  bool fp32, long long tokens, cudaStream_t stream);
 
 // ---------------------------------------------------------------- objectives
 // Paired preference loss over [2, P, S] token log-probabilities (side 0 chosen, 1 rejected;

@@ -389,3 +389,35 @@ def test_kernel_kept_repeated_labels(dtype, kept, status):
     lp = linear_token_logprobs(h.requires_grad_(True), w.requires_grad_(True), y2)
     dh, dw = torch.autograd.grad(lp, (h, w), g)
     assert torch.isnan(lp[5:7]).all() and torch.isfinite(dh).all() and torch.isfinite(dw).all()
+
+
+@GPU
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("T,D,V", [(1, 64, 300), (300, 128, 700), (1500, 520, 900), (5000, 64, 2000)])
+def test_kernel_label_entries_are_not_rounded(T, D, V, keep, monkeypatch, status):
+    """The labels' entries of G, most of a gradient, stay in fp32; bf16 rounds the others (2^-8 of
+    a term; with kept exponentials twice in dW) and the results (2^-8). 2^-14 of all terms covers
+    G's own error in fp32 (logits of order 10 that are 1e-6 off). Labels repeat: low ids are
+    frequent."""
+    from pluggy_b200.ops import logprob
+
+    monkeypatch.setattr(logprob, "KEEP_PRODUCT", 0 if keep else 1 << 62)
+    h, w, y, g = make(T, D, V, "cuda", ignored=0.2)
+    frequent = (V * torch.rand(T, generator=torch.Generator().manual_seed(T)).pow(3)).long().cuda()
+    y = torch.where(y == IGN, y, frequent)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    dh, dw = torch.autograd.grad(linear_token_logprobs(h, w, y), (h, w), g)
+    with torch.no_grad():
+        H, W = torch.where((y != IGN)[:, None], h.double(), 0.0), w.double()
+        go = torch.where(y != IGN, g.double(), 0.0)[:, None]
+        G = -torch.softmax(H @ W.t(), 1) * go
+        own = torch.zeros_like(G).scatter_(1, y.clamp_min(0)[:, None], 1.0)
+        rest, G = (G * (1 - own)).abs(), G + own * go
+        A = G.abs()
+        rdh, rdw = G @ W, G.t() @ H
+        tol_h = 2.0 ** -8 * (rdh.abs() + rest @ W.abs()) + 2.0 ** -14 * (A @ W.abs()) + 1e-6
+        tol_w = (2.0 ** -8 * (rdw.abs() + (2.01 if keep else 1) * (rest.t() @ H.abs()))
+                 + 2.0 ** -14 * (A.t() @ H.abs()) + 1e-6)
+    assert ((dh - rdh).abs() <= tol_h).all()
+    assert ((dw - rdw).abs() <= tol_w).all()
