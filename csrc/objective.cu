@@ -1,11 +1,12 @@
 // Losses over per-token log-probabilities (paired preference loss, clipped policy loss with
 // a KL term) and over MoE router logits (balance and z loss), forward and backward.
 //
-// All of them stream their inputs once and are bound by memory (or, at a few thousand
-// tokens, by launch latency). Every sum runs in a fixed order: per-warp or per-block
-// partial sums go to a workspace and one block joins them, so results repeat bit for bit.
-// Masked places are skipped by selection, never by a product with 0, so that whatever they
-// hold (infinities, NaN) reaches neither a loss nor a gradient.
+// All of them stream their inputs and are bound by memory, or, at a few thousand tokens, by
+// the host: a forward and backward of one to four launches takes it 70 to 80 us, the GPU 10
+// to 16. Every sum runs in a fixed order: per-warp or per-block partial sums go to a
+// workspace and one block joins them, so results repeat bit for bit. Masked places are
+// skipped by selection, never by a product with 0, so that whatever they hold (infinities,
+// NaN) reaches neither a loss nor a gradient.
 #include <algorithm>
 #include <stdexcept>
 #include <string>
@@ -20,7 +21,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Tokens of one row that a warp takes at a time: 1024 once that gives every warp of the
 // machine (148 SMs x 16) a unit, fewer, down to 128, where there would be too few of them
-// (8 rows of 1023 tokens: 17.9 us at 1024, 6.4 us at 128).
+// (policy loss of 8 rows of 1023 tokens: 17.9 us at 1024, 6.4 us at 128).
 constexpr int kMaxWarpTokens = 1024, kMinWarpTokens = 128;
 
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -65,7 +66,10 @@ __device__ __forceinline__ void load_mask(const uint8_t* p, bool (&m)[VEC]) {
 }
 
 // ------------------------------------------------------------------ preference loss
-// Row r = side * P + pair of [2, P, S] tensors.
+// Row r = side * P + pair of [2, P, S] tensors. A warp sums up to kMaxWarpTokens of a row, so that
+// few long rows fill the machine as many short ones do; the pairs are joined apart because the
+// loss needs both sides of a pair. Bound by memory: 9 bytes a token with an fp32 reference (511
+// pairs of 8192 tokens, bf16 reference: 59 MB in 21 us, 2.8 TB/s: too short to run at full rate).
 template <int VEC>
 __global__ void __launch_bounds__(256) pref_sums_kernel(const PrefArgs a, float2* __restrict__ part,
                                                         int chunks, int len, unsigned* __restrict__ ticket) {
@@ -111,6 +115,8 @@ __global__ void __launch_bounds__(256) pref_sums_kernel(const PrefArgs a, float2
 // One warp per pair joins its chunks; the last block sums the blocks' losses.
 //   h = s_0 - s_1;  sigmoid: (1 - eps) softplus(-b h) + eps softplus(b h);
 //   hinge: max(0, 1 - b h);  ipo: (h - 1 / (2 b))^2
+// The sums and their difference are taken in 64 bits: h is what is left of sums of thousands of
+// tokens. Bound by latency (the chain of a pair and the ticket: 6.7 us for two pairs).
 __global__ void __launch_bounds__(256) pref_pairs_kernel(const PrefArgs a, const float2* __restrict__ part,
                                                          int chunks, double* __restrict__ block_loss,
                                                          unsigned* __restrict__ ticket,
@@ -189,7 +195,8 @@ __global__ void __launch_bounds__(256) pref_pairs_kernel(const PrefArgs a, const
   }
 }
 
-// grad[r, t] = gout * row_scale[r] where the mask holds, else 0 (contiguous [2, P, S])
+// grad[r, t] = gout * row_scale[r] where the mask holds, else 0 (contiguous [2, P, S]). Bound by
+// its writes (511 pairs of 8192 tokens, 42 MB: 12 us).
 template <int VEC>
 __global__ void __launch_bounds__(256) pref_grad_kernel(const PrefArgs a, const float* __restrict__ row_scale,
                                                         const float* __restrict__ gout,
@@ -221,7 +228,9 @@ __global__ void __launch_bounds__(256) pref_grad_kernel(const PrefArgs a, const 
 
 // ---------------------------------------------------------------------- policy loss
 // counts[r] = tokens of row r; block_counts[b] = (tokens, rows with any) of block b's rows.
-// A row is counted by one warp, or by the whole block when rows are long.
+// A row is counted by one warp, or by the whole block when rows are long. It runs ahead of the
+// main pass because a token's gradient needs the counts, and a mask is one byte of a token's 21
+// (1024 x 16384: 8 us).
 template <bool BLOCK_ROW>
 __global__ void __launch_bounds__(256) policy_counts_kernel(const PolicyArgs a, int* __restrict__ counts,
                                                             longlong2* __restrict__ block_counts,
@@ -305,7 +314,10 @@ __device__ __forceinline__ void kl_terms(float d, float& em1, float& k3) {
 //   loss = -A e^r (the bound instead of e^r once A pushes r past it) + kl_coef (e^d - 1 - d)
 //   grad = -A e^r (0 past the bound) - kl_coef (e^d - 1)
 // each times the token's weight in the mean, known from the counts.
-// OLD, REF, ADV: old log-probabilities, reference and per-token advantages are given
+// OLD, REF, ADV: old log-probabilities, reference and per-token advantages are given (a kernel for
+// each set: 67 us instead of 80 with the choice made per token). Loss and gradient come from one
+// pass, so that nothing is read twice. Bound by memory: 21 bytes a token (1024 x 16384: 352 MB in
+// 66 us, 5.3 TB/s, 0.81 of the measured copy rate).
 constexpr int kPolicyResident = 3;
 template <int VEC, bool OLD, bool REF, bool ADV>
 __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const PolicyArgs a, const int* __restrict__ counts,
@@ -436,7 +448,8 @@ __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const Poli
   }
 }
 
-// x *= *s, unless *s is 1 (the usual gradient of a loss): then nothing is read or written
+// x *= *s, unless *s is 1 (the usual gradient of a loss): then nothing is read or written and the
+// launch costs 2 us
 template <int VEC>
 __global__ void __launch_bounds__(256) scale_unless_one_kernel(float* __restrict__ x, long long n,
                                                                const float* __restrict__ s) {
@@ -551,11 +564,14 @@ __device__ __forceinline__ float group_max(float v) {
 }
 
 // Blocks an SM: the sums keep 32 bf16 values a lane (fewer shuffles and scalar steps for a row:
-// 112 us instead of 131 for the rows alone of 24 x 32768 x 256), the gradient 16.
+// 97 us instead of 130 with 16, 24 x 32768 x 256), the gradient 16.
 constexpr int kRouterThreads = 256, kRouterSumsResident = 2, kRouterGradResident = 4;
 
 // Per block: column sums of the probabilities, the sum of lse^2, the kept tokens and the
 // histogram of the chosen experts over the block's rows; lse of every row for the backward.
+// A row lies in the registers of a group of lanes, so its maximum, sum and probabilities take one
+// read and no shared memory. Bound by instructions (exponential, sums, shuffles) together with
+// memory: 24 x 32768 x 256 bf16 and 8 indices each, 453 MB in 101 us, 4.5 TB/s.
 template <typename T, int VEC, int G, int NV, bool FULL>
 __global__ void __launch_bounds__(kRouterThreads, kRouterSumsResident) router_sums_kernel(const __grid_constant__ RouterArgs a,
                                                                      float* __restrict__ lse_out,
@@ -678,7 +694,7 @@ __global__ void __launch_bounds__(kRouterThreads, kRouterSumsResident) router_su
 }
 
 // Joins the partial sums, 32 columns a block; the last block to finish adds the blocks' parts
-// of the loss in their order. counts, and the backward's constants
+// of the loss in their order (9 to 11 us, latency). counts, and the backward's constants
 //   slope[e] = c_b E / n * f_e  and  slope[E] = 2 c_z / n
 __global__ void __launch_bounds__(1024) router_join_kernel(const float* __restrict__ part_p,
                                                            const int* __restrict__ part_n,
@@ -764,7 +780,10 @@ __global__ void __launch_bounds__(1024) router_join_kernel(const float* __restri
   }
 }
 
-// dlogit = gout p (slope_e - <p, slope> + slope_E lse), 0 in masked rows
+// dlogit = gout p (slope_e - <p, slope> + slope_E lse), 0 in masked rows. The probabilities are
+// taken from the logits and lse again: half the bytes of storing them. Bound by memory: 24 x 32768
+// x 256 bf16 read and written, 805 MB in 128 us, 6.3 TB/s, 0.96 of the measured copy rate (the
+// last rows first, so that some are still in L2, gained 0.3%: not kept).
 template <typename T, int VEC, int G, int NV, bool FULL>
 __global__ void __launch_bounds__(kRouterThreads, NV * VEC > 16 ? 2 : sizeof(T) == 2 ? kRouterGradResident : 3) router_grad_kernel(const __grid_constant__ RouterArgs a,
                                                                      const float* __restrict__ lse_in,

@@ -11,8 +11,9 @@ reference model or one sampled token at a time.
 
 CUDA path (csrc/logprob.cu): the product's tcgen05 epilogue reduces every accumulator
 tile to a (maximum, sum of exponentials) pair per row, so no logits are written; the
-backward recomputes them one vocabulary range at a time as the bf16 gradient
-``g_t * (onehot - softmax)``, whose two products give the gradients. Ranges are split over
+backward recomputes them one vocabulary range at a time as the bf16 matrix
+``-g_t * softmax``, whose two products give the gradients; the labels' own entries, most of a
+gradient, never leave fp32. Ranges are split over
 the vocabulary rather than over the tokens so that each row of the weight's gradient is
 written once, in its final type, instead of being summed over chunks of tokens. Large
 problems save that second product of hidden and weight: the forward stores bf16
@@ -31,7 +32,7 @@ from pluggy_b200.ops._ext import ext, status_word
 # from its forward to its backward, or recomputes at a time
 WORKSPACE = 8 << 30
 # tokens * vocabulary * D from which the matrix is kept: below it the product that this saves
-# takes less than 0.1 ms, and recomputing rounds the weight's gradient once less
+# takes less than 0.1 ms, and recomputing rounds a term of the weight's gradient once less
 KEEP_PRODUCT = 1 << 36
 # bytes of the k splits' fp32 sums of the hidden rows' gradient
 SPLIT_WORKSPACE = 512 << 20
