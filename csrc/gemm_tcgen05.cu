@@ -91,11 +91,14 @@ __device__ __forceinline__ int pick_splits(int tiles, int slots, int k_blocks, i
   return best;
 }
 
-// m tiles and k blocks in use under the device limits
+// m tiles and k blocks in use under the device limits. Kernels without EXT have neither limits,
+// splits stored apart nor a row table, and none of their registers.
+template <bool EXT>
 __device__ __forceinline__ void limited_extent(const Args& args, int tile_m, int& m_tiles,
                                                int& k_blocks) {
   m_tiles = args.m_tiles;
   k_blocks = args.k_blocks;
+  if (!EXT) return;
   if (args.m_limit != nullptr) m_tiles = min(m_tiles, (max(*args.m_limit, 0) + tile_m - 1) / tile_m);
   if (args.k_limit != nullptr) k_blocks = min(k_blocks, (max(*args.k_limit, 0) + BK - 1) / BK);
 }
@@ -186,7 +189,7 @@ __device__ __forceinline__ void store_acc_rows_rs(const Args& args, uint32_t t_r
   __syncwarp();
 }
 
-template <int BN>
+template <int BN, bool EXT>
 __device__ __forceinline__ void store_acc_row(const Args& args, uint32_t t_row, long long row,
                                               bool row_ok, int col_base, int kb0, uint8_t* stage,
                                               bool zero = false) {
@@ -194,12 +197,8 @@ __device__ __forceinline__ void store_acc_row(const Args& args, uint32_t t_row, 
     store_acc_rows_rs<BN>(args, t_row, row, col_base, stage);
     return;
   }
-  bool add = args.D != nullptr && args.beta != 0.f && kb0 == 0;
   long long drow = row;
-  if (add && row_ok && args.d_rows != nullptr) {
-    drow = args.d_rows[row];
-    add = drow >= 0;
-  }
+  if (EXT && row_ok && args.d_rows != nullptr) drow = args.d_rows[row];
 #pragma unroll 1
   for (int c = 0; c < BN / 32; ++c) {
     uint32_t r[32];
@@ -212,7 +211,7 @@ __device__ __forceinline__ void store_acc_row(const Args& args, uint32_t t_row, 
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = zero ? 0.f : __uint_as_float(r[i]) * args.alpha;
     const bool full = col0 + 32 <= args.N;
-    if (add) {
+    if (args.D != nullptr && args.beta != 0.f && kb0 == 0 && (!EXT || drow >= 0)) {
       if (args.d_fp32) {
         const float* dp = reinterpret_cast<const float*>(args.D) + drow * args.ldd + col0;
         if (full) {
@@ -292,7 +291,7 @@ __device__ __forceinline__ void store_acc_row(const Args& args, uint32_t t_row, 
   }
 }
 
-template <int BN, bool A_MN, bool B_MN>
+template <int BN, bool A_MN, bool B_MN, bool EXT>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 Args args) {
@@ -341,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_base_smem;
 
   int m_tiles, k_blocks;
-  limited_extent(args, BM, m_tiles, k_blocks);
+  limited_extent<EXT>(args, BM, m_tiles, k_blocks);
   const int total_tiles = m_tiles * args.n_tiles;
   const int total_work = total_tiles * (args.grp_mode == 2 ? args.grp_count : args.splits);
   const int kb_per_split = (k_blocks + args.splits - 1) / args.splits;
@@ -514,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const long long crow = args.grp_mode == 2 ? g * args.grp_c_rows + row : row;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
       // the addend D is applied by the first k split (mode 2 has one split per group)
-      store_acc_row<BN>(args, t_row, crow, row_ok, nt * BN, args.grp_mode == 2 ? 0 : kb0,
+      store_acc_row<BN, EXT>(args, t_row, crow, row_ok, nt * BN, args.grp_mode == 2 ? 0 : kb0,
                         epi_stage + q * 32 * 128, kb1 <= kb0);
       tc_fence_before();
       __syncwarp();
@@ -553,7 +552,7 @@ struct PairCfg {
   static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256 + kEpiStageBytes;
 };
 
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, bool EXT>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      Args args) {
@@ -606,11 +605,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_base_smem;
 
   int m_tiles, k_blocks;
-  limited_extent(args, 2 * BM, m_tiles, k_blocks);
+  limited_extent<EXT>(args, 2 * BM, m_tiles, k_blocks);
   const int total_tiles = m_tiles * args.n_tiles;  // 256 x 256 tiles
-  const int splits = args.max_split > 1 ? pick_splits(total_tiles, npairs, k_blocks, args.max_split)
+  const int splits = EXT && args.max_split > 1 ? pick_splits(total_tiles, npairs, k_blocks, args.max_split)
                                         : args.splits;
-  if (args.max_split > 1 && blockIdx.x == 0 && threadIdx.x == 0) *args.split_out = splits;
+  if (EXT && args.max_split > 1 && blockIdx.x == 0 && threadIdx.x == 0) *args.split_out = splits;
   const int total_work = total_tiles * splits;
   const int kb_per_split = (k_blocks + splits - 1) / splits;
   auto decode = [&](int w, int& mt, int& nt, int& kb0, int& kb1) {
@@ -765,9 +764,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
       // splits stored apart: split i's rows follow at i * split_stride (whole rows of C)
       const long long crow =
-          args.max_split > 1 ? row + kb0 / max(kb_per_split, 1) * (args.split_stride / args.ldc) : row;
-      store_acc_row<BN>(args, t_row, crow, row < args.M, nt * BN, kb0, epi_stage + q * 32 * 128,
-                        kb1 <= kb0);
+          EXT && args.max_split > 1 ? row + kb0 / max(kb_per_split, 1) * (args.split_stride / args.ldc) : row;
+      store_acc_row<BN, EXT>(args, t_row, crow, row < args.M, nt * BN, kb0, epi_stage + q * 32 * 128,
+                        EXT && kb1 <= kb0);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(&acce_bar[buf], 0);
@@ -863,7 +862,7 @@ static void set_rs_fields(const GemmProblem& p, Args& a, int tile_m) {
   if (a.m_tiles > 0) a.rs_mshift = static_cast<int>((p.rs_rank * a.rs_seg / tile_m) % a.m_tiles);
 }
 
-template <int BN, bool A_MN, bool B_MN>
+template <int BN, bool A_MN, bool B_MN, bool EXT>
 static void launch(const GemmProblem& p, cudaStream_t stream) {
   using C_ = Cfg<BN>;
   // A map
@@ -919,13 +918,13 @@ static void launch(const GemmProblem& p, cudaStream_t stream) {
   if (p.grp_mode == 1) a.raster_m = 0;
   const int work = tiles * (p.grp_mode == 2 ? p.grp_count : splits);
   const int grid = work < sms ? work : sms;
-  auto kern = gemm_kernel<BN, A_MN, B_MN>;
+  auto kern = gemm_kernel<BN, A_MN, B_MN, EXT>;
   set_max_smem_once(reinterpret_cast<const void*>(kern), C_::kSmemBytes);
   kern<<<grid, kThreads, C_::kSmemBytes, stream>>>(ta, tb, a);
   PLG_CUDA_CHECK(cudaGetLastError());
 }
 
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, bool EXT>
 static void launch_pair(const GemmProblem& p, cudaStream_t stream) {
   using C_ = PairCfg;
   constexpr int BN = C_::BN;
@@ -949,7 +948,7 @@ static void launch_pair(const GemmProblem& p, cudaStream_t stream) {
   a.split_stride = p.split_stride;
   a.split_out = p.split_out;
   set_rs_fields(p, a, 2 * BM);
-  auto kern = gemm_pair_kernel<A_MN, B_MN>;
+  auto kern = gemm_pair_kernel<A_MN, B_MN, EXT>;
   set_max_smem_once(reinterpret_cast<const void*>(kern), C_::kSmemBytes);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads, 1, 1);
@@ -1030,27 +1029,35 @@ void gemm_bf16(const GemmProblem& p, cudaStream_t stream) {
   const bool wide = p.N >= 256 && p.bn != 128;
   // large problems: 256 x 256 tiles on SM pairs (bn == 256 keeps the one-SM kernel)
   const bool pair = wide && p.bn == 0 && p.M >= 256 && num_sms() >= 2 && !p.grp_mode;
-#define PLG_GEMM_CASE(BN_, AM, BMJ) \
-  if (p.a_mn_major == AM && p.b_mn_major == BMJ) return launch<BN_, AM, BMJ>(p, stream);
-#define PLG_GEMM_PAIR(AM, BMJ) \
-  if (p.a_mn_major == AM && p.b_mn_major == BMJ) return launch_pair<AM, BMJ>(p, stream);
+  const bool ext = p.m_limit != nullptr || p.k_limit != nullptr || p.max_split > 1 || p.d_rows != nullptr;
+  if (ext && !p.b_mn_major) throw std::invalid_argument("gemm: device row counts and row tables need an MN-major B");
+#define PLG_GEMM_CASE(BN_, AM, BMJ, X) \
+  if (p.a_mn_major == AM && p.b_mn_major == BMJ && ext == X) return launch<BN_, AM, BMJ, X>(p, stream);
+#define PLG_GEMM_PAIR(AM, BMJ, X) \
+  if (p.a_mn_major == AM && p.b_mn_major == BMJ && ext == X) return launch_pair<AM, BMJ, X>(p, stream);
   if (pair) {
-    PLG_GEMM_PAIR(false, false)
-    PLG_GEMM_PAIR(false, true)
-    PLG_GEMM_PAIR(true, true)
-    PLG_GEMM_PAIR(true, false)
+    PLG_GEMM_PAIR(false, false, false)
+    PLG_GEMM_PAIR(false, true, false)
+    PLG_GEMM_PAIR(true, true, false)
+    PLG_GEMM_PAIR(true, false, false)
+    PLG_GEMM_PAIR(false, true, true)
+    PLG_GEMM_PAIR(true, true, true)
   }
 #undef PLG_GEMM_PAIR
   if (wide) {
-    PLG_GEMM_CASE(256, false, false)
-    PLG_GEMM_CASE(256, false, true)
-    PLG_GEMM_CASE(256, true, true)
-    PLG_GEMM_CASE(256, true, false)
+    PLG_GEMM_CASE(256, false, false, false)
+    PLG_GEMM_CASE(256, false, true, false)
+    PLG_GEMM_CASE(256, true, true, false)
+    PLG_GEMM_CASE(256, true, false, false)
+    PLG_GEMM_CASE(256, false, true, true)
+    PLG_GEMM_CASE(256, true, true, true)
   } else {
-    PLG_GEMM_CASE(128, false, false)
-    PLG_GEMM_CASE(128, false, true)
-    PLG_GEMM_CASE(128, true, true)
-    PLG_GEMM_CASE(128, true, false)
+    PLG_GEMM_CASE(128, false, false, false)
+    PLG_GEMM_CASE(128, false, true, false)
+    PLG_GEMM_CASE(128, true, true, false)
+    PLG_GEMM_CASE(128, true, false, false)
+    PLG_GEMM_CASE(128, false, true, true)
+    PLG_GEMM_CASE(128, true, true, true)
   }
 #undef PLG_GEMM_CASE
 }

@@ -51,7 +51,7 @@ struct GemmProblem {
   long long grp_b_rows = 0;
   const int* grp_koff = nullptr;
   int grp_count = 0;
-  // Device row counts (ungrouped, no split-K): rows of C past *m_limit are not computed, the
+  // Device row counts (ungrouped, no split-K, B MN-major): rows of C past *m_limit are not computed, the
   // sum stops at the 64-row block holding row *k_limit - 1 (A and B finite to its end; a
   // count of 0 writes zeros).
   const int* m_limit = nullptr;
