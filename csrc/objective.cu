@@ -403,8 +403,10 @@ __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const Poli
           float em1, k3;
           kl_terms(df[j], em1, k3);
           sk += mm[j] ? k3 : 0.f;
-          l = fmaf(a.kl_coef, k3, l);
-          d = fmaf(-a.kl_coef, em1, d);
+          if (a.kl_coef != 0.f) {  // a KL that is only reported may be infinite
+            l = fmaf(a.kl_coef, k3, l);
+            d = fmaf(-a.kl_coef, em1, d);
+          }
         }
         sl += mm[j] ? l : 0.f;
         sc += (mm[j] && clip) ? 1 : 0;

@@ -534,3 +534,17 @@ def test_nothing_to_do(dev):
     loss, counts = router_balance_loss(x, torch.zeros(0, 2, dtype=torch.int64, device=dev))
     assert loss == 0 and (counts == 0).all()
     loss.backward()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_policy_reported_kl_may_overflow(dev):
+    """With kl_coef 0 a KL estimate beyond fp32 is reported and reaches neither loss nor gradient."""
+    lp = torch.tensor([[-100.0, -1.0, -2.0]], device=dev, requires_grad=True)
+    adv, mask = torch.ones(1, device=dev), torch.ones(1, 3, dtype=torch.bool, device=dev)
+    want = policy_loss(lp, None, adv, mask)[0]
+    (egrad,) = torch.autograd.grad(want, lp, retain_graph=True)
+    for far in (-1.0, float("-inf")):
+        ref = torch.tensor([[far, -1.5, -1.0]], device=dev)
+        loss, kl, _ = policy_loss(lp, None, adv, mask, ref_logps=ref)
+        (grad,) = torch.autograd.grad(loss, lp)
+        assert torch.isinf(kl) and torch.equal(loss, want) and torch.equal(grad, egrad)
