@@ -394,7 +394,8 @@ __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const Poli
       if (t + 32 * VEC < t1) fetch(t + 32 * VEC);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float ratio = OLD ? expf(lr[j]) : 1.f;
+        // an advantage of 0 gives 0 also where e^r overflows
+        const float ratio = OLD ? expf(adv[j] == 0.f && lr[j] > 0.f ? 0.f : lr[j]) : 1.f;
         const bool up = adv[j] > 0.f && lr[j] > a.log_hi, dn = adv[j] < 0.f && lr[j] < a.log_lo;
         const bool clip = up || dn;
         float l = -(up ? a.hi : dn ? a.lo : ratio) * adv[j];

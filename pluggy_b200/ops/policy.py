@@ -53,7 +53,9 @@ def policy_loss_reference(logps, old_logps, advantages, mask, ref_logps=None, cl
     up = (adv > 0) & (r > math.log1p(clip_high))
     dn = (adv < 0) & (r < math.log1p(-clip_low))
     bound = torch.where(up, 1 + clip_high, 1 - clip_low)
-    per = -torch.where(up | dn, bound, torch.exp(torch.where(up | dn, 0.0, r))) * adv
+    # an advantage of 0 gives 0 also where e^r overflows
+    flat = up | dn | ((adv == 0) & (r > 0))
+    per = -torch.where(up | dn, bound, torch.exp(torch.where(flat, 0.0, r))) * adv
     kl = torch.zeros_like(lp)
     if ref_logps is not None:
         kl = _KlTerm.apply(at(ref_logps) - lp)

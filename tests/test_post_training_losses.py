@@ -548,3 +548,22 @@ def test_policy_reported_kl_may_overflow(dev):
         loss, kl, _ = policy_loss(lp, None, adv, mask, ref_logps=ref)
         (grad,) = torch.autograd.grad(loss, lp)
         assert torch.isinf(kl) and torch.equal(loss, want) and torch.equal(grad, egrad)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("per_token", [False, True])
+def test_policy_zero_advantage_and_overflowing_ratio(per_token, dev):
+    """exp(99) is beyond fp32, its product with an advantage of 0 is 0; a NaN ratio stays NaN."""
+    lp = torch.tensor([[-1.0, -1.0, -1.0], [-1.0, -2.0, -1.0]], device=dev, requires_grad=True)
+    old = torch.tensor([[-100.0, -1.5, -100.0], [-1.0, -1.5, -1.0]], device=dev)
+    mask = torch.ones(2, 3, dtype=torch.bool, device=dev)
+    adv = torch.tensor([0.0, 0.5], device=dev)
+    adv = adv[:, None].expand(2, 3).contiguous() if per_token else adv
+    loss, _, share = policy_loss(lp, old, adv, mask)
+    (grad,) = torch.autograd.grad(loss, lp)
+    want, _, _, egrad, mag, gmag = policy_exact(lp.detach(), old, adv, mask, None, 0.2, 0.2, 0.0, "token")
+    assert (loss - want).abs() <= 2.0 ** -18 * mag and share == 0
+    assert ((grad - egrad).abs() <= 2.0 ** -20 * gmag).all() and (grad[0] == 0).all()
+    bad = old.clone()
+    bad[0, 1] = float("nan")
+    assert torch.isnan(policy_loss(lp, bad, adv, mask)[0])
