@@ -857,6 +857,14 @@ struct FirstOrderFn : torch::autograd::Function<FirstOrderFn> {
   }
 };
 
+// Forward-mode derivatives are refused: the calls that skip their autograd function would
+// return results without a tangent, which reads as a derivative of zero.
+void refuse_tangents(const char* op, std::initializer_list<OptTensor> inputs) {
+  for (const OptTensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.has_value() || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), op,
+                                ": no forward-mode derivatives");
+}
+
 variable_list first_order(variable_list g) {
   if (at::GradMode::is_enabled())
     for (at::Tensor& t : g)
@@ -899,6 +907,7 @@ at::Tensor token_logprobs(const at::Tensor& hidden, const at::Tensor& weight, co
                           const at::Tensor& labels, int64_t ignore_index, double softcap, double temperature,
                           bool pack, bool keep, int64_t workspace, int64_t split_workspace,
                           const at::Tensor& status) {
+  refuse_tangents("linear_token_logprobs", {hidden, weight, w});
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
     return TokenLogprobsFn::apply(hidden, weight, w, labels, ignore_index, softcap, temperature, keep, workspace,
                                   split_workspace, status);
@@ -928,6 +937,7 @@ struct PreferenceFn : torch::autograd::Function<PreferenceFn> {
 // (loss, chosen rewards, rejected rewards)
 variable_list preference_loss(const at::Tensor& logps, const OptTensor& ref, const at::Tensor& mask, int64_t kind,
                               double beta, double smoothing, bool normalized) {
+  refuse_tangents("preference_loss", {logps, ref});
   return PreferenceFn::apply(logps, ref, mask, kind, beta, smoothing, normalized);
 }
 
@@ -959,6 +969,7 @@ struct PolicyFn : torch::autograd::Function<PolicyFn> {
 variable_list policy_loss(const at::Tensor& logps, const OptTensor& old, const at::Tensor& adv,
                           const at::Tensor& mask, const OptTensor& ref, double clip_low, double clip_high,
                           double kl_coef, bool by_sequence) {
+  refuse_tangents("policy_loss", {logps, old, adv, ref});
   if (at::GradMode::is_enabled() && logps.requires_grad())
     return PolicyFn::apply(logps, old, adv, mask, ref, clip_low, clip_high, kl_coef, by_sequence);
   return policy_fwd(logps, old, adv, mask, ref, clip_low, clip_high, kl_coef, by_sequence, false);
@@ -990,6 +1001,7 @@ struct RouterBalanceFn : torch::autograd::Function<RouterBalanceFn> {
 // (loss, tokens of each expert)
 variable_list router_balance_loss(const std::vector<at::Tensor>& logits, const std::vector<at::Tensor>& idx,
                                   const OptTensor& mask, double balance, double zcoef) {
+  for (const at::Tensor& x : logits) refuse_tangents("router_balance_loss", {x});
   return RouterBalanceFn::apply(at::TensorList(logits), idx, mask, balance, zcoef);
 }
 

@@ -245,3 +245,34 @@ def test_gradients_are_not_differentiated_again():
             assert torch.equal(a, b)
             with pytest.raises(RuntimeError, match="differentiated again"):
                 b.float().sum().backward()
+
+
+@GPU
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", ["hidden", "weight", "pref_logps", "pref_ref", "logps", "old", "advantages", "ref",
+                                   "router"])
+def test_forward_mode_is_refused(which, grad):
+    """A tangent on any input raises; it is never dropped, whether gradients are on or off."""
+    import torch.autograd.forward_ad as fw
+
+    from pluggy_b200.ops import linear_token_logprobs, policy_loss, preference_loss, router_balance_loss
+
+    m = torch.ones(2, 3, 40, dtype=torch.bool, device="cuda")
+    x, a = torch.randn(2, 3, 40, device="cuda"), torch.ones(3, device="cuda")
+    h, w = torch.randn(5, 64, device="cuda"), torch.randn(30, 64, device="cuda")
+    y = torch.zeros(5, dtype=torch.int64, device="cuda")
+
+    def dual(t):
+        return fw.make_dual(t, torch.ones_like(t))
+
+    run = {"hidden": lambda: linear_token_logprobs(dual(h), w, y),
+           "weight": lambda: linear_token_logprobs(h, dual(w), y),
+           "pref_logps": lambda: preference_loss(dual(x), None, m),
+           "pref_ref": lambda: preference_loss(x, dual(x), m),
+           "logps": lambda: policy_loss(dual(x[0]), None, a, m[0]),
+           "old": lambda: policy_loss(x[0], dual(x[0]), a, m[0]),
+           "advantages": lambda: policy_loss(x[0], None, dual(a), m[0]),
+           "ref": lambda: policy_loss(x[0], None, a, m[0], ref_logps=dual(x[0])),
+           "router": lambda: router_balance_loss(dual(h), torch.zeros(5, 2, dtype=torch.int64, device="cuda"))}
+    with fw.dual_level(), torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+        run[which]()
