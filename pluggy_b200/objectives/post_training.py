@@ -6,6 +6,9 @@ Both read per-token log-probabilities of the model's own head
 right-padded: under causal attention nothing before the padding sees it, so the packed
 forward serves them, and padded positions carry ``ignore_index`` labels.
 
+The data sources of the trainer make no such batches, so its config check refuses these
+objectives: a program calls them from its own loop (``examples/post_training.py``).
+
 ``score(model, ...)`` gives the same log-probabilities without gradients: the reference
 model's, or the policy's before its update.
 """
@@ -63,6 +66,7 @@ class PreferenceObjective:
     ``metrics`` holds the last call's mean rewards and the share of pairs ranked right."""
 
     KEYS = ("chosen_ids", "chosen_labels", "rejected_ids", "rejected_labels")
+    batch_keys = KEYS  # what every batch must hold
 
     def __init__(self, ignore_index: int = -100, beta: float = 0.1, kind: str = "sigmoid",
                  label_smoothing: float = 0.0, length_normalized: bool = False,
@@ -108,6 +112,8 @@ class PolicyObjective:
     [R, S] entries belong to the position that predicts the token, as :meth:`score` gives them.
     ``metrics`` holds the last call's loss, KL estimate and clipped share."""
 
+    batch_keys = ("input_ids", "labels", "advantages")  # what every batch must hold
+
     def __init__(self, ignore_index: int = -100, clip_low: float = 0.2, clip_high: float = 0.2,
                  kl_coef: float = 0.0, reduction: str = "token", temperature: float = 1.0):
         self.ignore_index, self.clip_low, self.clip_high = ignore_index, clip_low, clip_high
@@ -122,8 +128,7 @@ class PolicyObjective:
                               self.temperature)[0]
 
     def compute_loss(self, model: nn.Module, batch: dict[str, torch.Tensor]) -> torch.Tensor:
-        _need(batch, ("input_ids", "labels", "advantages") + (("ref_logps",) if self.kl_coef else ()),
-              "POLICY")
+        _need(batch, self.batch_keys + (("ref_logps",) if self.kl_coef else ()), "POLICY")
         lp, mask = token_logprobs(model, batch["input_ids"], batch["labels"], self.ignore_index,
                                   self.temperature)
         loss, kl, clipped = policy_loss(

@@ -10,6 +10,8 @@ from __future__ import annotations
 
 import inspect
 
+# what the data sources put into a batch
+LOADER_KEYS = ("input_ids", "labels")
 REQUIRED_TOP = ("model", "mesh", "optimizer", "objective", "data", "run_name")
 
 
@@ -79,9 +81,14 @@ def validate_config(cfg: dict) -> None:
     if ob.get("name") not in OBJECTIVE_REGISTRY:
         errs.append(f"objective.name {ob.get('name')!r} not in {sorted(OBJECTIVE_REGISTRY)}")
     else:
-        e = kwarg_error(OBJECTIVE_REGISTRY[ob["name"]], ob.get("config", {}), "objective.config")
+        cls = OBJECTIVE_REGISTRY[ob["name"]]
+        e = kwarg_error(cls, ob.get("config", {}), "objective.config")
         if e:
             errs.append(e)
+        more = sorted(set(getattr(cls, "batch_keys", LOADER_KEYS)) - set(LOADER_KEYS))
+        if more:
+            errs.append(f"objective.name {ob['name']!r} needs batches with {more}, which no data source "
+                        "makes: call the objective from a training loop of your own")
     d = cfg["data"]
     for k in ("global_batch_size", "micro_batch_size", "seq_len"):
         if not isinstance(d.get(k), int) or d[k] < 1:

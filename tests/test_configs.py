@@ -42,3 +42,15 @@ def test_cuda_graph_key_is_checked():
         c = dict(cfg, **bad)
         with pytest.raises(ConfigError, match="cuda_graph"):
             validate_config(c)
+
+
+@pytest.mark.parametrize("name,config", [("PREFERENCE", {"reference_free": True}), ("PREFERENCE", {}), ("POLICY", {})])
+def test_objectives_without_a_data_source_are_refused(name, config):
+    """The data sources make input_ids and labels alone: a run would fail at its first step."""
+    from pluggy_b200.train.validate import ConfigError, validate_config
+
+    with open(os.path.join(ROOT, "configs", "qwen3_0.6b_ddp_synthetic.json")) as f:
+        cfg = json.load(f)
+    cfg["objective"] = {"name": name, "config": config}
+    with pytest.raises(ConfigError, match="data source"):
+        validate_config(cfg)
