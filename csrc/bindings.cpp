@@ -669,15 +669,17 @@ std::vector<at::Tensor> preference_fwd(const at::Tensor& logps, const c10::optio
   a.beta = static_cast<float>(beta);
   a.smoothing = static_cast<float>(smoothing);
   a.normalized = normalized;
-  at::Tensor out = at::empty({1}, logps.options()), rewards = at::empty({2, a.P}, logps.options()),
-             row_scale = at::empty({2, a.P}, logps.options());
+  // results are tensors of their own: views of one buffer could not be changed in place
+  at::Tensor loss = at::empty({}, logps.options()), chosen = at::empty({a.P}, logps.options()),
+             rejected = at::empty({a.P}, logps.options()), row_scale = at::empty({2, a.P}, logps.options());
   // workspace: partial sums, block losses, ticket
   const int64_t nb = plg::pref_blocks(a.P), np = 2LL * a.P * plg::pref_chunks(a.P, a.S);
   at::Tensor ws = at::empty({8 * (np + nb + 1)}, mask.options().dtype(at::kByte));
   char* w = static_cast<char*>(ws.data_ptr());
   plg::pref_forward(a, w, reinterpret_cast<double*>(w + 8 * np), reinterpret_cast<unsigned*>(w + 8 * (np + nb)),
-                    row_scale.data_ptr<float>(), out.data_ptr<float>(), rewards.data_ptr<float>(), cur_stream());
-  return {out.select(0, 0), rewards.select(0, 0), rewards.select(0, 1), row_scale};
+                    row_scale.data_ptr<float>(), loss.data_ptr<float>(), chosen.data_ptr<float>(),
+                    rejected.data_ptr<float>(), cur_stream());
+  return {loss, chosen, rejected, row_scale};
 }
 
 at::Tensor preference_bwd(const at::Tensor& mask, const at::Tensor& row_scale, const at::Tensor& gout) {
@@ -736,13 +738,15 @@ std::vector<at::Tensor> policy_fwd(const at::Tensor& logps, const c10::optional<
   at::Tensor ws = at::empty({16 * cb + 24 * sb + 4LL * a.R + 4}, mask.options().dtype(at::kByte));
   char* w = static_cast<char*>(ws.data_ptr());
   int* counts = reinterpret_cast<int*>(w + 16 * cb + 24 * sb);
-  at::Tensor out = at::empty({3}, logps.options()), grad;
+  at::Tensor loss = at::empty({}, logps.options()), kl = at::empty({}, logps.options()),
+             clipped = at::empty({}, logps.options()), grad;
   if (train) grad = at::empty(mask.sizes(), logps.options());
   plg::policy_forward(a, counts, w, reinterpret_cast<double*>(w + 16 * cb),
                       reinterpret_cast<unsigned*>(counts + a.R),
-                      train ? grad.data_ptr<float>() : nullptr, out.data_ptr<float>(), cur_stream());
-  if (!train) return {out.select(0, 0), out.select(0, 1), out.select(0, 2)};
-  return {out.select(0, 0), out.select(0, 1), out.select(0, 2), grad};
+                      train ? grad.data_ptr<float>() : nullptr, loss.data_ptr<float>(), kl.data_ptr<float>(),
+                      clipped.data_ptr<float>(), cur_stream());
+  if (!train) return {loss, kl, clipped};
+  return {loss, kl, clipped, grad};
 }
 
 void scale_unless_one_b(at::Tensor& x, const at::Tensor& s) {

@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(256) pref_pairs_kernel(const PrefArgs a, const
                                                          unsigned* __restrict__ ticket,
                                                          float* __restrict__ row_scale,
                                                          float* __restrict__ loss,
-                                                         float* __restrict__ rewards) {
+                                                         float* __restrict__ chosen,
+                                                         float* __restrict__ rejected) {
   __shared__ double s_loss[8];
   __shared__ bool s_last;
   dependency_wait();
@@ -171,8 +172,8 @@ __global__ void __launch_bounds__(256) pref_pairs_kernel(const PrefArgs a, const
       const float c = d / static_cast<float>(a.P);
       row_scale[i] = c * inv[0];
       row_scale[a.P + i] = -c * inv[1];
-      rewards[i] = static_cast<float>(a.beta * s[0]);
-      rewards[a.P + i] = static_cast<float>(a.beta * s[1]);
+      chosen[i] = static_cast<float>(a.beta * s[0]);
+      rejected[i] = static_cast<float>(a.beta * s[1]);
       acc += l;
     }
   }
@@ -324,7 +325,8 @@ __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const Poli
                                                      const longlong2* __restrict__ block_counts, int nblocks,
                                                      double* __restrict__ block_sums,
                                                      unsigned* __restrict__ ticket, float* __restrict__ grad,
-                                                     float* __restrict__ out, int chunks, int len) {
+                                                     float* __restrict__ loss_out, float* __restrict__ kl_out,
+                                                     float* __restrict__ clipped_out, int chunks, int len) {
   __shared__ long long s_cnt[2][8];
   __shared__ double s_sum[3][8];
   __shared__ bool s_last;
@@ -447,7 +449,10 @@ __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const Poli
     double t = 0.0;
     for (int b = lane; b < gridDim.x; b += 32) t += static_cast<volatile double*>(block_sums)[b * 3 + warp];
     t = warp_sum_d(t);
-    if (lane == 0) out[warp] = static_cast<float>(warp == 0 ? t : t * inv_tokens);
+    if (lane == 0) {
+      if (warp == 0) *loss_out = static_cast<float>(t);
+      else *(warp == 1 ? kl_out : clipped_out) = static_cast<float>(t * inv_tokens);
+    }
   }
 }
 
@@ -916,7 +921,7 @@ int pref_chunks(int P, int S) { return chunks_of(2LL * P, S); }
 int pref_blocks(int P) { return std::max(1, std::min((P + 7) / 8, 148)); }
 
 void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* ticket, float* row_scale,
-                  float* loss, float* rewards, cudaStream_t st) {
+                  float* loss, float* chosen, float* rejected, cudaStream_t st) {
   if (a.P <= 0) return;
   const int chunks = pref_chunks(a.P, a.S), len = warp_tokens(2LL * a.P, a.S);
   const bool vec = a.S % 4 == 0 && aligned4(a.logps, 4, {a.lp_side, a.lp_pair}) &&
@@ -927,7 +932,7 @@ void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* t
   else pref_sums_kernel<1><<<grid, 256, 0, st>>>(a, static_cast<float2*>(part), chunks, len, ticket);
   PLG_CUDA_CHECK(cudaGetLastError());
   launch_dependent(pref_pairs_kernel, pref_blocks(a.P), 256, st, a, static_cast<const float2*>(part), chunks,
-                   block_loss, ticket, row_scale, loss, rewards);
+                   block_loss, ticket, row_scale, loss, chosen, rejected);
 }
 
 void pref_backward(const PrefArgs& a, const float* row_scale, const float* gout, float* grad, cudaStream_t st) {
@@ -951,7 +956,7 @@ int policy_blocks(int R, int S) {
 }
 
 void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double* block_sums,
-                    unsigned* ticket, float* grad, float* out, cudaStream_t st) {
+                    unsigned* ticket, float* grad, float* loss, float* kl, float* clipped, cudaStream_t st) {
   if (a.R <= 0) return;
   const int cb = policy_count_blocks(a.R, a.S);
   longlong2* bc = static_cast<longlong2*>(block_counts);
@@ -967,7 +972,7 @@ void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double
   auto launch = [&](auto old, auto ref, auto adv) {
     auto kern = vec ? policy_kernel<4, old.value, ref.value, adv.value>
                     : policy_kernel<1, old.value, ref.value, adv.value>;
-    launch_dependent(kern, grid, 256, st, a, counts, bc, cb, block_sums, ticket, grad, out, chunks, len);
+    launch_dependent(kern, grid, 256, st, a, counts, bc, cb, block_sums, ticket, grad, loss, kl, clipped, chunks, len);
   };
   auto pick = [&](auto old, auto ref) {
     if (a.adv_tok) launch(old, ref, std::true_type{});

@@ -232,9 +232,9 @@ struct PrefArgs {
 };
 int pref_chunks(int P, int S);  // part holds float2 [2 * P * chunks]
 int pref_blocks(int P);         // block_loss holds that many doubles
-// row_scale [2, P] = d loss / d logps of each row's tokens; rewards [2, P] = beta * sums
+// row_scale [2, P] = d loss / d logps of each row's tokens; chosen, rejected [P] = beta * sums
 void pref_forward(const PrefArgs& a, void* part, double* block_loss, unsigned* ticket, float* row_scale,
-                  float* loss, float* rewards, cudaStream_t stream);
+                  float* loss, float* chosen, float* rejected, cudaStream_t stream);
 void pref_backward(const PrefArgs& a, const float* row_scale, const float* gout, float* grad,
                    cudaStream_t stream);
 
@@ -260,9 +260,9 @@ struct PolicyArgs {
 };
 int policy_count_blocks(int R, int S);  // block_counts holds that many (2 x int64)
 int policy_blocks(int R, int S);        // block_sums holds 3 doubles for each
-// grad [R, S] (optional) = d loss / d logps; out [3] = loss, mean KL, clipped share
+// grad [R, S] (optional) = d loss / d logps; kl = mean KL, clipped = share of the tokens
 void policy_forward(const PolicyArgs& a, int* counts, void* block_counts, double* block_sums,
-                    unsigned* ticket, float* grad, float* out, cudaStream_t stream);
+                    unsigned* ticket, float* grad, float* loss, float* kl, float* clipped, cudaStream_t stream);
 void scale_unless_one(float* x, long long n, const float* s, cudaStream_t stream);
 
 // Balance and z loss of L routers over [T, E] logits (row stride ld[l], columns contiguous)

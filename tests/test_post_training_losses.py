@@ -567,3 +567,27 @@ def test_policy_zero_advantage_and_overflowing_ratio(per_token, dev):
     bad = old.clone()
     bad[0, 1] = float("nan")
     assert torch.isnan(policy_loss(lp, bad, adv, mask)[0])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("op", ["preference", "policy", "router"])
+def test_results_may_be_changed_in_place(op, grad, dev):
+    """`loss /= n`, `loss += aux` and the like, as on any other tensor."""
+    m = torch.ones(2, 3, 40, dtype=torch.bool, device=dev)
+    z = torch.randn(2, 3, 40, generator=gen_for(5)).to(dev)
+    run = {"preference": lambda x: preference_loss(x, None, m),
+           "policy": lambda x: policy_loss(x[0], None, torch.ones(3, device=dev), m[0]),
+           "router": lambda x: router_balance_loss(x[0], torch.zeros(3, 2, dtype=torch.int64, device=dev))}[op]
+    x = z.clone().requires_grad_(grad)
+    want = run(x)
+    got = run(x)
+    loss = got[0]
+    loss /= 4
+    loss += 1
+    for a, b in zip(got[1:], want[1:]):
+        a *= 2
+        assert torch.equal(a, 2 * b)
+    assert torch.equal(loss, want[0] / 4 + 1)
+    if grad:
+        assert torch.equal(4 * torch.autograd.grad(loss, x)[0], torch.autograd.grad(want[0], x)[0])
