@@ -429,7 +429,8 @@ int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 // Log-probabilities of labels [T] under hidden [T, D] (bf16 or fp32) and w [V, D] (bf16).
 // Returns {out}, or with train {out, h, ints, stats, x}: packed rows h [R, D], ints int32
 // [2 T + 3] (row_map, inverse, {rows, flag, splits}), stats fp32 [3, R] (lse2, label_grad,
-// ref) and, if keep, x bf16 [R, V] (else undefined).
+// ref) and, if keep, x bf16 [R, V rounded up to 8] (else undefined): whole, so that saved-tensor
+// hooks, which may pack its rows, leave them 16-byte aligned.
 std::vector<c10::optional<at::Tensor>> token_logprobs_fwd(const at::Tensor& hidden, const at::Tensor& w,
                                                           const at::Tensor& labels, int64_t ignore_index,
                                                           double softcap, double temperature, bool pack,
@@ -461,7 +462,7 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_fwd(const at::Tensor& hidd
       stats = at::empty({3, R}, f32);
       sp = stats.data_ptr<float>();
     }
-    if (keep) x = at::empty({R, round_up(V, 8)}, b16).narrow(1, 0, V);
+    if (keep) x = at::empty({R, round_up(V, 8)}, b16);
   } else {
     h = is_bf16(hidden) ? hidden : hidden.to(at::kBFloat16);
   }

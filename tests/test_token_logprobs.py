@@ -421,3 +421,21 @@ def test_kernel_label_entries_are_not_rounded(T, D, V, keep, monkeypatch, status
                  + 2.0 ** -14 * (A.t() @ H.abs()) + 1e-6)
     assert ((dh - rdh).abs() <= tol_h).all()
     assert ((dw - rdw).abs() <= tol_w).all()
+
+
+@GPU
+@pytest.mark.parametrize("V", [904, 901])
+@pytest.mark.parametrize("keep", [True, False])
+def test_kernel_saved_tensors_on_the_host(V, keep, monkeypatch, status):
+    """Saved-tensor hooks that hand back contiguous copies, vocabularies of no whole 16 bytes too."""
+    from pluggy_b200.ops import logprob
+
+    monkeypatch.setattr(logprob, "KEEP_PRODUCT", 0 if keep else 1 << 62)
+    h, w, y, g = make(300, 64, V, "cuda")
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    want = torch.autograd.grad(linear_token_logprobs(h, w, y), (h, w), g)
+    with torch.autograd.graph.save_on_cpu():
+        lp = linear_token_logprobs(h, w, y)
+    for a, b in zip(torch.autograd.grad(lp, (h, w), g), want):
+        assert torch.equal(a, b)
