@@ -883,7 +883,9 @@ struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
                             double temperature, bool keep, int64_t workspace, int64_t split_workspace,
                             const at::Tensor& status) {
     auto r = token_logprobs_fwd(hidden, w, labels, ignore_index, softcap, temperature, true, true, keep, status);
-    ctx->save_for_backward({w, labels, *r[1], *r[2], *r[3], r[4].has_value() ? *r[4] : at::Tensor(), status});
+    ctx->save_for_backward({w, labels, *r[1], *r[2], *r[3], r[4].has_value() ? *r[4] : at::Tensor()});
+    // the word itself, past the saved-tensor hooks: the backward's kernels report into it
+    ctx->saved_data["status"] = status;
     ctx->saved_data["softcap"] = softcap;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["workspace"] = workspace;
@@ -898,7 +900,8 @@ struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
                                 g[0].contiguous(), ctx->saved_data["softcap"].toDouble(),
                                 ctx->saved_data["temperature"].toDouble(), ctx->saved_data["workspace"].toInt(),
                                 ctx->saved_data["split_workspace"].toInt(), f32 & 1, f32 >> 1 & 1,
-                                ctx->needs_input_grad(0), ctx->needs_input_grad(1), s[6]);
+                                ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                ctx->saved_data["status"].toTensor());
     variable_list out(11);
     if (r[0].has_value()) out[0] = *r[0];
     if (r[1].has_value()) out[1] = *r[1];

@@ -439,3 +439,21 @@ def test_kernel_saved_tensors_on_the_host(V, keep, monkeypatch, status):
         lp = linear_token_logprobs(h, w, y)
     for a, b in zip(torch.autograd.grad(lp, (h, w), g), want):
         assert torch.equal(a, b)
+
+
+@GPU
+def test_kernel_status_word_is_not_a_saved_tensor(status):
+    """Saved-tensor hooks would hand the backward a copy, and its reports would be lost."""
+    from pluggy_b200.ops._ext import status_word
+
+    h, w, y, g = make(300, 64, 90, "cuda")
+    seen = []
+
+    def pack(t):
+        seen.append(t.data_ptr())
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        lp = linear_token_logprobs(h.requires_grad_(True), w, y)
+    assert seen and status_word().data_ptr() not in seen
+    torch.autograd.grad(lp, h, g)
