@@ -696,8 +696,10 @@ __global__ void __launch_bounds__(kRouterThreads, kRouterSumsResident) router_su
       z += s_z[w];
       n += s_kept[w];
     }
-    part_z[blockIdx.x * 2] = s_bad ? __longlong_as_double(0x7ff8000000000000LL) : z;
-    part_z[blockIdx.x * 2 + 1] = static_cast<double>(n);
+    part_z[blockIdx.x * 2] = z;
+    // a NaN marks a chosen index outside [0, E): all fractions, so the loss and the gradient of
+    // every kept row, become NaN with it
+    part_z[blockIdx.x * 2 + 1] = s_bad ? __longlong_as_double(0x7ff8000000000000LL) : static_cast<double>(n);
   }
 }
 
@@ -751,7 +753,7 @@ __global__ void __launch_bounds__(1024) router_join_kernel(const float* __restri
     k = warp_sum_d(k);
     if (lane == 0) {
       s_tot[0] = z;
-      s_tot[1] = k > 0.0 ? k : 1.0;
+      s_tot[1] = k == 0.0 ? 1.0 : k;
     }
   }
   __syncthreads();
@@ -781,9 +783,7 @@ __global__ void __launch_bounds__(1024) router_join_kernel(const float* __restri
     __threadfence();
     double t = 0.0;
     for (int b = 0; b < gridDim.x; ++b) t += static_cast<volatile double*>(dots)[b];
-    // NaN in s_tot[0] marks a chosen index outside [0, E)
-    const bool bad = !(s_tot[0] == s_tot[0]);
-    *loss = static_cast<float>(balance * E * t + (zcoef != 0.f || bad ? zcoef * s_tot[0] / tokens : 0.0));
+    *loss = static_cast<float>(balance * E * t + (zcoef != 0.f ? zcoef * s_tot[0] / tokens : 0.0));
     slope[E] = static_cast<float>(2.0 * zcoef / tokens);
   }
 }

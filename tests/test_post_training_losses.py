@@ -591,3 +591,26 @@ def test_results_may_be_changed_in_place(op, grad, dev):
     assert torch.equal(loss, want[0] / 4 + 1)
     if grad:
         assert torch.equal(4 * torch.autograd.grad(loss, x)[0], torch.autograd.grad(want[0], x)[0])
+
+
+@GPU
+@pytest.mark.parametrize("cb,cz", [(0.5, 0.1), (0.5, 0.0), (0.0, 0.1)])
+def test_router_index_outside_has_no_finite_gradient(cb, cz):
+    """The fractions are unknown then: NaN in the loss and in every kept row's gradient. NaN logits
+    stay in their own row."""
+    xs, idx, mask = router_inputs(2, 300, 60, 2, "cuda", torch.bfloat16, True)
+    mask[5], mask[6] = True, False
+    idx[1][5, 0] = 60
+    for x in xs:
+        x.requires_grad_(True)
+    loss, _ = router_balance_loss(xs, idx, balance_coef=cb, z_coef=cz, mask=mask)
+    assert torch.isnan(loss)
+    for g in torch.autograd.grad(loss, xs):
+        assert torch.isnan(g[mask]).all() and (g[~mask] == 0).all()
+    idx[1][5, 0] = 0
+    xs = [x.detach().clone() for x in xs]
+    xs[0][5, 3] = float("nan")
+    for x in xs:
+        x.requires_grad_(True)
+    a, b = torch.autograd.grad(router_balance_loss(xs, idx, balance_coef=cb, z_coef=cz, mask=mask)[0], xs)
+    assert torch.isnan(a[5]).all() and torch.isfinite(b).all() and torch.isfinite(a).sum() == a.numel() - 60
