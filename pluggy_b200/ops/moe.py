@@ -92,13 +92,15 @@ def router_balance_loss_reference(router_logits, top_indices, balance_coef=1.0, 
         keep = mask.repeat(len(router_logits)).nonzero().squeeze(1)
         x, idx = x[keep], idx[keep]
     n = max(1, x.shape[0])
-    counts = expert_histogram(idx, E)
+    inside = (idx >= 0) & (idx < E)
+    counts = expert_histogram(idx[inside], E)
     lse = torch.logsumexp(x, dim=-1)
     probs = torch.exp(x - lse.unsqueeze(1))
     loss = balance_coef * E * (counts / n * probs.sum(0) / n).sum()
     if z_coef:
         loss = loss + z_coef * lse.square().sum() / n
-    return loss, counts
+    # the fractions are unknown where a choice lies outside: NaN, in the gradient too
+    return (loss if inside.all() else loss * float("nan")), counts
 
 
 def router_balance_loss(router_logits, top_indices, *, balance_coef: float = 1.0, z_coef: float = 0.0,
@@ -113,8 +115,8 @@ def router_balance_loss(router_logits, top_indices, *, balance_coef: float = 1.0
         loss = balance_coef * E * sum_e (counts[e] / n) * mean(p[:, e]) + z_coef * mean(logsumexp^2)
 
     Returns ``(loss, counts int64 [E])``; the gradient goes to the logits (the counts are
-    constants, as in the models' auxiliary loss). An index outside [0, E) makes the loss NaN. On
-    CUDA at most 128 layers of 1024 experts in one call.
+    constants, as in the models' auxiliary loss). An index outside [0, E) is not counted and makes
+    the loss and the gradient of every kept row NaN. On CUDA at most 128 layers of 1024 experts in one call.
 
     CUDA path (csrc/objective.cu): all layers in one launch that keeps a row's probabilities
     in registers and writes only its log-sum-exp, one small kernel for the loss, one launch

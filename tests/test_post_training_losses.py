@@ -614,3 +614,22 @@ def test_router_index_outside_has_no_finite_gradient(cb, cz):
         x.requires_grad_(True)
     a, b = torch.autograd.grad(router_balance_loss(xs, idx, balance_coef=cb, z_coef=cz, mask=mask)[0], xs)
     assert torch.isnan(a[5]).all() and torch.isfinite(b).all() and torch.isfinite(a).sum() == a.numel() - 60
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bad", [60, -1, 1 << 40])
+def test_router_index_outside_on_every_device(bad, dev):
+    xs, idx, mask = router_inputs(2, 100, 60, 2, dev, torch.float32, True)
+    mask[5], mask[6] = True, False
+    want = router_balance_loss(xs, idx, mask=mask)[1].clone()
+    want[idx[0][5, 1]] -= 1
+    idx[0][5, 1] = bad
+    idx[0][6, 1] = bad  # of a masked token: not looked at
+    for x in xs:
+        x.requires_grad_(True)
+    loss, counts = router_balance_loss(xs, idx, z_coef=0.1, mask=mask)
+    assert torch.isnan(loss) and torch.equal(counts, want)
+    for g in torch.autograd.grad(loss, xs):
+        assert torch.isnan(g[mask]).all() and (g[~mask] == 0).all()
+    idx[0][5, 1] = 0
+    assert torch.isfinite(router_balance_loss(xs, idx, z_coef=0.1, mask=mask)[0])
