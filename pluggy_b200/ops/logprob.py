@@ -43,14 +43,17 @@ UNPACKED_ROWS = 256
 
 def token_logprobs_reference(hidden, weight, labels, ignore_index=-100, softcap=None,
                              temperature=1.0):
-    """fp32 math in eager torch on [T, D] rows; ignored rows take no part in the graph."""
-    keep = (labels != ignore_index).nonzero().squeeze(1)
+    """fp32 math in eager torch on [T, D] rows; ignored rows and those whose label is outside the
+    vocabulary (NaN) take no part in the graph."""
+    outside = (labels != ignore_index) & ((labels < 0) | (labels >= weight.shape[0]))
+    keep = ((labels != ignore_index) & ~outside).nonzero().squeeze(1)
     z = hidden[keep].float() @ weight.float().t()
     if softcap:
         z = torch.tanh(z / softcap) * softcap
     z = z / temperature
     lp = z.gather(1, labels[keep].unsqueeze(1)).squeeze(1) - torch.logsumexp(z, dim=-1)
-    return torch.zeros(labels.shape, dtype=torch.float32, device=hidden.device).index_put((keep,), lp)
+    out = torch.zeros(labels.shape, dtype=torch.float32, device=hidden.device)
+    return out.masked_fill_(outside, float("nan")).index_put((keep,), lp)
 
 
 def _rows_aligned(t: torch.Tensor) -> torch.Tensor:

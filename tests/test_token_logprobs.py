@@ -457,3 +457,18 @@ def test_kernel_status_word_is_not_a_saved_tensor(status):
         lp = linear_token_logprobs(h.requires_grad_(True), w, y)
     assert seen and status_word().data_ptr() not in seen
     torch.autograd.grad(lp, h, g)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+def test_label_outside_is_nan_on_every_device(dev):
+    h, w, _, g = make(6, 16, 9, dev, dtype=torch.float32)
+    y = torch.tensor([0, 9, -3, IGN, 8, 1 << 40], device=dev)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    lp = linear_token_logprobs(h, w, y)
+    assert torch.isnan(lp[[1, 2, 5]]).all() and torch.isfinite(lp[[0, 3, 4]]).all() and lp[3] == 0
+    dh, dw = torch.autograd.grad(lp, (h, w), g)
+    assert (dh[[1, 2, 3, 5]] == 0).all() and torch.isfinite(dh).all() and torch.isfinite(dw).all()
+    assert (dh[[0, 4]] != 0).any(1).all()
+    # ignore_index may be a vocabulary entry
+    assert (linear_token_logprobs(h, w, y, ignore_index=8)[4] == 0)
