@@ -57,8 +57,9 @@ def token_logprobs_reference(hidden, weight, labels, ignore_index=-100, softcap=
 
 
 def _rows_aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` or a copy whose rows start on 16-byte boundaries (what the TMA loads need)."""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+    """``t`` or a copy whose rows start on 16-byte boundaries and do not overlap, as those of an
+    expanded row do (what the TMA loads need)."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -472,3 +472,33 @@ def test_label_outside_is_nan_on_every_device(dev):
     assert (dh[[0, 4]] != 0).any(1).all()
     # ignore_index may be a vocabulary entry
     assert (linear_token_logprobs(h, w, y, ignore_index=8)[4] == 0)
+
+
+def test_overlapping_rows_are_copied():
+    """Rows expanded from one and sliding windows: their stride is no row stride of a tensor map."""
+    from pluggy_b200.ops.logprob import _rows_aligned
+
+    x = torch.randn(1, 64)
+    for t in (x.expand(5, 64), x.view(-1).as_strided((4, 32), (8, 1)), x.view(8, 8).t()):
+        c = _rows_aligned(t)
+        assert c.is_contiguous() and torch.equal(c, t)
+    y = torch.randn(6, 128)[:, :64]
+    assert _rows_aligned(y) is y or y.data_ptr() % 16
+
+
+@GPU
+@pytest.mark.parametrize("T", [1, 5, 200, 300])
+def test_kernel_overlapping_rows(T, status):
+    """Hidden rows expanded from one, a sliding window over one buffer, one weight row for all."""
+    h, w, y, g = make(T, 64, 500, "cuda", ignored=0.0)
+    for hv in (h[:1].expand(T, 64), h.new_empty(8 * T + 56).copy_(torch.randn(8 * T + 56)).as_strided((T, 64), (8, 1))):
+        lp = linear_token_logprobs(hv, w, y)
+        assert torch.equal(lp, linear_token_logprobs(hv.contiguous(), w, y))
+        ref, *_, bound = exact(hv.contiguous(), w, y, g)
+        assert ((lp - ref).abs() <= 2.0 ** -22 * 8 * bound + 2.0 ** -20 * ref.abs()).all()
+        a, b = hv.detach().requires_grad_(True), hv.contiguous().requires_grad_(True)
+        (da,) = torch.autograd.grad(linear_token_logprobs(a, w, y), a, g)
+        (db,) = torch.autograd.grad(linear_token_logprobs(b, w, y), b, g)
+        assert torch.equal(da, db)
+    lp = linear_token_logprobs(h, w[:1].expand(500, 64), y)
+    assert ((lp + torch.log(torch.tensor(500.0))).abs() <= 2.0 ** -22 * 8 * bound + 2.0 ** -20 * 7).all()
