@@ -24,6 +24,8 @@ hidden rows reach no output.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from pluggy_b200.ops._ext import ext, status_word
@@ -88,8 +90,8 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: to
     if labels.shape != hidden.shape[:-1] or labels.dtype != torch.int64:
         raise ValueError(f"linear_token_logprobs: labels must be int64 {tuple(hidden.shape[:-1])}, got "
                          f"{labels.dtype} {tuple(labels.shape)}")
-    if not temperature > 0 or (softcap is not None and softcap < 0):
-        raise ValueError("linear_token_logprobs: temperature must be positive, softcap not negative")
+    if not temperature > 0 or (softcap is not None and not 0 <= softcap < math.inf):
+        raise ValueError("linear_token_logprobs: temperature must be positive, softcap finite and not negative")
     if weight.shape[0] == 0:
         raise ValueError("linear_token_logprobs: an empty vocabulary")
     for name, t in (("hidden", hidden), ("weight", weight)):

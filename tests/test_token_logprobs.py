@@ -502,3 +502,12 @@ def test_kernel_overlapping_rows(T, status):
         assert torch.equal(da, db)
     lp = linear_token_logprobs(h, w[:1].expand(500, 64), y)
     assert ((lp + torch.log(torch.tensor(500.0))).abs() <= 2.0 ** -22 * 8 * bound + 2.0 ** -20 * 7).all()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("softcap", [float("nan"), float("inf")])
+def test_softcap_that_is_no_number_is_refused(softcap, dev):
+    """NaN read as no softcap on CUDA, infinity as 0 * inf."""
+    h, w, y, _ = make(3, 16, 9, dev, dtype=torch.float32)
+    with pytest.raises(ValueError, match="softcap"):
+        linear_token_logprobs(h, w, y, softcap=softcap)
