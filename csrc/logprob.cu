@@ -21,10 +21,12 @@
 //   X[t, v] = bf16(2^(z log2e - r_t) * softcap'(a)),   r_t = z[t, y_t] log2e + 40
 // with a reference r_t that one dot product gives beforehand, and the backward pass folds c_t
 // = -(g_t / temperature) 2^(r_t - lse2_t) into the hidden rows (for dW) and into the result
-// (for dh). Since lse2 >= z_y log2e, the entries that matter lie above 2^-100 and below
-// 2^(-out log2e - 40): bf16's range holds them unless out < -97 or so. If any row is beyond
-// that, a flag in device memory makes the backward pass recompute. What it costs: c_t h_t is
-// rounded to bf16 (2^-8 of a term of dW other than the labels').
+// (for dh). Both factors have to lie in bf16's range, 2^-126 to 2^127. X's entries reach at most
+// 2^(-out log2e - 40), those of probability p are p times that, and c_t is g_t / temperature
+// divided by it: kept up to 2^60 (out > -69 or so) the entries of p > 2^-86 and the c_t h_t of
+// |g_t h_t| > 2^-66 are normal numbers. If any row is beyond that, a flag in device memory makes
+// the backward pass recompute. What it costs: c_t h_t is rounded to bf16 (2^-8 of a term of dW
+// other than the labels').
 //
 // Rows whose label is ignore_index are left out of the products: compact_kernel lists
 // the others on the device, gather_kernel packs their hidden rows, and every later kernel reads
@@ -57,7 +59,7 @@ constexpr int kSmemBytes = kStages * kMaxStageBytes + kEpiWarps * 2 * kBoxBytes 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRefOffset = 40.f;   // r_t - z_y log2e
-constexpr float kRefLimit = 100.f;   // lse2 - r_t beyond which X is recomputed
+constexpr float kRefLimit = 60.f;    // lse2 - r_t beyond which X is recomputed
 // Reduction length of one accumulator of the statistics: the tensor cores truncate each
 // addition, a bias of about 1e-9 of the sum per column of D (measured: 2.5e-6 of a logit at
 // D = 2560, 1e-6 at 1024; an fp32 chain's rounding is about 5e-7), so longer sums are cut

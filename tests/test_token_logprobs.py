@@ -511,3 +511,25 @@ def test_softcap_that_is_no_number_is_refused(softcap, dev):
     h, w, y, _ = make(3, 16, 9, dev, dtype=torch.float32)
     with pytest.raises(ValueError, match="softcap"):
         linear_token_logprobs(h, w, y, softcap=softcap)
+
+
+@GPU
+@pytest.mark.parametrize("far", [-95.0, -71.0, -67.0, -40.0])
+def test_kernel_unlikely_labels_with_small_gradients(far, kept, status):
+    """Labels at log-probability `far`, incoming gradients of 1e-8 and hidden values of 0.02: no
+    factor of dW leaves bf16's range, so that the bound holds relative to the terms. 1e-30 stands
+    for entries of probability below 1e-20."""
+    gen = torch.Generator().manual_seed(0)
+    T, D, V = 300, 64, 700
+    h = (0.02 * torch.randn(T, D, generator=gen)).bfloat16().cuda()
+    w = (156 * torch.randn(V, D, generator=gen)).bfloat16().cuda()
+    y = (torch.log_softmax(h.double() @ w.double().t(), 1) - far).abs().argmin(1)
+    g = torch.full((T,), 1e-8, device="cuda")
+    lp, rdh, rdw, bdh, bdw, _ = exact(h, w, y, g)
+    assert (lp.median() - far).abs() < 1  # near -40 single rows have no label this close
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    dh, dw = torch.autograd.grad(linear_token_logprobs(h, w, y), (h, w), g)
+    # 2^-14: G's own error in fp32 (logits of order 100 that are 1e-5 off)
+    assert ((dh - rdh).abs() <= (2.0 ** -7 + 2.0 ** -14) * bdh + 1e-30).all()
+    assert ((dw - rdw).abs() <= KEPT_DW * (2.0 ** -7 + 2.0 ** -14) * bdw + 1e-30).all()
