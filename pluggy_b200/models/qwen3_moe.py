@@ -14,7 +14,10 @@ Parity: reference ``pluggy/models/qwen3_moe/qwen3_moe.py:140-444``:
 * ``fused_router_losses=True`` (off by default) computes ``aux_loss()`` and the counts by
   :func:`pluggy_b200.ops.router_balance_loss`: the same formulas on the routers' own top-k
   choices (the default recomputes the top-k, which differs only where probabilities tie),
-  without the concatenated logits, and with padded tokens left out.
+  without the concatenated logits, and with the tokens that ``attention_mask`` pads left out;
+* ``forward(..., token_mask=...)`` (bool [B, S]) leaves tokens out of the auxiliary loss and the
+  counts, with either setting, without a say in the attention: right-padded batches keep the
+  packed forward.
 
 CUDA path: the attention sublayer is the fused ``_engine.AttnSublayer``; the
 sparse MLP composes this package's kernels (RMSNorm, router GEMM, one grouped
@@ -150,26 +153,44 @@ class Qwen3MoeTransformerBlock(Qwen3TransformerBlock):
         return x + self.ffn(h).float()
 
 
-def load_balancing_loss(router_logits, num_experts: int, top_k: int):
+def _masked_histogram(idx, n: int, keep):
+    """int64 [n]: how many entries of ``idx`` [T, k] in the rows where ``keep`` [T] holds equal each value."""
+    ones = keep.long().unsqueeze(1).expand_as(idx).reshape(-1)
+    return torch.zeros(n, dtype=torch.int64, device=idx.device).scatter_add_(0, idx.reshape(-1), ones)
+
+
+def load_balancing_loss(router_logits, num_experts: int, top_k: int, token_mask=None):
+    """``token_mask`` (bool [T], every layer's rows alike): the tokens that count (None: all)."""
     if not router_logits:
         return torch.tensor(0.0)
     logits = torch.cat([g.float() for g in router_logits], dim=0)
     probs = F.softmax(logits, dim=-1)
     _, top = torch.topk(probs, top_k, dim=-1)
+    if token_mask is not None:
+        keep = token_mask.repeat(len(router_logits))
+        n = keep.sum().clamp_min(1)
+        mean = torch.where(keep.unsqueeze(1), probs, 0.0).sum(dim=0) / n
+        return (_masked_histogram(top, num_experts, keep).float() / n * mean).sum() * num_experts
     # the reference's one_hot(top, E).mean(0) summed over the k slots: the fraction of
     # (token, slot) pairs routed to each expert, counted without the [T, k, E] one-hot
     frac = expert_histogram(top, num_experts).float() / top.shape[0]
     return (frac * probs.mean(dim=0)).sum() * num_experts
 
 
-def router_z_loss(router_logits):
+def router_z_loss(router_logits, token_mask=None):
     if not router_logits:
         return torch.tensor(0.0)
     logits = torch.cat([g.float() for g in router_logits], dim=0)
+    if token_mask is not None:
+        keep = token_mask.repeat(len(router_logits))
+        z = torch.square(torch.logsumexp(logits, dim=-1))
+        return torch.where(keep, z, 0.0).sum() / keep.sum().clamp_min(1)
     return torch.square(torch.logsumexp(logits, dim=-1)).mean()
 
 
 class Qwen3Moe(nn.Module):
+    takes_token_mask = True  # forward(token_mask=...)
+
     def __init__(self, num_layers: int, num_heads: int, num_kv_heads: int, emb_dim: int,
                  head_dim: int, vocab_size: int, moe_ffn_dim: int, num_experts: int = 128,
                  top_k: int = 8, ffn_dim: int | None = None, norm_topk_prob: bool = True,
@@ -201,6 +222,9 @@ class Qwen3Moe(nn.Module):
         if tie_embeddings:
             self.lm_head.weight = self.token_emb.weight
         self._router_logits: list[torch.Tensor] = []
+        # tokens that count in the router losses: forward's token_mask, and that with the
+        # padding mask, which the default losses do not read
+        self._loss_mask: torch.Tensor | None = None
         self._token_mask: torch.Tensor | None = None
         self.last_tokens_per_expert: torch.Tensor | None = None
         self.weight_cache = WeightCache()
@@ -249,7 +273,9 @@ class Qwen3Moe(nn.Module):
             for b in self.blocks:
                 idx = getattr(b.ffn, "last_top_idx", None) if isinstance(b.ffn, Qwen3MoeSparseMLP) \
                     else None
-                if idx is not None:
+                if idx is not None and self._loss_mask is not None:
+                    counts += _masked_histogram(idx, self.num_experts, self._loss_mask).float()
+                elif idx is not None:
                     counts += expert_histogram(idx, self.num_experts).float()
         self.last_tokens_per_expert = counts
 
@@ -267,20 +293,31 @@ class Qwen3Moe(nn.Module):
         loss = torch.zeros((), device=logits[0].device)
         if self.router_aux_loss_coef != 0.0:
             loss = loss + self.router_aux_loss_coef * load_balancing_loss(logits, self.num_experts,
-                                                                          self.top_k)
+                                                                          self.top_k, self._loss_mask)
         if self.router_z_loss_coef != 0.0:
-            loss = loss + self.router_z_loss_coef * router_z_loss(logits)
+            loss = loss + self.router_z_loss_coef * router_z_loss(logits, self._loss_mask)
         return loss
 
+    def _set_masks(self, x, attention_mask, token_mask) -> None:
+        self._loss_mask = self._token_mask = None
+        if token_mask is not None:
+            if token_mask.shape != x.shape or token_mask.dtype != torch.bool:
+                raise ValueError(f"token_mask must be bool {tuple(x.shape)}, got {token_mask.dtype} "
+                                 f"{tuple(token_mask.shape)}")
+            self._loss_mask = self._token_mask = token_mask.reshape(-1)
+        if attention_mask is not None:
+            am = attention_mask.bool().reshape(-1)
+            self._token_mask = am if token_mask is None else am & self._loss_mask
+
     def forward(self, x, attention_mask=None, return_hidden_states: bool = False,
-                return_final_hidden: bool = False, position_ids=None):
+                return_final_hidden: bool = False, position_ids=None, token_mask=None):
         for b in self.blocks:
             if isinstance(b.ffn, Qwen3MoeSparseMLP):
                 b.ffn.last_router_logits = None
                 b.ffn.last_top_idx = None
         self._router_logits = []
-        self._token_mask = None if attention_mask is None else attention_mask.bool().reshape(-1)
         B, S = x.shape
+        self._set_masks(x, attention_mask, token_mask)
         fused = (x.is_cuda and attention_mask is None and not return_hidden_states
                  and position_ids is None and getattr(self, "tp", None) is None
                  and getattr(self, "cp", None) is None

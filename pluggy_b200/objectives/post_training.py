@@ -4,7 +4,9 @@ Both read per-token log-probabilities of the model's own head
 (:func:`pluggy_b200.ops.linear_token_logprobs`, no logits in memory) and add the model's
 ``aux_loss()`` (MoE router losses) when it has one, as the AR objective does. Sequences are
 right-padded: under causal attention nothing before the padding sees it, so the packed
-forward serves them, and padded positions carry ``ignore_index`` labels.
+forward serves them, and padded positions carry ``ignore_index`` labels. What follows a
+sequence's last label is taken for padding and counts neither in the router losses nor in
+the experts' token counts (models with ``takes_token_mask``).
 
 The data sources of the trainer make no such batches, so its config check refuses these
 objectives: a program calls them from its own loop (``examples/post_training.py``).
@@ -24,6 +26,13 @@ from pluggy_b200.ops.policy import policy_loss
 from pluggy_b200.ops.preference import preference_loss
 
 
+def before_padding(labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+    """bool [B, S]: positions up to each row's last label."""
+    at = torch.arange(1, labels.shape[1] + 1, device=labels.device)
+    last = torch.where(labels != ignore_index, at, 0).amax(1, keepdim=True) if labels.shape[1] else at
+    return at <= last
+
+
 def token_logprobs(model: nn.Module, ids: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
                    temperature: float = 1.0):
     """``(logps [B, S] fp32, mask [B, S])``: position t holds the log-probability of ``labels[t + 1]``
@@ -36,7 +45,8 @@ def token_logprobs(model: nn.Module, ids: torch.Tensor, labels: torch.Tensor, ig
     if ids.shape != labels.shape or ids.dim() != 2:
         raise ValueError(f"ids and labels must be [B, S] alike, got {tuple(ids.shape)} and "
                          f"{tuple(labels.shape)}")
-    hidden = model(ids, return_final_hidden=True)
+    kw = {"token_mask": before_padding(labels, ignore_index)} if getattr(core, "takes_token_mask", False) else {}
+    hidden = model(ids, return_final_hidden=True, **kw)
     labels = shift_labels(labels, ignore_index)
     lowp_fn = getattr(core, "lm_head_lowp", None)
     lowp = lowp_fn() if callable(lowp_fn) and hidden.is_cuda else None

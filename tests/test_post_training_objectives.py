@@ -276,3 +276,82 @@ def test_forward_mode_is_refused(which, grad):
            "router": lambda: router_balance_loss(dual(h), torch.zeros(5, 2, dtype=torch.int64, device="cuda"))}
     with fw.dual_level(), torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
         run[which]()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("name", ["PREFERENCE", "POLICY"])
+def test_padding_does_not_reach_the_router_losses(name, fused, dev):
+    """The auxiliary loss, the routers' gradients and the experts' counts are those of the tokens
+    before the padding, of the same forward pass; on the CPU, where two passes agree, longer padding
+    and other ids in it leave them as they are."""
+    from pluggy_b200.models.qwen3_moe import load_balancing_loss, router_z_loss
+
+    lengths = [64, 40, 64, 10, 0, 33]
+    P, S = len(lengths) // 2, 64
+
+    def batch(total, pad):
+        g = torch.Generator().manual_seed(1)
+        ids, labels = torch.full((2 * P, total), pad), torch.full((2 * P, total), IGN)
+        full = torch.randint(0, 200, (2 * P, S), generator=g)
+        for i, n in enumerate(lengths):
+            ids[i, :n] = full[i, :n]
+            labels[i, 4:n] = full[i, 4:n]
+        if name == "POLICY":
+            out = {"input_ids": ids, "labels": labels, "advantages": torch.linspace(-1, 1, 2 * P)}
+        else:
+            out = {f"{side}_{k}": t[i * P:(i + 1) * P] for i, side in enumerate(("chosen", "rejected"))
+                   for k, t in (("ids", ids), ("labels", labels))}
+        return {k: t.to(dev) for k, t in out.items()}
+
+    m = small("qwen3_moe", dev, router_aux_loss_coef=0.1, router_z_loss_coef=0.01, fused_router_losses=fused)
+    obj = build_objective(name, dict(reference_free=True) if name == "PREFERENCE" else {})
+    got = []
+    for total, pad in ((S, 0), (2 * S, 0), (2 * S, 7)):
+        loss = obj.compute_loss(m, batch(total, pad))
+        aux = m.aux_loss()
+        assert abs(loss - obj.metrics["loss"] - aux) <= 1e-5 * loss.abs()
+        keep = (torch.arange(total)[None, :] < torch.tensor(lengths)[:, None]).reshape(-1).to(dev)
+        logits = [x[keep] for x in m._router_logits]
+        want = 0.1 * load_balancing_loss(logits, 32, 4) + 0.01 * router_z_loss(logits)
+        weights = [b.ffn.router.weight for b in m.blocks]
+        grads = torch.autograd.grad(aux, weights, retain_graph=True)
+        assert abs(aux - want) <= 2.0 ** -16 * want
+        for x, y in zip(grads, torch.autograd.grad(want, weights)):
+            # on the GPU the routers' logits, and so their gradients, are bf16
+            assert (x - y).norm() <= (2.0 ** -7 if dev == "cuda" else 1e-4) * y.norm()
+        got.append((aux.detach(), grads, m.last_tokens_per_expert))
+        assert got[-1][2].sum() == sum(lengths) * 4 * 2
+    for aux, grads, counts in got[1:] if dev == "cpu" else ():
+        assert abs(aux - got[0][0]) <= 1e-5 * got[0][0] and torch.equal(counts, got[0][2])
+        for x, y in zip(grads, got[0][1]):
+            assert (x - y).norm() <= 2e-5 * y.norm()
+
+
+def test_token_mask_argument():
+    """Checked against the ids; an all-true mask is no mask; nothing left gives 0."""
+    m = small("qwen3_moe", router_aux_loss_coef=0.1)
+    ids = torch.randint(0, 200, (2, 16), generator=torch.Generator().manual_seed(3))
+    with pytest.raises(ValueError, match="token_mask"):
+        m(ids, token_mask=torch.ones(2, 15, dtype=torch.bool))
+    with pytest.raises(ValueError, match="token_mask"):
+        m(ids, token_mask=torch.ones(2, 16))
+    m(ids)
+    want, counts = m.aux_loss(), m.last_tokens_per_expert
+    m(ids, token_mask=torch.ones(2, 16, dtype=torch.bool))
+    for fused in (False, True):
+        m.fused_router_losses = fused
+        assert abs(m.aux_loss() - want) <= 1e-5 * want
+        assert torch.equal(m.last_tokens_per_expert, counts)
+    m(ids, token_mask=torch.zeros(2, 16, dtype=torch.bool))
+    for fused in (False, True):
+        m.fused_router_losses = fused
+        assert m.aux_loss() == 0
+    # padding of the attention and of the losses together
+    am = torch.ones(2, 16, dtype=torch.long)
+    am[0, 12:] = 0
+    tm = torch.ones(2, 16, dtype=torch.bool)
+    tm[1, 10:] = False
+    m(ids, attention_mask=am, token_mask=tm)
+    m.aux_loss()
+    assert m.last_tokens_per_expert.sum() == (12 + 10) * 4 * 2
