@@ -533,3 +533,29 @@ def test_kernel_unlikely_labels_with_small_gradients(far, kept, status):
     # 2^-14: G's own error in fp32 (logits of order 100 that are 1e-5 off)
     assert ((dh - rdh).abs() <= (2.0 ** -7 + 2.0 ** -14) * bdh + 1e-30).all()
     assert ((dw - rdw).abs() <= KEPT_DW * (2.0 ** -7 + 2.0 ** -14) * bdw + 1e-30).all()
+
+
+@GPU
+@pytest.mark.parametrize("D", [1032, 2056, 2560])
+@pytest.mark.parametrize("softcap,tau", [(4.0, 0.6), (None, 1.0)])
+@pytest.mark.parametrize("keep", [False, True])
+def test_kernel_long_sums_with_softcap(D, softcap, tau, keep, monkeypatch, status):
+    """D above 1024: a logit is summed in several accumulator pieces (above 512 where at most 128
+    rows are scored), with and without a softcap, scoring and both gradients."""
+    from pluggy_b200.ops import logprob
+
+    monkeypatch.setattr(logprob, "KEEP_PRODUCT", 0 if keep else 1 << 62)
+    for T, V in ((300, 1500), (100, 700)):
+        check_case(*make(T, D, V, "cuda"), softcap, tau, dw_slack=KEPT_DW if keep else 1.0)
+
+
+@GPU
+@pytest.mark.parametrize("softcap,tau", [(4.0, 0.6), (None, 1.0)])
+@pytest.mark.parametrize("keep", [False, True])
+def test_kernel_many_tokens_of_wide_rows(softcap, tau, keep, monkeypatch, status):
+    """More tokens than the search through all labels takes (they are sorted), rows wider than a
+    block's 1024 columns."""
+    from pluggy_b200.ops import logprob
+
+    monkeypatch.setattr(logprob, "KEEP_PRODUCT", 0 if keep else 1 << 62)
+    check_case(*make(4500, 1288, 600, "cuda"), softcap, tau, dw_slack=KEPT_DW if keep else 1.0)
