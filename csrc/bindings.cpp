@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 #include <vector>
@@ -392,6 +393,10 @@ void router_topk_b(const at::Tensor& logits, int64_t k, bool renorm, const c10::
                    cur_stream());
 }
 
+// Kernels (memsets included) launched by the post-training operators, whose backward passes do not
+// come through a binding that could be counted
+std::atomic<int64_t> g_launches{0};
+
 // ---- token log-probabilities of a linear head
 const int64_t* labels_ptr(const at::Tensor& labels) {
   check_cuda(labels, "labels");
@@ -481,6 +486,7 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_fwd(const at::Tensor& hidd
                   keep ? x.stride(0) : 0, st);
   plg::head_join(p, part.data_ptr(), target, V, ignore_index, out.data_ptr<float>(), keep ? sp + 2 * R : nullptr,
                  sp, train ? sp + R : nullptr, pack ? ip + 2 * T + 1 : nullptr, st);
+  g_launches += pack ? 4 : 2;
   if (!train) return {out};
   return {out, h, ints, stats, keep ? c10::optional<at::Tensor>(x) : c10::nullopt};
 }
@@ -510,6 +516,7 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
   if (kept.has_value()) {
     x = *kept;
     plg::head_recompute(p, sp, g, count + 1, x.data_ptr(), x.stride(0), st);  // only if flagged
+    g_launches += 2;
     hs = at::empty_like(h);
     scale = at::empty({R}, f32);
     plg::head_scale_rows(p, sp, sp + 2 * R, g, x.data_ptr(), x.stride(0), scale.data_ptr<float>(), hs.data_ptr(),
@@ -537,9 +544,11 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
     plg::head_label_rows(p, sorted.defined() ? sorted.data_ptr<int>() : nullptr,
                          token.defined() ? token.data_ptr<int64_t>() : nullptr, ip + T, sp + R, g,
                          label_sums.data_ptr<float>(), label_row.data_ptr<int>(), static_cast<int>(T), st);
+    g_launches += 2;
   }
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int64_t n = std::min(width, V - v0);
+    g_launches += !kept.has_value() + need_h + need_w;
     if (!kept.has_value()) {
       plg::HeadProblem r = p;
       r.w = static_cast<const char*>(p.w) + 2 * v0 * p.ldw;
@@ -601,6 +610,7 @@ std::vector<c10::optional<at::Tensor>> token_logprobs_bwd(
     plg::head_scatter(p, dh_rows.data_ptr<float>(), R * D, count + 2,
                       kept.has_value() ? scale.data_ptr<float>() : nullptr, sp + R, g, ip + T, dh.data_ptr(), dh_f32,
                       T, st);
+    ++g_launches;
   }
   return {need_h ? c10::optional<at::Tensor>(dh) : c10::nullopt,
           need_w ? c10::optional<at::Tensor>(dw) : c10::nullopt};
@@ -680,6 +690,7 @@ std::vector<at::Tensor> preference_fwd(const at::Tensor& logps, const c10::optio
   plg::pref_forward(a, w, reinterpret_cast<double*>(w + 8 * np), reinterpret_cast<unsigned*>(w + 8 * (np + nb)),
                     row_scale.data_ptr<float>(), loss.data_ptr<float>(), chosen.data_ptr<float>(),
                     rejected.data_ptr<float>(), cur_stream());
+  g_launches += 2;
   return {loss, chosen, rejected, row_scale};
 }
 
@@ -689,6 +700,7 @@ at::Tensor preference_bwd(const at::Tensor& mask, const at::Tensor& row_scale, c
   at::Tensor grad = at::empty(mask.sizes(), row_scale.options());
   plg::pref_backward(a, float_ptr(row_scale, 2LL * a.P, "row_scale"), float_ptr(gout, 1, "gout"),
                      grad.data_ptr<float>(), cur_stream());
+  g_launches += grad.numel() > 0;
   return grad;
 }
 
@@ -746,6 +758,7 @@ std::vector<at::Tensor> policy_fwd(const at::Tensor& logps, const c10::optional<
                       reinterpret_cast<unsigned*>(counts + a.R),
                       train ? grad.data_ptr<float>() : nullptr, loss.data_ptr<float>(), kl.data_ptr<float>(),
                       clipped.data_ptr<float>(), cur_stream());
+  g_launches += 2;
   if (!train) return {loss, kl, clipped};
   return {loss, kl, clipped, grad};
 }
@@ -753,6 +766,7 @@ std::vector<at::Tensor> policy_fwd(const at::Tensor& logps, const c10::optional<
 void scale_unless_one_b(at::Tensor& x, const at::Tensor& s) {
   const c10::cuda::CUDAGuard guard(x.device());
   plg::scale_unless_one(float_ptr(x, x.numel(), "x"), x.numel(), float_ptr(s, 1, "s"), cur_stream());
+  g_launches += x.numel() > 0;
 }
 
 // the layers' logits and, for the forward, their indices; tensors that had to be copied are kept
@@ -826,6 +840,7 @@ std::vector<at::Tensor> router_balance_fwd(const std::vector<at::Tensor>& logits
                               reinterpret_cast<double*>(w), dp, reinterpret_cast<unsigned*>(dp + dots),
                               loss.data_ptr<float>(), counts.data_ptr<int64_t>(),
                               slope.data_ptr<float>(), cur_stream());
+  g_launches += 2;
   return {loss, counts, lse, slope};
 }
 
@@ -841,6 +856,7 @@ std::vector<at::Tensor> router_balance_bwd(const std::vector<at::Tensor>& logits
   plg::router_balance_backward(a, is_bf16(logits[0]), float_ptr(lse, a.L * a.T, "lse"),
                                float_ptr(slope, a.E + 1, "slope"), float_ptr(gout, 1, "gout"), grad.data_ptr(),
                                cur_stream());
+  g_launches += grad.numel() > 0;
   return grad.unbind(0);
 }
 
@@ -1480,6 +1496,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("preference_loss", &preference_loss);
   m.def("policy_loss", &policy_loss);
   m.def("router_balance_loss", &router_balance_loss);
+  m.def("post_training_launches", [] { return g_launches.load(); });
   m.def("gemm_grouped", &gemm_grouped, py::arg("a"), py::arg("b"), py::arg("b_mn_major"), py::arg("c"),
         py::arg("mode"), py::arg("table"), py::arg("groups"), py::arg("b_rows"), py::arg("alpha"),
         py::arg("beta"), py::arg("status") = py::none());

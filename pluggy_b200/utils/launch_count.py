@@ -17,15 +17,18 @@ KERNELS_PER_CALL = {
     "glu_fwd": 1, "glu_bwd": 1, "cast_f32_bf16": 1, "embedding_fwd": 1, "embedding_bwd": 1,
     "softcap": 1, "ce_rows": 1, "multi_sumsq": 2, "multi_scale": 1, "adamw_multi": 1,
     "attn_fwd": 1, "attn_bwd": 4,
-    # forward kernels; the backward's are launched by the extension's own autograd functions
-    "token_logprobs": 4, "preference_loss": 2, "policy_loss": 2, "router_balance_loss": 2,
+    # counted by the extension, whose own autograd functions launch their backward passes
+    "token_logprobs": 0, "preference_loss": 0, "policy_loss": 0, "router_balance_loss": 0,
+    "post_training_launches": 0,
 }
 
 
 class _Counting:
     def __init__(self, mod):
         self._mod = mod
-        self.count = 0
+        self._count = 0
+        self._start = mod.post_training_launches()
+        self._end: int | None = None  # the extension's count when counting stopped
         self.by_name: dict[str, int] = {}
 
     def __getattr__(self, name):
@@ -35,11 +38,19 @@ class _Counting:
 
         def wrapped(*a, **k):
             n = KERNELS_PER_CALL.get(name, 1)
-            self.count += n
+            self._count += n
             self.by_name[name] = self.by_name.get(name, 0) + n
             return fn(*a, **k)
 
         return wrapped
+
+    @property
+    def count(self) -> int:
+        end = self._mod.post_training_launches() if self._end is None else self._end
+        return self._count + end - self._start
+
+    def stop(self) -> None:
+        self._end = self._mod.post_training_launches()
 
 
 @contextlib.contextmanager
@@ -50,4 +61,5 @@ def count_launches():
     try:
         yield counter
     finally:
+        counter.stop()
         _ext._C = real

@@ -355,3 +355,53 @@ def test_token_mask_argument():
     m(ids, attention_mask=am, token_mask=tm)
     m.aux_loss()
     assert m.last_tokens_per_expert.sum() == (12 + 10) * 4 * 2
+
+
+@GPU
+def test_launch_counts(monkeypatch):
+    """The counted launches are the package's kernels and memsets that the profiler sees, forward and
+    backward."""
+    from torch.profiler import ProfilerActivity, profile
+
+    from pluggy_b200.ops import linear_token_logprobs, logprob, policy_loss, preference_loss, router_balance_loss
+    from pluggy_b200.utils.launch_count import count_launches
+
+    m = torch.ones(2, 3, 40, dtype=torch.bool, device="cuda")
+    x = torch.randn(2, 3, 40, device="cuda").requires_grad_(True)
+    h = torch.randn(300, 64, device="cuda").bfloat16().requires_grad_(True)
+    w = torch.randn(700, 64, device="cuda").bfloat16().requires_grad_(True)
+    y, g = torch.zeros(300, dtype=torch.int64, device="cuda"), torch.ones(300, device="cuda")
+    idx = torch.zeros(300, 2, dtype=torch.int64, device="cuda")
+    ones, one = torch.ones(3, device="cuda"), torch.ones((), device="cuda")
+
+    def logprobs(*wrt, **kw):
+        return lambda: torch.autograd.grad(linear_token_logprobs(h, w, y, **kw), wrt, g)
+
+    def score(n):
+        def run():
+            with torch.no_grad():
+                linear_token_logprobs(h[:n], w, y[:n])
+        return run
+
+    def loss(fn, leaf):
+        return lambda: torch.autograd.grad(fn()[0], leaf, one)
+
+    recompute, keep_all = 1 << 62, 0
+    # kernels and memsets; the last gradient of the head takes three vocabulary ranges
+    cases = [(score(5), 2, 0, recompute), (score(200), 2, 0, recompute), (score(300), 4, 0, recompute),
+             (logprobs(h, w), 9, 1, recompute), (logprobs(h, w), 10, 1, keep_all), (logprobs(h), 7, 0, recompute),
+             (logprobs(w, workspace_bytes=512 * 2 * 256), 5 + 2 * 3, 1, keep_all),
+             (loss(lambda: preference_loss(x, None, m), x), 3, 0, recompute),
+             (loss(lambda: policy_loss(x[0], None, ones, m[0]), x), 3, 0, recompute),
+             (loss(lambda: router_balance_loss(h, idx), h), 3, 0, recompute)]
+    for run, kernels, memsets, keep in cases:
+        monkeypatch.setattr(logprob, "KEEP_PRODUCT", keep)
+        run()
+        torch.cuda.synchronize()
+        with count_launches() as cnt, profile(activities=[ProfilerActivity.CPU, ProfilerActivity.CUDA]) as prof:
+            run()
+            torch.cuda.synchronize()
+        # torch's own kernels live in the namespaces at:: and c10::, and the gradient of x[0] has a memset
+        seen = [e.name for e in prof.events() if e.device_type == torch.autograd.DeviceType.CUDA
+                and not any(s in e.name for s in ("at::", "c10::", "Memcpy", "Memset"))]
+        assert cnt.count == kernels + memsets and len(seen) == kernels, (cnt.count, kernels, memsets, seen)
