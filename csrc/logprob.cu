@@ -1026,8 +1026,10 @@ __device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
 // (and, in y, at eight columns a thread) adds up that label's rows in token order: no atomics.
 // SORTED: tokens come sorted by label (stable), so a label's are neighbours; otherwise every
 // block looks through all labels, which for up to kLabelScanTokens tokens costs less than the
-// sort's launches (with them, D = 256: 10 against 30 us for 777 tokens, 23 against 38 for 2048,
-// 111 against 95 for 8192). Rows and entries are listed a block's width at a time, so that the row loads
+// sort's launches, or little more (us without and with the sort, its launches included:
+// D = 256: 13 and 34 for 1024 tokens, 23 and 39 for 2048, 51 and 48 for 4096, 134 and 84 for 8192;
+// D = 1024: 26 and 37, 56 and 50, 142 and 86 for 2048, 4096 and 8192; D = 2048: 36 and 39, 90 and
+// 53, 250 and 121, where the products of 4096 tokens take a millisecond). Rows and entries are listed a block's width at a time, so that the row loads
 // do not wait for them, and eight rows are fetched at once. Bound by latency: the chain of loads
 // that leads to a row and the longest run (16384 tokens, 300 of them with one label, D = 1024:
 // 90 us; 149 with four columns a thread and the rows' loads left to the compiler).

@@ -69,7 +69,8 @@ __device__ __forceinline__ void load_mask(const uint8_t* p, bool (&m)[VEC]) {
 // Row r = side * P + pair of [2, P, S] tensors. A warp sums up to kMaxWarpTokens of a row, so that
 // few long rows fill the machine as many short ones do; the pairs are joined apart because the
 // loss needs both sides of a pair. Bound by memory: 9 bytes a token with an fp32 reference (511
-// pairs of 8192 tokens, bf16 reference: 59 MB in 21 us, 2.8 TB/s: too short to run at full rate).
+// pairs of 8192 tokens, bf16 reference: 59 MB in 21 us, 2.8 TB/s; a lane's step loads 4 tokens, 4
+// to 16 bytes of each input).
 template <int VEC>
 __global__ void __launch_bounds__(256) pref_sums_kernel(const PrefArgs a, float2* __restrict__ part,
                                                         int chunks, int len, unsigned* __restrict__ ticket) {
@@ -318,7 +319,7 @@ __device__ __forceinline__ void kl_terms(float d, float& em1, float& k3) {
 // OLD, REF, ADV: old log-probabilities, reference and per-token advantages are given (a kernel for
 // each set: 67 us instead of 80 with the choice made per token). Loss and gradient come from one
 // pass, so that nothing is read twice. Bound by memory: 21 bytes a token (1024 x 16384: 352 MB in
-// 66 us, 5.3 TB/s, 0.81 of the measured copy rate).
+// 66 us on one box, 5.3 TB/s, 0.81 of the measured copy rate, and in 75 to 78 on another).
 constexpr int kPolicyResident = 3;
 template <int VEC, bool OLD, bool REF, bool ADV>
 __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const PolicyArgs a, const int* __restrict__ counts,

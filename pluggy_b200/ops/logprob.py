@@ -30,8 +30,9 @@ import torch
 
 from pluggy_b200.ops._ext import ext, status_word
 
-# Bytes of the bf16 matrix, two for each trained token and vocabulary entry, that a call keeps
-# from its forward to its backward, or recomputes at a time
+# Bytes of the bf16 matrix that a call keeps from its forward to its backward, or recomputes at a
+# time: two for each token, rounded up to 256 of them, and vocabulary entry. Ignored tokens are
+# among them, because how many there are is known on the device alone.
 WORKSPACE = 8 << 30
 # tokens * vocabulary * D from which the matrix is kept: below it the product that this saves
 # takes less than 0.1 ms, and recomputing rounds a term of the weight's gradient once less
@@ -83,7 +84,11 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: to
     fp32 ``weight`` is cast, or ``weight_lowp``, its cached bf16 copy, is read instead), and D
     must be a multiple of 8. The gradients have the inputs' types. ``workspace_bytes`` (8 GiB
     when None) bounds the bf16 matrix that a training call keeps for its backward: two bytes for
-    each token and vocabulary entry, recomputed in parts where that is more."""
+    each token, ignored ones included, and vocabulary entry, recomputed in parts where that is
+    more. Not in it: the hidden rows in bf16, kept, too; 16 bytes for each token and 128 to 256
+    vocabulary entries during the forward; in the backward 4 bytes for each token and column of
+    either gradient asked for, and for the hidden states' gradient several such parts, up to
+    512 MiB of them."""
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear_token_logprobs: hidden [..., D] and weight [V, D], got "
                          f"{tuple(hidden.shape)} and {tuple(weight.shape)}")
