@@ -319,7 +319,7 @@ __device__ __forceinline__ void kl_terms(float d, float& em1, float& k3) {
 // OLD, REF, ADV: old log-probabilities, reference and per-token advantages are given (a kernel for
 // each set: 67 us instead of 80 with the choice made per token). Loss and gradient come from one
 // pass, so that nothing is read twice. Bound by memory: 21 bytes a token (1024 x 16384: 352 MB in
-// 66 us on one box, 5.3 TB/s, 0.81 of the measured copy rate, and in 75 to 78 on another).
+// 66 us on one GPU, 5.3 TB/s, 0.81 of the measured copy rate, and in 75 to 78 on another).
 constexpr int kPolicyResident = 3;
 template <int VEC, bool OLD, bool REF, bool ADV>
 __global__ void __launch_bounds__(256, kPolicyResident) policy_kernel(const PolicyArgs a, const int* __restrict__ counts,
