@@ -34,9 +34,10 @@ def before_padding(labels: torch.Tensor, ignore_index: int = -100) -> torch.Tens
 
 
 def token_logprobs(model: nn.Module, ids: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
-                   temperature: float = 1.0):
+                   temperature: float = 1.0, workspace_bytes: int | None = None):
     """``(logps [B, S] fp32, mask [B, S])``: position t holds the log-probability of ``labels[t + 1]``
-    given ``ids[:t + 1]``; the mask is False where that label is ``ignore_index`` and at the end."""
+    given ``ids[:t + 1]``; the mask is False where that label is ``ignore_index`` and at the end.
+    ``workspace_bytes`` is :func:`linear_token_logprobs`'s."""
     core = getattr(model, "module", model)
     for axis in ("tp", "cp"):
         par = getattr(core, axis, None)
@@ -52,7 +53,7 @@ def token_logprobs(model: nn.Module, ids: torch.Tensor, labels: torch.Tensor, ig
     lowp = lowp_fn() if callable(lowp_fn) and hidden.is_cuda else None
     logps = linear_token_logprobs(hidden, core.lm_head.weight, labels, ignore_index, weight_lowp=lowp,
                                   softcap=getattr(core, "final_logit_softcapping", None),
-                                  temperature=temperature)
+                                  temperature=temperature, workspace_bytes=workspace_bytes)
     return logps, labels != ignore_index
 
 
@@ -73,14 +74,16 @@ class PreferenceObjective:
 
     Batch: ``chosen_ids``, ``chosen_labels``, ``rejected_ids``, ``rejected_labels`` [P, S], and
     ``ref_logps`` [2, P, S] from :meth:`score` of the reference model unless ``reference_free``.
-    ``metrics`` holds the last call's mean rewards and the share of pairs ranked right."""
+    ``metrics`` holds the last call's mean rewards and the share of pairs ranked right.
+    ``workspace_bytes`` bounds what a step keeps of its head for the backward (8 GiB when None)."""
 
     KEYS = ("chosen_ids", "chosen_labels", "rejected_ids", "rejected_labels")
     batch_keys = KEYS  # what every batch must hold
 
     def __init__(self, ignore_index: int = -100, beta: float = 0.1, kind: str = "sigmoid",
                  label_smoothing: float = 0.0, length_normalized: bool = False,
-                 reference_free: bool = False):
+                 reference_free: bool = False, workspace_bytes: int | None = None):
+        self.workspace_bytes = workspace_bytes
         self.ignore_index, self.beta, self.kind = ignore_index, beta, kind
         self.label_smoothing, self.length_normalized = label_smoothing, length_normalized
         self.reference_free = reference_free
@@ -90,7 +93,7 @@ class PreferenceObjective:
         _need(batch, self.KEYS, "PREFERENCE")
         ids = torch.cat((batch["chosen_ids"], batch["rejected_ids"]))
         labels = torch.cat((batch["chosen_labels"], batch["rejected_labels"]))
-        lp, mask = token_logprobs(model, ids, labels, self.ignore_index)
+        lp, mask = token_logprobs(model, ids, labels, self.ignore_index, workspace_bytes=self.workspace_bytes)
         shape = (2, *batch["chosen_ids"].shape)
         return lp.view(shape), mask.view(shape)
 
@@ -120,12 +123,15 @@ class PolicyObjective:
     ``advantages`` [R] or [R, S]; ``old_logps`` [R, S] from :meth:`score` of the policy that sampled
     (left out for the first update after sampling); ``ref_logps`` [R, S] where ``kl_coef`` is set.
     [R, S] entries belong to the position that predicts the token, as :meth:`score` gives them.
-    ``metrics`` holds the last call's loss, KL estimate and clipped share."""
+    ``metrics`` holds the last call's loss, KL estimate and clipped share.
+    ``workspace_bytes`` bounds what a step keeps of its head for the backward (8 GiB when None)."""
 
     batch_keys = ("input_ids", "labels", "advantages")  # what every batch must hold
 
     def __init__(self, ignore_index: int = -100, clip_low: float = 0.2, clip_high: float = 0.2,
-                 kl_coef: float = 0.0, reduction: str = "token", temperature: float = 1.0):
+                 kl_coef: float = 0.0, reduction: str = "token", temperature: float = 1.0,
+                 workspace_bytes: int | None = None):
+        self.workspace_bytes = workspace_bytes
         self.ignore_index, self.clip_low, self.clip_high = ignore_index, clip_low, clip_high
         self.kl_coef, self.reduction, self.temperature = kl_coef, reduction, temperature
         self.metrics: dict[str, torch.Tensor] = {}
@@ -135,12 +141,12 @@ class PolicyObjective:
         """``old_logps`` or ``ref_logps`` [R, S] of ``batch`` under ``model``."""
         _need(batch, ("input_ids", "labels"), "POLICY")
         return token_logprobs(model, batch["input_ids"], batch["labels"], self.ignore_index,
-                              self.temperature)[0]
+                              self.temperature, self.workspace_bytes)[0]
 
     def compute_loss(self, model: nn.Module, batch: dict[str, torch.Tensor]) -> torch.Tensor:
         _need(batch, self.batch_keys + (("ref_logps",) if self.kl_coef else ()), "POLICY")
         lp, mask = token_logprobs(model, batch["input_ids"], batch["labels"], self.ignore_index,
-                                  self.temperature)
+                                  self.temperature, self.workspace_bytes)
         loss, kl, clipped = policy_loss(
             lp, batch.get("old_logps"), batch["advantages"], mask, ref_logps=batch.get("ref_logps"),
             clip_low=self.clip_low, clip_high=self.clip_high, kl_coef=self.kl_coef,

@@ -1,5 +1,6 @@
 """The post-training objectives on models, and the MoE model's fused router losses."""
 
+import gc
 import importlib.util
 import os
 
@@ -405,3 +406,34 @@ def test_launch_counts(monkeypatch):
         seen = [e.name for e in prof.events() if e.device_type == torch.autograd.DeviceType.CUDA
                 and not any(s in e.name for s in ("at::", "c10::", "Memcpy", "Memset"))]
         assert cnt.count == kernels + memsets and len(seen) == kernels, (cnt.count, kernels, memsets, seen)
+
+
+@GPU
+@pytest.mark.parametrize("name", ["PREFERENCE", "POLICY"])
+def test_objectives_bound_what_they_keep(name, monkeypatch):
+    """``workspace_bytes`` reaches the head: a step that keeps nothing holds less until its backward,
+    and its gradients are the same up to the kept rows' rounding."""
+    from pluggy_b200.ops import logprob
+
+    monkeypatch.setattr(logprob, "KEEP_PRODUCT", 0)
+    V = 4000
+    m = small(dev="cuda", vocab_size=V)
+    b = pairs("cuda", P=4, S=512, V=V)
+    batch = b if name == "PREFERENCE" else {"input_ids": b["chosen_ids"].repeat(2, 1),
+                                            "labels": b["chosen_labels"].repeat(2, 1),
+                                            "advantages": torch.linspace(-1, 1, 8, device="cuda")}
+    held, grads = [], []
+    for ws in (None, 1 << 20):
+        cfg = dict(workspace_bytes=ws, **(dict(reference_free=True) if name == "PREFERENCE" else {}))
+        obj = build_objective(name, cfg)
+        obj.compute_loss(m, batch)  # caches and workspaces of a first call
+        gc.collect()
+        before = torch.cuda.memory_allocated()
+        loss = obj.compute_loss(m, batch)
+        held.append(torch.cuda.memory_allocated() - before)
+        grads.append(torch.autograd.grad(loss, m.lm_head.weight)[0])
+        del loss
+    kept = 2 * 8 * 512 * V  # bytes of the matrix
+    assert held[0] - held[1] >= kept - (2 << 20)
+    # c_t h_t is rounded to bf16 once more (2^-8 of a term); the passes' hidden states differ in bf16's last bits
+    assert (grads[0] - grads[1]).norm() <= 2.0 ** -6 * grads[1].norm()
