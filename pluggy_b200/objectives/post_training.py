@@ -28,9 +28,11 @@ from pluggy_b200.ops.preference import preference_loss
 
 def before_padding(labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
     """bool [B, S]: positions up to each row's last label."""
+    kept = labels != ignore_index
+    if labels.shape[1] == 0:
+        return kept
     at = torch.arange(1, labels.shape[1] + 1, device=labels.device)
-    last = torch.where(labels != ignore_index, at, 0).amax(1, keepdim=True) if labels.shape[1] else at
-    return at <= last
+    return at <= torch.where(kept, at, 0).amax(1, keepdim=True)
 
 
 def token_logprobs(model: nn.Module, ids: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,

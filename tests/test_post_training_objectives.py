@@ -437,3 +437,13 @@ def test_objectives_bound_what_they_keep(name, monkeypatch):
     assert held[0] - held[1] >= kept - (2 << 20)
     # c_t h_t is rounded to bf16 once more (2^-8 of a term); the passes' hidden states differ in bf16's last bits
     assert (grads[0] - grads[1]).norm() <= 2.0 ** -6 * grads[1].norm()
+
+
+def test_before_padding():
+    from pluggy_b200.objectives.post_training import before_padding
+
+    y = torch.tensor([[IGN, 5, IGN, 7, IGN], [IGN] * 5, [1, 2, 3, 4, 0], [9, IGN, IGN, IGN, IGN]])
+    assert before_padding(y).sum(1).tolist() == [4, 0, 5, 1]
+    assert before_padding(y)[0].tolist() == [True] * 4 + [False]
+    assert before_padding(y, 0)[2].tolist() == [True] * 4 + [False]
+    assert before_padding(y[:, :0]).shape == (4, 0)
