@@ -189,8 +189,6 @@ def router_z_loss(router_logits, token_mask=None):
 
 
 class Qwen3Moe(nn.Module):
-    takes_token_mask = True  # forward(token_mask=...)
-
     def __init__(self, num_layers: int, num_heads: int, num_kv_heads: int, emb_dim: int,
                  head_dim: int, vocab_size: int, moe_ffn_dim: int, num_experts: int = 128,
                  top_k: int = 8, ffn_dim: int | None = None, norm_topk_prob: bool = True,

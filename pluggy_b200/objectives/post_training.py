@@ -6,7 +6,7 @@ Both read per-token log-probabilities of the model's own head
 right-padded: under causal attention nothing before the padding sees it, so the packed
 forward serves them, and padded positions carry ``ignore_index`` labels. What follows a
 sequence's last label is taken for padding and counts neither in the router losses nor in
-the experts' token counts (models with ``takes_token_mask``).
+the experts' token counts (models whose ``forward`` takes a ``token_mask``).
 
 The data sources of the trainer make no such batches, so its config check refuses these
 objectives: a program calls them from its own loop (``examples/post_training.py``).
@@ -16,6 +16,8 @@ model's, or the policy's before its update.
 """
 
 from __future__ import annotations
+
+import inspect
 
 import torch
 import torch.nn as nn
@@ -48,7 +50,8 @@ def token_logprobs(model: nn.Module, ids: torch.Tensor, labels: torch.Tensor, ig
     if ids.shape != labels.shape or ids.dim() != 2:
         raise ValueError(f"ids and labels must be [B, S] alike, got {tuple(ids.shape)} and "
                          f"{tuple(labels.shape)}")
-    kw = {"token_mask": before_padding(labels, ignore_index)} if getattr(core, "takes_token_mask", False) else {}
+    masks = "token_mask" in inspect.signature(core.forward).parameters
+    kw = {"token_mask": before_padding(labels, ignore_index)} if masks else {}
     hidden = model(ids, return_final_hidden=True, **kw)
     labels = shift_labels(labels, ignore_index)
     lowp_fn = getattr(core, "lm_head_lowp", None)

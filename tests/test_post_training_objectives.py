@@ -447,3 +447,21 @@ def test_before_padding():
     assert before_padding(y)[0].tolist() == [True] * 4 + [False]
     assert before_padding(y, 0)[2].tolist() == [True] * 4 + [False]
     assert before_padding(y[:, :0]).shape == (4, 0)
+
+
+def test_models_without_a_token_mask():
+    """A model whose forward has no token_mask, a MoE subclass with the older signature among them,
+    runs as it did."""
+    from pluggy_b200.models.qwen3_moe import Qwen3Moe
+
+    class Own(Qwen3Moe):
+        def forward(self, x, attention_mask=None, return_hidden_states=False, return_final_hidden=False,
+                    position_ids=None):
+            return super().forward(x, attention_mask, return_hidden_states, return_final_hidden, position_ids)
+
+    torch.manual_seed(0)
+    m = Own(num_layers=1, num_heads=2, num_kv_heads=1, emb_dim=128, head_dim=64, vocab_size=200, moe_ffn_dim=128,
+            num_experts=8, top_k=2)
+    m.init_weights()
+    build_objective("PREFERENCE", dict(reference_free=True)).compute_loss(m, pairs("cpu"))
+    assert m.last_tokens_per_expert.sum() == 6 * 128 * 2
