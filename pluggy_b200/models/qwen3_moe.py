@@ -164,10 +164,12 @@ def load_balancing_loss(router_logits, num_experts: int, top_k: int, token_mask=
     if not router_logits:
         return torch.tensor(0.0)
     logits = torch.cat([g.float() for g in router_logits], dim=0)
+    if token_mask is not None:
+        keep = token_mask.repeat(len(router_logits))
+        logits = torch.where(keep.unsqueeze(1), logits, 0.0)
     probs = F.softmax(logits, dim=-1)
     _, top = torch.topk(probs, top_k, dim=-1)
     if token_mask is not None:
-        keep = token_mask.repeat(len(router_logits))
         n = keep.sum().clamp_min(1)
         mean = torch.where(keep.unsqueeze(1), probs, 0.0).sum(dim=0) / n
         return (_masked_histogram(top, num_experts, keep).float() / n * mean).sum() * num_experts
@@ -183,7 +185,7 @@ def router_z_loss(router_logits, token_mask=None):
     logits = torch.cat([g.float() for g in router_logits], dim=0)
     if token_mask is not None:
         keep = token_mask.repeat(len(router_logits))
-        z = torch.square(torch.logsumexp(logits, dim=-1))
+        z = torch.square(torch.logsumexp(torch.where(keep.unsqueeze(1), logits, 0.0), dim=-1))
         return torch.where(keep, z, 0.0).sum() / keep.sum().clamp_min(1)
     return torch.square(torch.logsumexp(logits, dim=-1)).mean()
 

@@ -465,3 +465,16 @@ def test_models_without_a_token_mask():
     m.init_weights()
     build_objective("PREFERENCE", dict(reference_free=True)).compute_loss(m, pairs("cpu"))
     assert m.last_tokens_per_expert.sum() == 6 * 128 * 2
+
+
+def test_masked_router_rows_may_hold_anything():
+    from pluggy_b200.models.qwen3_moe import load_balancing_loss, router_z_loss
+
+    keep = torch.tensor([True, False, True, False, True])
+    x = torch.randn(5, 8, generator=torch.Generator().manual_seed(0))
+    want = load_balancing_loss([x[keep]] * 2, 8, 2) + router_z_loss([x[keep]] * 2)
+    x[~keep] = float("nan")
+    x.requires_grad_(True)
+    got = load_balancing_loss([x] * 2, 8, 2, keep) + router_z_loss([x] * 2, keep)
+    (g,) = torch.autograd.grad(got, x)
+    assert abs(got - want) <= 1e-6 * want and (g[~keep] == 0).all() and torch.isfinite(g).all()
